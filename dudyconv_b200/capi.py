@@ -66,6 +66,20 @@ SIGNATURES = {
                                       + [_i64] * 8 + [_int, _int, _vp]),
     "dudy_fdc_exchange_finish": (_int, [ctypes.POINTER(PeerExchange), _vp, _i64, _i64, _int, _vp]),
     "dudy_logits_to_kernel_backward": (_int, [_vp] * 3 + [_i64] * 4 + [_int, _vp]),
+    "dudy_short_conv_forward": (_int, [_vp] * 7 + [_i64] * 4 + [_int, _int, _vp]),
+    "dudy_short_conv_backward_workspace_size": (_sz, [_i64] * 4 + [_int]),
+    "dudy_short_conv_backward": (_int, [_vp] * 12 + [_sz] + [_i64] * 4 + [_int, _int, _vp]),
+    "dudy_short_conv_step": (_int, [_vp] * 5 + [_i64] * 3 + [_int, _int, _vp]),
+    "dudy_selective_scan_checkpoint_bytes": (_sz, [_i64] * 5 + [_int]),
+    "dudy_selective_scan_forward_workspace_size": (_sz, [_i64] * 5 + [_int]),
+    "dudy_selective_scan_forward": (_int, [_vp] * 13 + [_sz] + [_i64] * 5 + [_int, _int, _vp]),
+    "dudy_selective_scan_backward_workspace_size": (_sz, [_i64] * 5 + [_int]),
+    "dudy_selective_scan_backward": (_int, [_vp] * 20 + [_sz] + [_i64] * 5 + [_int, _int, _vp]),
+    "dudy_selective_scan_step": (_int, [_vp] * 9 + [_i64] * 4 + [_int, _int, _vp]),
+    "dudy_block_norm_forward": (_int, [_vp] * 11 + [_i64] * 3 + [_int, ctypes.c_float, _int, _int,
+                                                                 _vp]),
+    "dudy_block_norm_backward_workspace_size": (_sz, [_i64] * 3 + [_int, _int]),
+    "dudy_block_norm_backward": (_int, [_vp] * 19 + [_sz] + [_i64] * 3 + [_int, _int, _int, _vp]),
 }
 
 _LIB = None
@@ -286,3 +300,124 @@ def fdc_exchange_finish(xchg: PeerExchange, grad_mix, stream=None):
     D, N = grad_mix.shape
     _check(lib().dudy_fdc_exchange_finish(ctypes.byref(xchg), _ptr(grad_mix), D, N,
                                           dtype_code(grad_mix), _stream(stream)))
+
+
+def _ws_bytes(workspace) -> int:
+    return 0 if workspace is None else workspace.numel() * workspace.element_size()
+
+
+def short_conv_forward(x, weight, bias, state, lengths, out, final_state=None, silu: bool = True,
+                       stream=None):
+    """Short causal depthwise conv; bias, state, lengths and final_state may be None."""
+    B, D, L = x.shape
+    _check(lib().dudy_short_conv_forward(_ptr(x), _ptr(weight), _ptr(bias), _ptr(state),
+                                         _ptr(lengths), _ptr(out), _ptr(final_state), B, D, L,
+                                         weight.shape[1], int(silu), dtype_code(x),
+                                         _stream(stream)))
+
+
+def short_conv_backward_workspace_size(x, weight) -> int:
+    B, D, L = x.shape
+    return int(lib().dudy_short_conv_backward_workspace_size(B, D, L, weight.shape[1],
+                                                             dtype_code(x)))
+
+
+def short_conv_backward(go, grad_final, x, weight, bias, state, lengths, grad_x, grad_weight,
+                        grad_bias, grad_state, workspace, silu: bool = True, stream=None):
+    B, D, L = x.shape
+    _check(lib().dudy_short_conv_backward(
+        _ptr(go), _ptr(grad_final), _ptr(x), _ptr(weight), _ptr(bias), _ptr(state),
+        _ptr(lengths), _ptr(grad_x), _ptr(grad_weight), _ptr(grad_bias), _ptr(grad_state),
+        _ptr(workspace), _ws_bytes(workspace), B, D, L, weight.shape[1], int(silu),
+        dtype_code(x), _stream(stream)))
+
+
+def short_conv_step(x, state, weight, bias, out, silu: bool = True, stream=None):
+    """One token per sequence; state [B,D,S-1] is updated in place."""
+    B, D = x.shape
+    _check(lib().dudy_short_conv_step(_ptr(x), _ptr(state), _ptr(weight), _ptr(bias), _ptr(out),
+                                      B, D, weight.shape[1], int(silu), dtype_code(x),
+                                      _stream(stream)))
+
+
+def _scan_dims(u, A, Bm):
+    B, D, L = u.shape
+    return B, D, L, A.shape[1], Bm.shape[1]
+
+
+def selective_scan_checkpoint_bytes(u, A, Bm) -> int:
+    return int(lib().dudy_selective_scan_checkpoint_bytes(*_scan_dims(u, A, Bm), dtype_code(u)))
+
+
+def selective_scan_forward_workspace_size(u, A, Bm) -> int:
+    return int(lib().dudy_selective_scan_forward_workspace_size(*_scan_dims(u, A, Bm),
+                                                                dtype_code(u)))
+
+
+def selective_scan_forward(u, delta, A, Bm, Cm, skip, delta_bias, state, lengths, y,
+                           final_state=None, checkpoints=None, workspace=None,
+                           softplus: bool = True, stream=None):
+    """Selective scan; skip, delta_bias, state, lengths, final_state, checkpoints may be None."""
+    _check(lib().dudy_selective_scan_forward(
+        _ptr(u), _ptr(delta), _ptr(A), _ptr(Bm), _ptr(Cm), _ptr(skip), _ptr(delta_bias),
+        _ptr(state), _ptr(lengths), _ptr(y), _ptr(final_state), _ptr(checkpoints),
+        _ptr(workspace), _ws_bytes(workspace), *_scan_dims(u, A, Bm), int(softplus),
+        dtype_code(u), _stream(stream)))
+
+
+def selective_scan_backward_workspace_size(u, A, Bm) -> int:
+    return int(lib().dudy_selective_scan_backward_workspace_size(*_scan_dims(u, A, Bm),
+                                                                 dtype_code(u)))
+
+
+def selective_scan_backward(go, grad_final, u, delta, A, Bm, Cm, skip, delta_bias, checkpoints,
+                            lengths, grad_u, grad_delta, grad_A, grad_B, grad_C, grad_skip,
+                            grad_delta_bias, grad_state, workspace, softplus: bool = True,
+                            stream=None):
+    _check(lib().dudy_selective_scan_backward(
+        _ptr(go), _ptr(grad_final), _ptr(u), _ptr(delta), _ptr(A), _ptr(Bm), _ptr(Cm),
+        _ptr(skip), _ptr(delta_bias), _ptr(checkpoints), _ptr(lengths), _ptr(grad_u),
+        _ptr(grad_delta), _ptr(grad_A), _ptr(grad_B), _ptr(grad_C), _ptr(grad_skip),
+        _ptr(grad_delta_bias), _ptr(grad_state), _ptr(workspace), _ws_bytes(workspace),
+        *_scan_dims(u, A, Bm), int(softplus), dtype_code(u), _stream(stream)))
+
+
+def selective_scan_step(u, delta, A, Bm, Cm, skip, delta_bias, state, y, softplus: bool = True,
+                        stream=None):
+    """One token per sequence; state [B,D,N] (fp32) is updated in place."""
+    B, D = u.shape
+    _check(lib().dudy_selective_scan_step(
+        _ptr(u), _ptr(delta), _ptr(A), _ptr(Bm), _ptr(Cm), _ptr(skip), _ptr(delta_bias),
+        _ptr(state), _ptr(y), B, D, A.shape[1], Bm.shape[1], int(softplus), dtype_code(u),
+        _stream(stream)))
+
+
+def block_norm_forward(x, gate, residual, post_weight, post_bias, scale, pre_weight, pre_bias, y,
+                       residual_out, stats=None, layer: bool = False, eps: float = 1e-5,
+                       stream=None):
+    """Norms after and before a block with gate and scaled residual; optional inputs None."""
+    B, D, L = x.shape
+    _check(lib().dudy_block_norm_forward(
+        _ptr(x), _ptr(gate), _ptr(residual), _ptr(post_weight), _ptr(post_bias), _ptr(scale),
+        _ptr(pre_weight), _ptr(pre_bias), _ptr(y), _ptr(residual_out), _ptr(stats), B, D, L,
+        int(layer), eps, dtype_code(x), dtype_code(residual), _stream(stream)))
+
+
+def block_norm_backward_workspace_size(x, residual) -> int:
+    B, D, L = x.shape
+    return int(lib().dudy_block_norm_backward_workspace_size(B, D, L, dtype_code(x),
+                                                             dtype_code(residual)))
+
+
+def block_norm_backward(grad_y, grad_residual_out, x, gate, residual, post_weight, post_bias,
+                        scale, pre_weight, stats, grad_x, grad_gate, grad_residual,
+                        grad_post_weight, grad_post_bias, grad_scale, grad_pre_weight,
+                        grad_pre_bias, workspace, layer: bool = False, stream=None):
+    B, D, L = x.shape
+    _check(lib().dudy_block_norm_backward(
+        _ptr(grad_y), _ptr(grad_residual_out), _ptr(x), _ptr(gate), _ptr(residual),
+        _ptr(post_weight), _ptr(post_bias), _ptr(scale), _ptr(pre_weight), _ptr(stats),
+        _ptr(grad_x), _ptr(grad_gate), _ptr(grad_residual), _ptr(grad_post_weight),
+        _ptr(grad_post_bias), _ptr(grad_scale), _ptr(grad_pre_weight), _ptr(grad_pre_bias),
+        _ptr(workspace), _ws_bytes(workspace), B, D, L, int(layer), dtype_code(x),
+        dtype_code(residual), _stream(stream)))

@@ -540,6 +540,308 @@ torch::Tensor logits_to_kernel_backward(torch::Tensor kc, torch::Tensor grad_kc)
   return gl;
 }
 
+// ---------------------------------------------------------------------------------------
+// state-space block (no counterpart in the reference): short causal conv, selective scan, and
+// the norms, gate and residual between blocks. Optional tensors come as None.
+// ---------------------------------------------------------------------------------------
+using OptTensor = c10::optional<torch::Tensor>;
+
+const void *opt_ptr(const OptTensor &t) { return t.has_value() ? t->data_ptr() : nullptr; }
+
+// A [..] tensor of `like`'s device and of type `dt`, with the given sizes
+void check_like(const torch::Tensor &t, const char *name, at::IntArrayRef sizes,
+                at::ScalarType dt, const torch::Tensor &like) {
+  TORCH_CHECK(t.is_cuda(), name, " must be CUDA tensor.");
+  TORCH_CHECK(t.device() == like.device(), "all tensors must be on the same device.");
+  TORCH_CHECK(t.sizes() == sizes, name, " must be ", sizes, ", got ", t.sizes(), ".");
+  TORCH_CHECK(t.scalar_type() == dt, name, " must be ", dt, ", got ", t.scalar_type(), ".");
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous.");
+}
+
+void check_like(const OptTensor &t, const char *name, at::IntArrayRef sizes, at::ScalarType dt,
+                const torch::Tensor &like) {
+  if (t.has_value()) check_like(*t, name, sizes, dt, like);
+}
+
+torch::Tensor scratch(size_t bytes, const torch::Tensor &like) {
+  return torch::empty({(int64_t)std::max<size_t>(bytes, 16)}, like.options().dtype(torch::kUInt8));
+}
+
+torch::Tensor floats(at::IntArrayRef sizes, const torch::Tensor &like) {
+  return torch::empty(sizes, like.options().dtype(torch::kFloat32));
+}
+
+void check_seq(const torch::Tensor &x, const char *name) {
+  TORCH_CHECK(x.is_cuda(), name, " must be CUDA tensor.");
+  TORCH_CHECK(x.dim() == 3, name, " must be [B,D,L], got ", x.sizes(), ".");
+  TORCH_CHECK(x.is_contiguous(), name, " must be contiguous.");
+  TORCH_CHECK(x.numel() > 0, "B, D and L must be positive.");
+  dtype_code(x);
+}
+
+void check_short_conv(const torch::Tensor &x, const torch::Tensor &w, const OptTensor &bias,
+                      const OptTensor &state, const OptTensor &lengths) {
+  check_seq(x, "x");
+  TORCH_CHECK(w.dim() == 2, "weight must be [D,S], got ", w.sizes(), ".");
+  const int64_t B = x.size(0), D = x.size(1), S = w.size(1);
+  TORCH_CHECK(S >= 2 && S <= DUDY_SHORT_CONV_MAX_TAPS, "S must be between 2 and ",
+              DUDY_SHORT_CONV_MAX_TAPS, ", got ", S, ".");
+  check_like(w, "weight", {D, S}, x.scalar_type(), x);
+  check_like(bias, "bias", {D}, x.scalar_type(), x);
+  check_like(state, "initial_state", {B, D, S - 1}, x.scalar_type(), x);
+  check_like(lengths, "lengths", {B}, at::kInt, x);
+}
+
+std::vector<torch::Tensor> short_conv_forward(torch::Tensor x, torch::Tensor w, OptTensor bias,
+                                              OptTensor state, OptTensor lengths, bool silu,
+                                              bool want_final) {
+  check_short_conv(x, w, bias, state, lengths);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t B = x.size(0), D = x.size(1), L = x.size(2), S = w.size(1);
+  std::vector<torch::Tensor> out{torch::empty_like(x)};
+  if (want_final) out.push_back(torch::empty({B, D, S - 1}, x.options()));
+  check_status(dudy_short_conv_forward(
+                   x.data_ptr(), w.data_ptr(), opt_ptr(bias), opt_ptr(state),
+                   (const int32_t *)opt_ptr(lengths), out[0].data_ptr(),
+                   want_final ? out[1].data_ptr() : nullptr, B, D, L, S, silu, dtype_code(x),
+                   stream_ptr()),
+               "fused_short_conv forward");
+  return out;
+}
+
+// grad_x, grad_weight, grad_bias (empty without a bias), grad_state (empty unless wanted)
+std::vector<torch::Tensor> short_conv_backward(torch::Tensor go, OptTensor gfinal,
+                                               torch::Tensor x, torch::Tensor w, OptTensor bias,
+                                               OptTensor state, OptTensor lengths, bool silu,
+                                               bool want_state) {
+  check_short_conv(x, w, bias, state, lengths);
+  const int64_t B = x.size(0), D = x.size(1), L = x.size(2), S = w.size(1);
+  check_like(go, "grad_out", x.sizes(), x.scalar_type(), x);
+  check_like(gfinal, "grad_final_state", {B, D, S - 1}, x.scalar_type(), x);
+  const c10::cuda::CUDAGuard guard(x.device());
+  auto gx = torch::empty_like(x), gw = torch::empty_like(w);
+  auto gb = torch::empty({bias.has_value() ? D : 0}, x.options());
+  auto gs = want_state ? torch::empty({B, D, S - 1}, x.options()) : torch::empty({0}, x.options());
+  const int dt = dtype_code(x);
+  auto ws = scratch(dudy_short_conv_backward_workspace_size(B, D, L, S, dt), x);
+  check_status(dudy_short_conv_backward(
+                   go.data_ptr(), opt_ptr(gfinal), x.data_ptr(), w.data_ptr(), opt_ptr(bias),
+                   opt_ptr(state), (const int32_t *)opt_ptr(lengths), gx.data_ptr(),
+                   gw.data_ptr(), bias.has_value() ? gb.data_ptr() : nullptr,
+                   want_state ? gs.data_ptr() : nullptr, ws.data_ptr(), (size_t)ws.numel(), B, D,
+                   L, S, silu, dt, stream_ptr()),
+               "fused_short_conv backward");
+  return {gx, gw, gb, gs};
+}
+
+torch::Tensor short_conv_step(torch::Tensor x, torch::Tensor state, torch::Tensor w,
+                              OptTensor bias, bool silu) {
+  TORCH_CHECK(x.is_cuda(), "x must be CUDA tensor.");
+  TORCH_CHECK(x.dim() == 2 && x.numel() > 0, "x must be [B,D], got ", x.sizes(), ".");
+  TORCH_CHECK(x.is_contiguous(), "x must be contiguous.");
+  TORCH_CHECK(w.dim() == 2, "weight must be [D,S], got ", w.sizes(), ".");
+  const int64_t B = x.size(0), D = x.size(1), S = w.size(1);
+  const int dt = dtype_code(x);
+  check_like(w, "weight", {D, S}, x.scalar_type(), x);
+  check_like(bias, "bias", {D}, x.scalar_type(), x);
+  check_like(state, "conv_state", {B, D, S - 1}, x.scalar_type(), x);
+  const c10::cuda::CUDAGuard guard(x.device());
+  auto out = torch::empty_like(x);
+  check_status(dudy_short_conv_step(x.data_ptr(), state.data_ptr(), w.data_ptr(), opt_ptr(bias),
+                                    out.data_ptr(), B, D, S, silu, dt, stream_ptr()),
+               "fused_short_conv step");
+  return out;
+}
+
+struct ScanDims {
+  int64_t B, D, L, N, G;
+};
+
+// u is [B,D,L] (L given) or [B,D] (L = 0: one token)
+ScanDims check_scan(const torch::Tensor &u, const torch::Tensor &delta, const torch::Tensor &A,
+                    const torch::Tensor &Bm, const torch::Tensor &Cm, const OptTensor &skip,
+                    const OptTensor &bias, bool token) {
+  if (token) {
+    TORCH_CHECK(u.is_cuda(), "u must be CUDA tensor.");
+    TORCH_CHECK(u.dim() == 2 && u.numel() > 0, "u must be [B,D], got ", u.sizes(), ".");
+    TORCH_CHECK(u.is_contiguous(), "u must be contiguous.");
+    dtype_code(u);
+  } else {
+    check_seq(u, "u");
+  }
+  TORCH_CHECK(A.dim() == 2, "A must be [D,N], got ", A.sizes(), ".");
+  TORCH_CHECK(Bm.dim() == u.dim() + 1, token ? "B must be [B,G,N], got " : "B must be [B,G,N,L], got ",
+              Bm.sizes(), ".");
+  const ScanDims d{u.size(0), u.size(1), token ? 1 : u.size(2), A.size(1), Bm.size(1)};
+  TORCH_CHECK(d.N >= 1 && d.N <= DUDY_SCAN_MAX_STATE, "N must be between 1 and ",
+              DUDY_SCAN_MAX_STATE, ", got ", d.N, ".");
+  TORCH_CHECK(d.G > 0 && d.D % d.G == 0, "D must be a multiple of the number of groups, got D=",
+              d.D, ", G=", d.G, ".");
+  const auto dt = u.scalar_type();
+  check_like(delta, "delta", u.sizes(), dt, u);
+  check_like(A, "A", {d.D, d.N}, at::kFloat, u);
+  std::vector<int64_t> bc{d.B, d.G, d.N};
+  if (!token) bc.push_back(d.L);
+  check_like(Bm, "B", bc, dt, u);
+  check_like(Cm, "C", bc, dt, u);
+  check_like(skip, "skip", {d.D}, at::kFloat, u);
+  check_like(bias, "delta_bias", {d.D}, at::kFloat, u);
+  return d;
+}
+
+// y, final_state (empty unless wanted), checkpoints (empty unless wanted)
+std::vector<torch::Tensor> selective_scan_forward(torch::Tensor u, torch::Tensor delta,
+                                                  torch::Tensor A, torch::Tensor Bm,
+                                                  torch::Tensor Cm, OptTensor skip,
+                                                  OptTensor bias, OptTensor state,
+                                                  OptTensor lengths, bool softplus,
+                                                  bool want_final, bool want_ckpt) {
+  const ScanDims d = check_scan(u, delta, A, Bm, Cm, skip, bias, false);
+  check_like(state, "initial_state", {d.B, d.D, d.N}, at::kFloat, u);
+  check_like(lengths, "lengths", {d.B}, at::kInt, u);
+  const c10::cuda::CUDAGuard guard(u.device());
+  const int dt = dtype_code(u);
+  auto y = torch::empty_like(u);
+  auto fin = want_final ? floats({d.B, d.D, d.N}, u) : torch::Tensor();
+  auto ck = want_ckpt
+                ? scratch(dudy_selective_scan_checkpoint_bytes(d.B, d.D, d.L, d.N, d.G, dt), u)
+                : torch::Tensor();
+  const size_t ws_bytes =
+      dudy_selective_scan_forward_workspace_size(d.B, d.D, d.L, d.N, d.G, dt);
+  auto ws = ws_bytes ? scratch(ws_bytes, u) : torch::Tensor();
+  check_status(dudy_selective_scan_forward(
+                   u.data_ptr(), delta.data_ptr(), (const float *)A.data_ptr(), Bm.data_ptr(),
+                   Cm.data_ptr(), (const float *)opt_ptr(skip), (const float *)opt_ptr(bias),
+                   (const float *)opt_ptr(state), (const int32_t *)opt_ptr(lengths), y.data_ptr(),
+                   want_final ? (float *)fin.data_ptr() : nullptr,
+                   want_ckpt ? (float *)ck.data_ptr() : nullptr,
+                   ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, d.B, d.D, d.L, d.N, d.G,
+                   softplus, dt, stream_ptr()),
+               "fused_selective_scan forward");
+  return {y, fin, ck};
+}
+
+// grad u, delta, A, B, C, skip, delta_bias, state (undefined where there is no such input)
+std::vector<torch::Tensor> selective_scan_backward(torch::Tensor go, OptTensor gfinal,
+                                                   torch::Tensor u, torch::Tensor delta,
+                                                   torch::Tensor A, torch::Tensor Bm,
+                                                   torch::Tensor Cm, OptTensor skip,
+                                                   OptTensor bias, torch::Tensor ckpt,
+                                                   OptTensor lengths, bool softplus,
+                                                   bool want_state) {
+  const ScanDims d = check_scan(u, delta, A, Bm, Cm, skip, bias, false);
+  check_like(go, "grad_out", u.sizes(), u.scalar_type(), u);
+  check_like(gfinal, "grad_final_state", {d.B, d.D, d.N}, at::kFloat, u);
+  check_like(lengths, "lengths", {d.B}, at::kInt, u);
+  const int dt = dtype_code(u);
+  TORCH_CHECK(ckpt.is_cuda() && ckpt.device() == u.device() &&
+                  (size_t)ckpt.nbytes() >=
+                      dudy_selective_scan_checkpoint_bytes(d.B, d.D, d.L, d.N, d.G, dt),
+              "checkpoints do not belong to these inputs.");
+  const c10::cuda::CUDAGuard guard(u.device());
+  auto gu = torch::empty_like(u), gd = torch::empty_like(u), gA = torch::empty_like(A);
+  auto gB = torch::empty_like(Bm), gC = torch::empty_like(Cm);
+  auto gs = skip.has_value() ? floats({d.D}, u) : torch::Tensor();
+  auto gb = bias.has_value() ? floats({d.D}, u) : torch::Tensor();
+  auto gst = want_state ? floats({d.B, d.D, d.N}, u) : torch::Tensor();
+  auto ws = scratch(dudy_selective_scan_backward_workspace_size(d.B, d.D, d.L, d.N, d.G, dt), u);
+  auto fp = [](const torch::Tensor &t) { return t.defined() ? (float *)t.data_ptr() : nullptr; };
+  check_status(dudy_selective_scan_backward(
+                   go.data_ptr(), (const float *)opt_ptr(gfinal), u.data_ptr(), delta.data_ptr(),
+                   (const float *)A.data_ptr(), Bm.data_ptr(), Cm.data_ptr(),
+                   (const float *)opt_ptr(skip), (const float *)opt_ptr(bias),
+                   (const float *)ckpt.data_ptr(), (const int32_t *)opt_ptr(lengths),
+                   gu.data_ptr(), gd.data_ptr(), (float *)gA.data_ptr(), gB.data_ptr(),
+                   gC.data_ptr(), fp(gs), fp(gb), fp(gst), ws.data_ptr(), (size_t)ws.numel(), d.B,
+                   d.D, d.L, d.N, d.G, softplus, dt, stream_ptr()),
+               "fused_selective_scan backward");
+  return {gu, gd, gA, gB, gC, gs, gb, gst};
+}
+
+torch::Tensor selective_scan_step(torch::Tensor u, torch::Tensor delta, torch::Tensor A,
+                                  torch::Tensor Bm, torch::Tensor Cm, torch::Tensor state,
+                                  OptTensor skip, OptTensor bias, bool softplus) {
+  const ScanDims d = check_scan(u, delta, A, Bm, Cm, skip, bias, true);
+  check_like(state, "state", {d.B, d.D, d.N}, at::kFloat, u);
+  const c10::cuda::CUDAGuard guard(u.device());
+  auto y = torch::empty_like(u);
+  check_status(dudy_selective_scan_step(
+                   u.data_ptr(), delta.data_ptr(), (const float *)A.data_ptr(), Bm.data_ptr(),
+                   Cm.data_ptr(), (const float *)opt_ptr(skip), (const float *)opt_ptr(bias),
+                   (float *)state.data_ptr(), y.data_ptr(), d.B, d.D, d.N, d.G, softplus,
+                   dtype_code(u), stream_ptr()),
+               "fused_selective_scan step");
+  return y;
+}
+
+void check_block_norm(const torch::Tensor &x, const torch::Tensor &residual,
+                      const OptTensor &gate, const torch::Tensor &w1, const OptTensor &b1,
+                      const OptTensor &scale, const torch::Tensor &w2, const OptTensor &b2) {
+  check_seq(x, "x");
+  const auto dt = x.scalar_type();
+  TORCH_CHECK(residual.scalar_type() == dt || residual.scalar_type() == at::kFloat,
+              "residual must be of x's type or float32, got ", residual.scalar_type(), ".");
+  check_like(residual, "residual", x.sizes(), residual.scalar_type(), x);
+  check_like(gate, "gate", x.sizes(), dt, x);
+  const int64_t D = x.size(1);
+  check_like(w1, "post_weight", {D}, dt, x);
+  check_like(b1, "post_bias", {D}, dt, x);
+  check_like(scale, "scale", {D}, dt, x);
+  check_like(w2, "pre_weight", {D}, dt, x);
+  check_like(b2, "pre_bias", {D}, dt, x);
+}
+
+// y, residual_out, stats (undefined unless wanted)
+std::vector<torch::Tensor> block_norm_forward(torch::Tensor x, torch::Tensor residual,
+                                              OptTensor gate, torch::Tensor w1, OptTensor b1,
+                                              OptTensor scale, torch::Tensor w2, OptTensor b2,
+                                              bool layer, double eps, bool want_stats) {
+  check_block_norm(x, residual, gate, w1, b1, scale, w2, b2);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t B = x.size(0), D = x.size(1), L = x.size(2);
+  auto y = torch::empty_like(x), rout = torch::empty_like(residual);
+  auto stats = want_stats ? floats({4, B, L}, x) : torch::Tensor();
+  check_status(dudy_block_norm_forward(
+                   x.data_ptr(), opt_ptr(gate), residual.data_ptr(), w1.data_ptr(), opt_ptr(b1),
+                   opt_ptr(scale), w2.data_ptr(), opt_ptr(b2), y.data_ptr(), rout.data_ptr(),
+                   want_stats ? (float *)stats.data_ptr() : nullptr, B, D, L, layer, (float)eps,
+                   dtype_code(x), dtype_code(residual), stream_ptr()),
+               "fused_gated_residual_norm forward");
+  return {y, rout, stats};
+}
+
+// grad x, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias (undefined where
+// there is no such input)
+std::vector<torch::Tensor> block_norm_backward(torch::Tensor gy, OptTensor grout,
+                                               torch::Tensor x, torch::Tensor residual,
+                                               OptTensor gate, torch::Tensor w1, OptTensor b1,
+                                               OptTensor scale, torch::Tensor w2, OptTensor b2,
+                                               torch::Tensor stats, bool layer) {
+  check_block_norm(x, residual, gate, w1, b1, scale, w2, b2);
+  const int64_t B = x.size(0), D = x.size(1), L = x.size(2);
+  check_like(gy, "grad_y", x.sizes(), x.scalar_type(), x);
+  check_like(grout, "grad_residual_out", x.sizes(), residual.scalar_type(), x);
+  check_like(stats, "stats", {4, B, L}, at::kFloat, x);
+  const c10::cuda::CUDAGuard guard(x.device());
+  auto like = [](const OptTensor &t) {
+    return t.has_value() ? torch::empty_like(*t) : torch::Tensor();
+  };
+  auto ptr = [](const torch::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
+  auto gx = torch::empty_like(x), gr = torch::empty_like(residual), gg = like(gate);
+  auto gw1 = torch::empty_like(w1), gb1 = like(b1), gsc = like(scale);
+  auto gw2 = torch::empty_like(w2), gb2 = like(b2);
+  const int dt = dtype_code(x), rdt = dtype_code(residual);
+  auto ws = scratch(dudy_block_norm_backward_workspace_size(B, D, L, dt, rdt), x);
+  check_status(dudy_block_norm_backward(
+                   gy.data_ptr(), opt_ptr(grout), x.data_ptr(), opt_ptr(gate),
+                   residual.data_ptr(), w1.data_ptr(), opt_ptr(b1), opt_ptr(scale),
+                   w2.data_ptr(), (const float *)stats.data_ptr(), gx.data_ptr(), ptr(gg),
+                   gr.data_ptr(), gw1.data_ptr(), ptr(gb1), ptr(gsc), gw2.data_ptr(), ptr(gb2),
+                   ws.data_ptr(), (size_t)ws.numel(), B, D, L, layer, dt, rdt, stream_ptr()),
+               "fused_gated_residual_norm backward");
+  return {gx, gr, gg, gw1, gb1, gsc, gw2, gb2};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -575,6 +877,33 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("logits_to_kernel_backward", &logits_to_kernel_backward,
         "Backward of logits_to_kernel from its output kc and grad_kc", py::arg("kc"),
         py::arg("grad_kc"));
+  m.def("short_conv_forward", &short_conv_forward, "Short causal depthwise conv forward",
+        py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("state"), py::arg("lengths"),
+        py::arg("silu"), py::arg("want_final"));
+  m.def("short_conv_backward", &short_conv_backward, "Short causal depthwise conv backward",
+        py::arg("go"), py::arg("grad_final"), py::arg("x"), py::arg("weight"), py::arg("bias"),
+        py::arg("state"), py::arg("lengths"), py::arg("silu"), py::arg("want_state"));
+  m.def("short_conv_step", &short_conv_step, "Short causal depthwise conv, one token",
+        py::arg("x"), py::arg("state"), py::arg("weight"), py::arg("bias"), py::arg("silu"));
+  m.def("selective_scan_forward", &selective_scan_forward, "Selective scan forward",
+        py::arg("u"), py::arg("delta"), py::arg("A"), py::arg("B"), py::arg("C"),
+        py::arg("skip"), py::arg("delta_bias"), py::arg("state"), py::arg("lengths"),
+        py::arg("softplus"), py::arg("want_final"), py::arg("want_checkpoints"));
+  m.def("selective_scan_backward", &selective_scan_backward, "Selective scan backward",
+        py::arg("go"), py::arg("grad_final"), py::arg("u"), py::arg("delta"), py::arg("A"),
+        py::arg("B"), py::arg("C"), py::arg("skip"), py::arg("delta_bias"),
+        py::arg("checkpoints"), py::arg("lengths"), py::arg("softplus"), py::arg("want_state"));
+  m.def("selective_scan_step", &selective_scan_step, "Selective scan, one token", py::arg("u"),
+        py::arg("delta"), py::arg("A"), py::arg("B"), py::arg("C"), py::arg("state"),
+        py::arg("skip"), py::arg("delta_bias"), py::arg("softplus"));
+  m.def("block_norm_forward", &block_norm_forward, "Gate, norms and residual between blocks",
+        py::arg("x"), py::arg("residual"), py::arg("gate"), py::arg("post_weight"),
+        py::arg("post_bias"), py::arg("scale"), py::arg("pre_weight"), py::arg("pre_bias"),
+        py::arg("layer"), py::arg("eps"), py::arg("want_stats"));
+  m.def("block_norm_backward", &block_norm_backward, "Backward of block_norm_forward",
+        py::arg("grad_y"), py::arg("grad_residual_out"), py::arg("x"), py::arg("residual"),
+        py::arg("gate"), py::arg("post_weight"), py::arg("post_bias"), py::arg("scale"),
+        py::arg("pre_weight"), py::arg("pre_bias"), py::arg("stats"), py::arg("layer"));
 }
 
 TORCH_LIBRARY(fused_source_conv_mixed, m) {

@@ -289,6 +289,102 @@ DUDY_API int dudy_fscm_backward(const void *go, const void *x, const void *weigh
                        int64_t off, int64_t T, int64_t dilation, int dtype, int plan,
                        int64_t tile_t, void *stream);
 
+/* ========================================================================================
+ * State-space block: short causal depthwise conv, selective scan, and the norms, gate and
+ * residual between blocks. No reference counterpart: sequence operators of the dynamic conv's
+ * [B,D,L] layout beside it. Element type of all tensors is `dtype` unless a parameter is
+ * declared float; sums, states and statistics are fp32. `lengths` (int32 [B] on the device, or
+ * NULL) gives each sequence's length in a batch padded on the right, clamped to [0, L]:
+ * positions at and behind it are not read, come out as zeros and carry no gradient, and the
+ * final state is the one at the length. Each gradient is a sum in a fixed order (no atomics).
+ * ======================================================================================== */
+
+/* ---- short causal depthwise conv ----
+ *   x [B,D,L]  weight [D,S]  bias [D] or NULL  state [B,D,S-1] or NULL (zeros)
+ *   xe = state in front of x;  v = bias + sum_{j<S} weight[d,j] xe[t-(S-1)+j]
+ *   out [B,D,L] = v sigmoid(v) (silu != 0) or v;  final_state [B,D,S-1] (or NULL) = the last
+ *   S-1 entries of xe before the sequence's length.  2 <= S <= DUDY_SHORT_CONV_MAX_TAPS. */
+#define DUDY_SHORT_CONV_MAX_TAPS 8
+DUDY_API int dudy_short_conv_forward(const void *x, const void *weight, const void *bias,
+                                     const void *state, const int32_t *lengths, void *out,
+                                     void *final_state, int64_t B, int64_t D, int64_t L,
+                                     int64_t S, int silu, int dtype, void *stream);
+DUDY_API size_t dudy_short_conv_backward_workspace_size(int64_t B, int64_t D, int64_t L,
+                                                        int64_t S, int dtype);
+/* grad_final [B,D,S-1] may be NULL (zeros); grad_bias and grad_state may be NULL (not wanted). */
+DUDY_API int dudy_short_conv_backward(const void *go, const void *grad_final, const void *x,
+                                      const void *weight, const void *bias, const void *state,
+                                      const int32_t *lengths, void *grad_x, void *grad_weight,
+                                      void *grad_bias, void *grad_state, void *workspace,
+                                      size_t workspace_bytes, int64_t B, int64_t D, int64_t L,
+                                      int64_t S, int silu, int dtype, void *stream);
+/* One token per sequence: x [B,D] -> out [B,D], state [B,D,S-1] updated in place. */
+DUDY_API int dudy_short_conv_step(const void *x, void *state, const void *weight,
+                                  const void *bias, void *out, int64_t B, int64_t D, int64_t S,
+                                  int silu, int dtype, void *stream);
+
+/* ---- selective state space scan ----
+ *   u, delta, y [B,D,L]  A [D,N] float  Bm, Cm [B,G,N,L]  skip, delta_bias [D] float or NULL
+ *   state [B,D,N] float or NULL (zeros);  channel d reads group d / (D/G)
+ *   dt = softplus(delta + delta_bias) (softplus != 0) or delta + delta_bias
+ *   h[n] = exp(dt A[d,n]) h[n] + dt u Bm[n];   y = sum_n Cm[n] h[n] + skip u
+ * 1 <= N <= DUDY_SCAN_MAX_STATE, D a multiple of G. `checkpoints` (or NULL) receives the states
+ * that the backward starts from, dudy_selective_scan_checkpoint_bytes bytes. */
+#define DUDY_SCAN_MAX_STATE 64
+DUDY_API size_t dudy_selective_scan_checkpoint_bytes(int64_t B, int64_t D, int64_t L, int64_t N,
+                                                     int64_t G, int dtype);
+DUDY_API size_t dudy_selective_scan_forward_workspace_size(int64_t B, int64_t D, int64_t L,
+                                                           int64_t N, int64_t G, int dtype);
+DUDY_API int dudy_selective_scan_forward(const void *u, const void *delta, const float *A,
+                                         const void *Bm, const void *Cm, const float *skip,
+                                         const float *delta_bias, const float *state,
+                                         const int32_t *lengths, void *y, float *final_state,
+                                         float *checkpoints, void *workspace,
+                                         size_t workspace_bytes, int64_t B, int64_t D, int64_t L,
+                                         int64_t N, int64_t G, int softplus, int dtype,
+                                         void *stream);
+DUDY_API size_t dudy_selective_scan_backward_workspace_size(int64_t B, int64_t D, int64_t L,
+                                                            int64_t N, int64_t G, int dtype);
+/* grad_final [B,D,N] float may be NULL (zeros); grad_skip, grad_delta_bias, grad_state may be
+ * NULL (not wanted). `lengths` as in the forward. */
+DUDY_API int dudy_selective_scan_backward(
+    const void *go, const float *grad_final, const void *u, const void *delta, const float *A,
+    const void *Bm, const void *Cm, const float *skip, const float *delta_bias,
+    const float *checkpoints, const int32_t *lengths, void *grad_u, void *grad_delta,
+    float *grad_A, void *grad_B, void *grad_C, float *grad_skip, float *grad_delta_bias,
+    float *grad_state, void *workspace, size_t workspace_bytes, int64_t B, int64_t D, int64_t L,
+    int64_t N, int64_t G, int softplus, int dtype, void *stream);
+/* One token per sequence: u, delta, y [B,D], Bm, Cm [B,G,N], state [B,D,N] updated in place. */
+DUDY_API int dudy_selective_scan_step(const void *u, const void *delta, const float *A,
+                                      const void *Bm, const void *Cm, const float *skip,
+                                      const float *delta_bias, float *state, void *y, int64_t B,
+                                      int64_t D, int64_t N, int64_t G, int softplus, int dtype,
+                                      void *stream);
+
+/* ---- norms after and before a block, with its gate, residual and residual scale ----
+ *   x, gate [B,D,L] (gate or NULL)  residual [B,D,L] of residual_dtype (dtype or float)
+ *   g = x gate sigmoid(gate) (or x);  p = norm(g) post_weight + post_bias
+ *   residual_out = residual + scale p;  y = norm(residual_out) pre_weight + pre_bias
+ * norm over the D channels of a token: rms (layer = 0) or with the mean taken off (layer = 1).
+ * Parameters are [D]; scale (1) and the biases (0) may be NULL. y uses residual_out before its
+ * rounding. `stats` (or NULL) receives 4*B*L floats that the backward needs. */
+DUDY_API int dudy_block_norm_forward(const void *x, const void *gate, const void *residual,
+                                     const void *post_weight, const void *post_bias,
+                                     const void *scale, const void *pre_weight,
+                                     const void *pre_bias, void *y, void *residual_out,
+                                     float *stats, int64_t B, int64_t D, int64_t L, int layer,
+                                     float eps, int dtype, int residual_dtype, void *stream);
+DUDY_API size_t dudy_block_norm_backward_workspace_size(int64_t B, int64_t D, int64_t L,
+                                                        int dtype, int residual_dtype);
+/* grad_residual_out may be NULL (zeros); parameter gradients may be NULL (not wanted). */
+DUDY_API int dudy_block_norm_backward(
+    const void *grad_y, const void *grad_residual_out, const void *x, const void *gate,
+    const void *residual, const void *post_weight, const void *post_bias, const void *scale,
+    const void *pre_weight, const float *stats, void *grad_x, void *grad_gate,
+    void *grad_residual, void *grad_post_weight, void *grad_post_bias, void *grad_scale,
+    void *grad_pre_weight, void *grad_pre_bias, void *workspace, size_t workspace_bytes,
+    int64_t B, int64_t D, int64_t L, int layer, int dtype, int residual_dtype, void *stream);
+
 /* Self-test of the bounded waits (no reference counterpart: its kernels have no
  * device-side waits). Runs one CTA built like the tensor-core kernels (one warp holding a
  * TMEM allocation) in which one warp waits, with a limit of `limit_us` microseconds
