@@ -7,7 +7,8 @@ What stands between two blocks of a ``[B, D, L]`` model, per token over its D ch
     residual_out = residual + scale * p
     y = norm(residual_out) * pre_weight + pre_bias    -> the next block's input
 
-``norm`` is ``"rms"`` (``v / sqrt(mean(v^2) + eps)``) or ``"layer"`` (the mean taken off first).
+``norm`` is ``"rms"`` (``v / sqrt(mean(v^2) + eps)``, without biases) or ``"layer"`` (the mean
+taken off first).
 PyTorch runs this as about ten passes over the tensors; here each direction reads its inputs and
 writes its outputs once. Statistics and sums are fp32; ``y`` is formed from ``residual_out``
 before its rounding. Gradients are sums in a fixed order: the same call gives the same bits.
@@ -68,6 +69,8 @@ def fused_gated_residual_norm(x: torch.Tensor, residual: torch.Tensor, post_weig
     stream ``residual`` (of x's type, or fp32), with ``[D]`` parameters of x's type; one token
     per sequence is ``L = 1``. Differentiable in all tensors."""
     layer = _layer(norm)
+    if not layer and (post_bias is not None or pre_bias is not None):
+        raise RuntimeError("an rms norm has no bias.")
     if not eps > 0:
         raise RuntimeError(f"eps must be positive, got {eps}.")
     args = (x, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias)
@@ -85,7 +88,8 @@ class FusedGatedResidualNorm1d(nn.Module):
                  init_scale: float = 1.0, use_bias: bool = False, dtype=None, device=None):
         super().__init__()
         self.embed_dim, self.norm, self.eps = int(embed_dim), norm, float(eps)
-        _layer(norm)
+        if not _layer(norm) and use_bias:
+            raise ValueError("an rms norm has no bias.")
         if self.embed_dim <= 0:
             raise ValueError("embed_dim must be positive.")
         kw = {"dtype": dtype, "device": device}

@@ -88,7 +88,7 @@ cudaError_t set_smem_once(const void *kern, int bytes) {
     int dev, bytes;
   };
   static std::mutex mu;
-  static Entry table[64];
+  static Entry table[256];
   static int used = 0;
   const int dev = current_device();
   std::lock_guard<std::mutex> lock(mu);
@@ -102,7 +102,7 @@ cudaError_t set_smem_once(const void *kern, int bytes) {
       table[i].bytes = bytes;
       return cudaSuccess;
     }
-  if (used < 64) table[used++] = Entry{kern, dev, bytes};
+  if (used < 256) table[used++] = Entry{kern, dev, bytes};
   return cudaSuccess;
 }
 

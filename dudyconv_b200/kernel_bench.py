@@ -4,6 +4,8 @@
            [--stage all|forward|grad_h|grad_kc_mix] [--plan tc|simt] [--iters 50]
            [--profile]
     python -m dudyconv_b200.kernel_bench --op fscm [--channels 16 --taps 3 --dilation 1]
+    python -m dudyconv_b200.kernel_bench --op short_conv|selective_scan|block_norm
+           [--dim 256 --taps 4 --state 16 --groups 1 --dtype fp16|bf16|fp32]
 
 
 Times each stage (forward, grad_h, grad_kc + grad_mix) with CUDA events, rotating two
@@ -93,9 +95,103 @@ def fscm_main(a):
     print(json.dumps(res))
 
 
+def state_space_main(a):
+    """Forward and backward of one operator of the state-space block (short_conv,
+    selective_scan, block_norm) through the C ABI. Algorithmic bytes: each row tensor once."""
+    dev = torch.device("cuda")
+    dt = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}[a.dtype]
+    B, L, D, N, G, S = a.batch, a.seq, a.dim, a.state, a.groups, a.taps
+    gen = torch.Generator(device=dev).manual_seed(0)
+
+    def randn(*shape, dtype=dt, scale=1.0):
+        return (torch.randn(*shape, device=dev, generator=gen) * scale).to(dtype)
+
+    def scratch(nbytes):
+        return torch.empty(max(256, nbytes), dtype=torch.uint8, device=dev)
+
+    rows = [[randn(B, D, L) for _ in range(5)] for _ in range(2)]
+    outs = [torch.empty(B, D, L, device=dev, dtype=dt) for _ in range(3)]
+    x0 = rows[0][0]
+    if a.op == "short_conv":
+        w, bias = randn(D, S, scale=S ** -0.5), randn(D)
+        gw, gb = torch.empty_like(w), torch.empty_like(bias)
+        ws = scratch(capi.short_conv_backward_workspace_size(x0, w))
+        moved = {"forward": 2, "backward": 3}
+
+        def launch(stage, i):
+            x, go = rows[i % 2][:2]
+            if stage == "forward":
+                capi.short_conv_forward(x, w, bias, None, None, outs[0])
+            else:
+                capi.short_conv_backward(go, None, x, w, bias, None, None, outs[1], gw, gb, None, ws)
+    elif a.op == "selective_scan":
+        A = -torch.arange(1, N + 1, device=dev, dtype=torch.float32).repeat(D, 1)
+        skip, dbias = torch.ones(D, device=dev), torch.full((D,), -4.0, device=dev)
+        bc = [[randn(B, G, N, L) for _ in range(2)] for _ in range(2)]
+        gA, gskip, gbias = torch.empty_like(A), torch.empty_like(skip), torch.empty_like(skip)
+        gB, gC = torch.empty_like(bc[0][0]), torch.empty_like(bc[0][0])
+        ck = scratch(capi.selective_scan_checkpoint_bytes(x0, A, bc[0][0]))
+        wf = scratch(capi.selective_scan_forward_workspace_size(x0, A, bc[0][0]))
+        ws = scratch(capi.selective_scan_backward_workspace_size(x0, A, bc[0][0]))
+        moved = {"forward": 3, "forward_saving": 3, "backward": 5}
+
+        def launch(stage, i):
+            u, de, go = rows[i % 2][:3]
+            Bm, Cm = bc[i % 2]
+            if stage != "backward":
+                capi.selective_scan_forward(u, de, A, Bm, Cm, skip, dbias, None, None, outs[0], None,
+                                            ck if stage == "forward_saving" else None, wf)
+            else:
+                capi.selective_scan_backward(go, None, u, de, A, Bm, Cm, skip, dbias, ck, None,
+                                             outs[1], outs[2], gA, gB, gC, gskip, gbias, None, ws)
+    else:
+        par = [randn(D) for _ in range(3)]
+        gp = [torch.empty_like(p) for p in par]
+        stats = torch.empty(4, B, L, device=dev)
+        ws = scratch(capi.block_norm_backward_workspace_size(x0, x0))
+        moved = {"forward": 5, "backward": 8}
+
+        def launch(stage, i):
+            x, z, r, gy, gr = rows[i % 2]
+            if stage == "forward":
+                capi.block_norm_forward(x, z, r, par[0], None, par[1], par[2], None, outs[0],
+                                        outs[1], stats)
+            else:
+                capi.block_norm_backward(gy, gr, x, z, r, par[0], None, par[1], par[2], stats,
+                                         outs[0], outs[1], outs[2], gp[0], None, gp[1], gp[2],
+                                         None, ws)
+
+    if a.profile:  # 4 launches of each pass, nothing timed
+        for st in moved:
+            for i in range(4):
+                launch(st, i)
+        torch.cuda.synchronize()
+        print(json.dumps({"profile_launches": 4}))
+        return
+    res = {"op": a.op, "batch": B, "seq": L, "D": D, "N": N, "G": G, "S": S, "dtype": a.dtype}
+    for st, n in moved.items():
+        for i in range(3):
+            launch(st, i)
+        torch.cuda.synchronize()
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        e0.record()
+        for i in range(a.iters):
+            launch(st, i)
+        e1.record()
+        torch.cuda.synchronize()
+        us = e0.elapsed_time(e1) / a.iters * 1e3
+        res[st] = {"us": round(us, 2), "GB/s": round(n * x0.numel() * x0.element_size() / us / 1e3, 1)}
+    print(json.dumps(res))
+
+
+STATE_SPACE = ("short_conv", "selective_scan", "block_norm")
+
+
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("--op", default="fdc", choices=["fdc", "fscm"])
+    ap.add_argument("--op", default="fdc", choices=("fdc", "fscm") + STATE_SPACE)
+    ap.add_argument("--state", type=int, default=16, help="selective_scan: states N")
+    ap.add_argument("--groups", type=int, default=1, help="selective_scan: groups G of B and C")
     ap.add_argument("--channels", type=int, default=16, help="fscm: source channels C")
     ap.add_argument("--batch", type=int, default=16)
     ap.add_argument("--seq", type=int, default=4096)
@@ -104,7 +200,8 @@ def main():
     ap.add_argument("--dim", type=int, default=256)
     ap.add_argument("--dilation", type=int, default=1)
     ap.add_argument("--offset", type=int, default=0)
-    ap.add_argument("--dtype", default="fp16", choices=["fp16", "bf16"])
+    ap.add_argument("--dtype", default="fp16", choices=["fp16", "bf16", "fp32"],
+                    help="fp32: the state-space operators only")
     ap.add_argument("--stage", default="all", choices=("all",) + STAGES)
     ap.add_argument("--plan", default="tc", choices=["tc", "simt"])
     ap.add_argument("--iters", type=int, default=50)
@@ -112,6 +209,8 @@ def main():
     a = ap.parse_args()
     if a.op == "fscm":
         return fscm_main(a)
+    if a.op in STATE_SPACE:
+        return state_space_main(a)
 
     dev = torch.device("cuda")
     dt = torch.float16 if a.dtype == "fp16" else torch.bfloat16

@@ -366,8 +366,8 @@ DUDY_API int dudy_selective_scan_step(const void *u, const void *delta, const fl
  *   g = x gate sigmoid(gate) (or x);  p = norm(g) post_weight + post_bias
  *   residual_out = residual + scale p;  y = norm(residual_out) pre_weight + pre_bias
  * norm over the D channels of a token: rms (layer = 0) or with the mean taken off (layer = 1).
- * Parameters are [D]; scale (1) and the biases (0) may be NULL. y uses residual_out before its
- * rounding. `stats` (or NULL) receives 4*B*L floats that the backward needs. */
+ * Parameters are [D]; scale (1) and the biases (0) may be NULL, and the biases are for layer
+ * norms. y uses residual_out before its rounding. `stats` (or NULL) receives 4*B*L floats that the backward needs. */
 DUDY_API int dudy_block_norm_forward(const void *x, const void *gate, const void *residual,
                                      const void *post_weight, const void *post_bias,
                                      const void *scale, const void *pre_weight,

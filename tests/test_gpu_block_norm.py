@@ -18,7 +18,7 @@ CASES = [  # B, D, L, dtype, residual dtype, norm, gate, scale, biases, offset
     (2, 64, 8, "fp16", "fp32", "rms", False, True, False, 0),
     (1, 33, 31, "fp32", "fp32", "layer", False, False, True, 0),
     (2, 256, 64, "fp16", "fp16", "rms", True, True, False, 0),
-    (1, 256, 136, "bf16", "fp32", "rms", True, True, True, 0),
+    (1, 256, 136, "bf16", "fp32", "rms", True, True, False, 0),
     (1, 200, 72, "fp32", "fp32", "layer", True, True, True, 0),
     (2, 128, 65, "bf16", "bf16", "layer", True, True, True, 0),
     (1, 512, 128, "fp16", "fp16", "layer", False, True, True, 0),
@@ -90,6 +90,7 @@ def test_one_output_alone_and_refusals():
         (lambda: f(x, r, w, w, gate=h), "gate must be Float"),
         (lambda: f(x, r, w, w, norm="batch"), "norm must be"),
         (lambda: f(x, r, w, w, eps=0.0), "eps must be positive"),
+        (lambda: f(x, r, w, w, pre_bias=w), "an rms norm has no bias"),
         (lambda: f(x[0], r[0], w, w), r"x must be \[B,D,L\]"),
         (lambda: f(x[..., :0], r[..., :0], w, w), "must be positive"),
     ]:

@@ -89,7 +89,8 @@ def test_python_checks():
     with pytest.raises(RuntimeError, match="norm must be 'rms' or 'layer'"):
         fused_gated_residual_norm(x, x, x[0, :, 0], x[0, :, 0], norm="none")
     for make in (lambda: FusedShortConv1d(0), lambda: FusedShortConv1d(4, 9), lambda: FusedSelectiveScan1d(4, 65),
-                 lambda: FusedSelectiveScan1d(4, 16, dt_min=0.0), lambda: FusedGatedResidualNorm1d(-1)):
+                 lambda: FusedSelectiveScan1d(4, 16, dt_min=0.0), lambda: FusedGatedResidualNorm1d(-1),
+                 lambda: FusedGatedResidualNorm1d(8, use_bias=True)):
         with pytest.raises(ValueError):
             make()
     torch.manual_seed(0)
@@ -98,5 +99,5 @@ def test_python_checks():
     dt = torch.nn.functional.softplus(s.delta_bias)
     assert ((dt > 0.99e-3) & (dt < 1.01e-1)).all()
     assert FusedShortConv1d(8, use_bias=False).bias is None
-    m = FusedGatedResidualNorm1d(8, use_bias=True, init_scale=0.1)
+    m = FusedGatedResidualNorm1d(8, "layer", use_bias=True, init_scale=0.1)
     assert sorted(n for n, _ in m.named_parameters()) == ["post_bias", "post_weight", "pre_bias", "pre_weight", "scale"]
