@@ -3,12 +3,21 @@
 //   dt = softplus(delta + delta_bias)             (or delta + delta_bias)
 //   h[t] = exp(dt A) h[t-1] + dt u B[t]           per channel d and state n
 //   y[t] = sum_n C[t] h[t] + skip u
-// A thread owns four neighbouring states n of a channel; LPC lanes hold a channel's states
-// (N <= 4 LPC, padded with A = B = C = 0, which add nothing) and a warp 32 / LPC lanes across
-// channels. Time is cut into superchunks: the warps of a block take consecutive pieces of one,
-// run the recurrence from zero, exchange their end states and decay products through shared
-// memory and run it again from the state that enters their piece, with the decays kept in
-// registers. So the exponentials, which bound the forward, are computed once.
+// A thread owns four neighbouring states n of two or four channels; LPC lanes hold a channel's
+// states (N <= 4 LPC, padded with A = B = C = 0, which add nothing). Time is cut into
+// superchunks: the warps of a block take consecutive pieces of one, run the recurrence from
+// zero, exchange their end states and decay products through shared memory and run it again
+// from the state that enters their piece, with the decays kept in registers. So each
+// exponential is computed once: the special function unit (16 a clock and SM, 59 us for the
+// 268 M of B=16, D=256, L=4096, N=16) bounds the forward, not HBM (17 us).
+//
+// Where there are too few rows of channels to fill the GPU, the sequence is cut once more, into
+// `splits` chunks of whole superchunks, a block to each: a first kernel finds each chunk's end
+// state from zero and its decay product, and the main kernel's block folds those of the chunks
+// before its own into the state that it starts from. That doubles the exponentials and divides
+// the steps in a row by `splits`.
+//
+// All arithmetic is fp32, two at a time where pairs lie side by side (__ffma2_rn).
 #pragma once
 
 #include <type_traits>
@@ -38,36 +47,99 @@ __device__ __forceinline__ int64_t clamp_len(const int32_t *lengths, int64_t b, 
   return n < 0 ? 0 : (n > L ? L : n);
 }
 
-// exp(x) for the decays. 16-bit tensors: one multiply and the base-2 exponential of the
-// special function unit (relative error about 2^-22, against 2^-9 or 2^-12 of the result's
+// exp(dt A) as decay(dt * scaled(A)). 16-bit tensors: the base-2 exponential of the special
+// function unit on A log2(e) (relative error about 2^-22, against 2^-9 or 2^-12 of the result's
 // rounding); fp32 tensors: the accurate exponential.
 template <typename T>
-__device__ __forceinline__ float decay(float x) {
+__device__ __forceinline__ float scaled(float a) {
+  return a * 1.4426950408889634f;
+}
+template <>
+__device__ __forceinline__ float scaled<float>(float a) {
+  return a;
+}
+template <typename T>
+__device__ __forceinline__ constexpr float unscaled() {
+  return sizeof(T) == 4 ? 1.f : 0.6931471805599453f;
+}
+__device__ __forceinline__ float ex2(float x) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+template <typename T>
+__device__ __forceinline__ float decay(float x) {
+  return ex2(x);
 }
 template <>
 __device__ __forceinline__ float decay<float>(float x) {
   return expf(x);
 }
 
-// softplus and its derivative. 16-bit tensors: log(1 + e) = e - e^2/2 + e^3/3 - e^4/4 where
-// e = exp(x) is small (the logarithm of a rounded 1 + e would lose its digits), else the fast
-// logarithm; both are exact to a few 2^-20. Above 20, log(1 + e) = x to fp32's precision.
+// softplus(x) = max(x, 0) + log(1 + e), e = exp(-|x|), and its derivative. 16-bit tensors take
+// log(1 + e) = 2 artanh(e / (2 + e)) by its power series: the argument is at most 1/3, so seven
+// terms leave 2^-26, and small steps keep their relative precision (the logarithm of a rounded
+// 1 + e would not). fp32 tensors: the accurate functions.
 template <typename T>
 __device__ __forceinline__ float softplus(float x, float &slope) {
-  const float e = __expf(x);
-  slope = x > 20.f ? 1.f : __fdividef(e, 1.f + e);
-  const float small = e * fmaf(-e, fmaf(-e, fmaf(-e, 0.25f, 1.f / 3.f), 0.5f), 1.f);
-  return x > 20.f ? x : (e < 0.03f ? small : __logf(1.f + e));
+  const float e = ex2(-1.4426950408889634f * fabsf(x));
+  const float s = __fdividef(e, 2.f + e), q = s * s;
+  float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
+  p = fmaf(p, q, 1.f / 9.f);
+  p = fmaf(p, q, 1.f / 7.f);
+  p = fmaf(p, q, 1.f / 5.f);
+  p = fmaf(p, q, 1.f / 3.f);
+  p = fmaf(p, q, 1.f);
+  slope = __fdividef(x > 0.f ? 1.f : e, 1.f + e);
+  return fmaf(s + s, p, fmaxf(x, 0.f));
 }
 template <>
 __device__ __forceinline__ float softplus<float>(float x, float &slope) {
-  const float e = expf(x);
-  slope = x > 20.f ? 1.f : e / (1.f + e);
-  return x > 20.f ? x : log1pf(e);
+  const float e = expf(-fabsf(x));
+  slope = (x > 0.f ? 1.f : e) / (1.f + e);
+  return fmaxf(x, 0.f) + log1pf(e);
 }
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 lo(const float4 &v) { return make_float2(v.x, v.y); }
+__device__ __forceinline__ float2 hi(const float4 &v) { return make_float2(v.z, v.w); }
+__device__ __forceinline__ float4 quad(const float2 &a, const float2 &b) {
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// Sums of n values each over the lanes that differ in the bits [STRIDE, STRIDE * LANES) of the
+// lane number. While there are several values, half of them go to the partner lane and half
+// come from it, so a stage costs n / 2 shuffles; afterwards lane l of the group (its number in
+// those bits) holds the sums of values l * n / LANES .. , or, with more lanes than n / KEEP
+// values, all lanes that agree in the upper bits hold the same KEEP values.
+template <int STRIDE, int LANES, int N, int KEEP = 1>
+struct Scatter {
+  static constexpr int kLeft = LANES == 1 || N == KEEP ? N : Scatter<STRIDE, LANES / 2, N / 2, KEEP>::kLeft;
+  static __device__ __forceinline__ void sum(float *v, int lane) {
+    if constexpr (LANES > 1) {
+      constexpr int o = STRIDE * LANES / 2;
+      if constexpr (N > KEEP) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          const float send = up ? v[i] : v[i + N / 2];
+          const float keep = up ? v[i + N / 2] : v[i];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+        Scatter<STRIDE, LANES / 2, N / 2, KEEP>::sum(v, lane);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+        Scatter<STRIDE, LANES / 2, N, KEEP>::sum(v, lane);
+      }
+    }
+  }
+};
+template <int STRIDE, int N, int KEEP>
+struct Scatter<STRIDE, 1, N, KEEP> {
+  static constexpr int kLeft = N;
+  static __device__ __forceinline__ void sum(float *, int) {}
+};
 
 // Copies a tile of `rows` rows x TS positions of a [.., L] tensor into shared memory as it is
 // (pitch PITCH elements): positions [t0, t0 + TS), zero at and behind `end`, and zero rows at
@@ -86,6 +158,24 @@ __device__ __forceinline__ void stage_rows(T *dst, const T *src, int rows, int v
 #pragma unroll
       for (int k = 0; k < V; ++k)
         to[k] = r < valid && t + k < end ? src[(int64_t)r * L + t + k] : Elem<T>::from_f(0.f);
+    }
+  }
+}
+
+// dst[r * PITCH + c] = row r of an fp32 [rows, N] matrix, zero behind N and behind `valid` rows.
+// Asynchronous where N is a multiple of four and src starts on 16 bytes.
+template <int NP>
+__device__ __forceinline__ void stage_states(float *dst, const float *src, int rows, int valid,
+                                             int N) {
+  const bool vec = N % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
+  for (int i = threadIdx.x; i < rows * (NP / 4); i += kThreads) {
+    const int r = i / (NP / 4), c = i % (NP / 4) * 4;
+    float *to = dst + r * NP + c;
+    if (vec && r < valid && c < N) {
+      cp_async16(to, src + r * N + c);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) to[k] = r < valid && c + k < N ? src[r * N + c + k] : 0.f;
     }
   }
 }

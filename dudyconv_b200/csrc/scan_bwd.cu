@@ -13,7 +13,7 @@
 // most of a sum over channels or states happens in its registers and only the rest by
 // shuffles. dB and dC of a block's channels are written as fp32 parts, one per block of
 // channels, and added by a second kernel in a fixed order; so are dA and the two [D] sums over
-// the batch.
+// the batch and the chunks.
 #include "scan.cuh"
 
 namespace dudy {
@@ -23,8 +23,8 @@ namespace {
 constexpr int kND = 4;                 // channels of a thread
 constexpr int kQ = 4;                  // positions of a warp in a superchunk
 constexpr int kTS = kWarps * kQ;       // positions of a superchunk
+constexpr int kOP = kTS + 4;
 static_assert(kTS == kCkpt, "a state is saved at each superchunk's start");
-constexpr int kST = kND * kNS;         // states of a thread
 
 struct Bwd {
   const void *go, *u, *delta, *Bm, *Cm;
@@ -33,334 +33,433 @@ struct Bwd {
   void *gu, *gdelta;
   float *ginit;
   float *part_b, *part_c;  // [tiles][B*G*N*L]
-  float *part_a;           // [B][D*N]
-  float *part_d;           // [2][B][D]: skip, delta_bias
-  int vec;
+  float *part_a;           // [splits][B][D*N]
+  float *part_d;           // [2][splits][B][D]: skip, delta_bias
+  float *rend, *prod;      // [splits][B*D][N]: what a chunk passes to its left from zero, and its
+                           // decays' product
+  int64_t chunk;           // positions of a chunk, a multiple of kTS
+  int splits, vec;
 };
 
 template <typename T, int LPC>
-struct BwdSmem {
+struct BwdTile {
   static constexpr int CT = 32 / LPC * kND;      // channels of a block
   static constexpr int NP = kNS * LPC;
   static constexpr int PITCH = kTS + 16 / (int)sizeof(T);
   T raw_u[CT * PITCH], raw_d[CT * PITCH], raw_g[CT * PITCH];
   T raw_b[NP * PITCH], raw_c[NP * PITCH];
-  float dt[kTS * CT], u[kTS * CT], go[kTS * CT], slope[kTS * CT];
-  float b[kTS * NP], c[kTS * NP];
-  float gu[CT * (kTS + 1)], gd[CT * (kTS + 1)];
-  float gb[NP * (kTS + 1)], gc[NP * (kTS + 1)];
-  // exchanged states, [warp][channel of the thread][lane]: forward end, decay product, and the
+  float dt[kTS * CT], du[kTS * CT], go[kTS * CT];
+  float u[kTS * CT], slope[kTS * CT];            // du's and ddelta's results take their places
+  float2 b[kTS * NP], c[kTS * NP];               // each twice side by side
+  float gb[NP * kOP], gc[NP * kOP];
+  float h0[2][CT * NP];                          // the states saved at the superchunk's start
+  // exchanged states, [warp][four of the thread's states][lane]: forward end, decay product and
   // backward end; the sums over warps at the end use the same room
   float4 end[kWarps * kND * 32], prod[kWarps * kND * 32], rend[kWarps * kND * 32];
   float4 rcarry[2 * kND * 32];
 };
 
-template <typename T, int LPC>
+// A thread's states lie in pairs of channels: e[p][n] holds channels 2p and 2p + 1 of state n,
+// so that a position's dt, dt u and gradient of two channels are operands as they are read.
+template <typename T, int LPC, bool PRE>
 __global__ void __launch_bounds__(kThreads, 1)
 scan_bwd_kernel(Bwd a, Shape s) {
-  using Smem = BwdSmem<T, LPC>;
-  constexpr int CT = Smem::CT, NP = Smem::NP, PITCH = Smem::PITCH, OP = kTS + 1;
+  using Tile = BwdTile<T, LPC>;
+  constexpr int CT = Tile::CT, NP = Tile::NP, PITCH = Tile::PITCH;
   extern __shared__ __align__(16) char smem_raw[];
-  Smem &m = *reinterpret_cast<Smem *>(smem_raw);
+  Tile &m = *reinterpret_cast<Tile *>(smem_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ln = lane % LPC, ld = lane / LPC, n0 = ln * kNS, c0 = ld * kND;
 
-  const int64_t R = s.D / s.G, tiles = (R + CT - 1) / CT;
-  const int64_t tile = blockIdx.x % tiles, bg = blockIdx.x / tiles;
-  const int64_t b = bg / s.G, g = bg % s.G;
-  const int chans = (int)(R - tile * CT < CT ? R - tile * CT : CT);
+  const int split = blockIdx.x % a.splits;
+  if (PRE && split == 0) return;  // nothing lies to the left of the first chunk
+  const int64_t bid = blockIdx.x / a.splits;
+  const int R = (int)(s.D / s.G), tiles = (R + CT - 1) / CT;
+  const int tile = (int)(bid % tiles);
+  const int64_t bg = bid / tiles, b = bg / s.G, g = bg % s.G;
+  const int chans = R - tile * CT < CT ? R - tile * CT : CT;
   const int64_t d0 = g * R + tile * CT, row0 = b * s.D + d0;
   const int64_t len = clamp_len(a.lengths, b, s.L);
+  const int64_t from = split * a.chunk;
+  const int64_t to = from + a.chunk < s.L ? from + a.chunk : s.L;
+  const int64_t end = to < len ? to : len;
   const T *u = (const T *)a.u + row0 * s.L, *delta = (const T *)a.delta + row0 * s.L;
   const T *go = (const T *)a.go + row0 * s.L;
   const T *Bm = (const T *)a.Bm + bg * s.N * s.L, *Cm = (const T *)a.Cm + bg * s.N * s.L;
   T *gu = (T *)a.gu + row0 * s.L, *gdelta = (T *)a.gdelta + row0 * s.L;
-  const int64_t nbc = s.B * s.G * s.N * s.L;
+  const int64_t nbc = s.B * s.G * s.N * s.L, nst = s.B * s.D * s.N;
   float *pb = a.part_b + tile * nbc + bg * s.N * s.L;
   float *pc = a.part_c + tile * nbc + bg * s.N * s.L;
 
-  float A[kST], dA[kST], r[kST], skip[kND], dskip[kND], dbias[kND];
+  float2 A[2][kNS], dA[2][kNS], r[2][kNS], dskip[2], dbias[2], total[2][kNS];
 #pragma unroll
-  for (int j = 0; j < kND; ++j) {
-    const bool mine = c0 + j < chans;
-    skip[j] = mine && a.skip ? a.skip[d0 + c0 + j] : 0.f;
-    dskip[j] = dbias[j] = 0.f;
+  for (int p = 0; p < 2; ++p) {
+    dskip[p] = dbias[p] = both(0.f);
 #pragma unroll
     for (int i = 0; i < kNS; ++i) {
-      const bool ok = mine && n0 + i < s.N;
-      A[j * kNS + i] = ok ? a.A[(d0 + c0 + j) * s.N + n0 + i] : 0.f;
-      r[j * kNS + i] = ok && a.gfinal ? a.gfinal[(row0 + c0 + j) * s.N + n0 + i] : 0.f;
-      dA[j * kNS + i] = 0.f;
+      float av[2], rv[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int c = c0 + 2 * p + x;
+        const bool ok = c < chans && n0 + i < s.N;
+        const int64_t at = (row0 + c) * s.N + n0 + i;
+        av[x] = ok ? scaled<T>(a.A[(d0 + c) * s.N + n0 + i]) : 0.f;
+        rv[x] = 0.f;
+        if (!PRE && ok) {
+          if (a.gfinal) rv[x] = a.gfinal[at];
+          for (int k = a.splits - 1; k > split; --k)
+            rv[x] = fmaf(a.prod[k * nst + at], rv[x], a.rend[k * nst + at]);
+        }
+      }
+      A[p][i] = make_float2(av[0], av[1]);
+      r[p][i] = make_float2(rv[0], rv[1]);
+      dA[p][i] = both(0.f);
+      total[p][i] = both(1.f);
     }
   }
-  auto put = [&](float4 *to, const float *v) {
+  auto put = [&](float4 *dst, const float2 (&v)[2][kNS]) {
 #pragma unroll
-    for (int j = 0; j < kND; ++j)
-      to[j * 32 + lane] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    for (int p = 0; p < 2; ++p) {
+      dst[(2 * p) * 32 + lane] = quad(v[p][0], v[p][1]);
+      dst[(2 * p + 1) * 32 + lane] = quad(v[p][2], v[p][3]);
+    }
+  };
+  // v = prod v + add over what a warp put
+  auto fold = [&](float2 (&v)[2][kNS], const float4 *add, const float4 *prod) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float4 x = prod[(2 * p + i) * 32 + lane], e = add[(2 * p + i) * 32 + lane];
+        v[p][2 * i] = __ffma2_rn(lo(x), v[p][2 * i], lo(e));
+        v[p][2 * i + 1] = __ffma2_rn(hi(x), v[p][2 * i + 1], hi(e));
+        if (PRE) {
+          total[p][2 * i] = __fmul2_rn(total[p][2 * i], lo(x));
+          total[p][2 * i + 1] = __fmul2_rn(total[p][2 * i + 1], hi(x));
+        }
+      }
   };
   if (warp == 0) put(m.rcarry, r);
 
-  auto stage = [&](int64_t t0) {
-    stage_rows<T, kTS, PITCH>(m.raw_u, u, CT, chans, s.L, t0, len, a.vec);
-    stage_rows<T, kTS, PITCH>(m.raw_d, delta, CT, chans, s.L, t0, len, a.vec);
-    stage_rows<T, kTS, PITCH>(m.raw_g, go, CT, chans, s.L, t0, len, a.vec);
-    stage_rows<T, kTS, PITCH>(m.raw_b, Bm, NP, s.N, s.L, t0, len, a.vec);
-    stage_rows<T, kTS, PITCH>(m.raw_c, Cm, NP, s.N, s.L, t0, len, a.vec);
+  auto stage = [&](int64_t t0, int turn) {
+    stage_rows<T, kTS, PITCH>(m.raw_d, delta, CT, chans, s.L, t0, end, a.vec);
+    stage_rows<T, kTS, PITCH>(m.raw_g, go, CT, chans, s.L, t0, end, a.vec);
+    stage_rows<T, kTS, PITCH>(m.raw_c, Cm, NP, s.N, s.L, t0, end, a.vec);
+    if (PRE) return;
+    stage_rows<T, kTS, PITCH>(m.raw_u, u, CT, chans, s.L, t0, end, a.vec);
+    stage_rows<T, kTS, PITCH>(m.raw_b, Bm, NP, s.N, s.L, t0, end, a.vec);
+    stage_states<NP>(m.h0[turn], a.ckpt + ((b * s.ckpts() + t0 / kCkpt) * s.D + d0) * s.N, CT,
+                     chans, s.N);
   };
-  const int supers = (int)((len + kTS - 1) / kTS);
-  if (supers) stage((int64_t)(supers - 1) * kTS);
-  int parity = 0;
-  for (int k = supers - 1; k >= 0; --k, parity ^= 1) {
-    const int64_t t0 = (int64_t)k * kTS;
-    float hin[kST];
-#pragma unroll
-    for (int i = 0; i < kST; ++i) {
-      const int j = i / kNS, n = n0 + i % kNS;
-      hin[i] = c0 + j < chans && n < s.N
-                   ? a.ckpt[((row0 + c0 + j) * s.ckpts() + k) * s.N + n] : 0.f;
-    }
+  const int supers = end > from ? (int)((end - from + kTS - 1) / kTS) : 0;
+  if (supers) stage(from + (int64_t)(supers - 1) * kTS, 0);
+  int turn = 0;
+  for (int k = supers - 1; k >= 0; --k, turn ^= 1) {
+    const int64_t t0 = from + (int64_t)k * kTS;
     cp_async_wait_all();
     __syncthreads();
-    for (int i = threadIdx.x; i < CT * (kTS / 8); i += kThreads) {
-      const int d = i % CT, c = i / CT * 8;
-      float uv[8], dv[8], gv[8];
-      row_load8(m.raw_u + d * PITCH + c, uv);
-      row_load8(m.raw_d + d * PITCH + c, dv);
-      row_load8(m.raw_g + d * PITCH + c, gv);
+    for (int i = threadIdx.x; i < CT * (kTS / 4); i += kThreads) {
+      const int d = i % CT, c = i / CT * 4;
+      const T *ru = m.raw_u + d * PITCH + c, *rd = m.raw_d + d * PITCH + c;
+      const T *rg = m.raw_g + d * PITCH + c;
       const float bias = d < chans && a.delta_bias ? a.delta_bias[d0 + d] : 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float dt = dv[j] + bias, slope = 1.f;
+      for (int j = 0; j < 4; ++j) {
+        float dt = Elem<T>::to_f(rd[j]) + bias, slope = 1.f;
         if (s.softplus) dt = softplus<T>(dt, slope);
-        if (t0 + c + j >= len) dt = slope = 0.f;
+        if (t0 + c + j >= end) dt = slope = 0.f;
         const int at = (c + j) * CT + d;
         m.dt[at] = dt;
-        m.u[at] = uv[j];
-        m.go[at] = gv[j];
+        m.go[at] = Elem<T>::to_f(rg[j]);
+        if (PRE) continue;
+        const float uv = Elem<T>::to_f(ru[j]);
+        m.du[at] = dt * uv;
+        m.u[at] = uv;
         m.slope[at] = slope;
       }
     }
-    for (int i = threadIdx.x; i < NP * (kTS / 8); i += kThreads) {
-      const int n = i % NP, c = i / NP * 8;
-      float bv[8], cv[8];
-      row_load8(m.raw_b + n * PITCH + c, bv);
-      row_load8(m.raw_c + n * PITCH + c, cv);
+    for (int i = threadIdx.x; i < NP * (kTS / 4); i += kThreads) {
+      const int n = i % NP, c = i / NP * 4;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        m.b[(c + j) * NP + n] = bv[j];
-        m.c[(c + j) * NP + n] = cv[j];
+      for (int j = 0; j < 4; ++j) {
+        m.c[(c + j) * NP + n] = both(Elem<T>::to_f(m.raw_c[n * PITCH + c + j]));
+        if (!PRE) m.b[(c + j) * NP + n] = both(Elem<T>::to_f(m.raw_b[n * PITCH + c + j]));
       }
     }
     __syncthreads();
-    if (k > 0) stage(t0 - kTS);
+    if (k > 0) stage(t0 - kTS, turn ^ 1);
 
     // both directions from zero
-    float dec[kQ][kST], h[kQ][kST], loc[kST];
+    const float *sdt = m.dt + warp * kQ * CT + c0, *sdu = m.du + warp * kQ * CT + c0;
+    const float *sgo = m.go + warp * kQ * CT + c0;
+    const float2 *sb2 = m.b + warp * kQ * NP + n0, *sc2 = m.c + warp * kQ * NP + n0;
+    auto four = [](const float *p) { return *reinterpret_cast<const float4 *>(p); };
+    auto pairs = [](const float2 *p, float2 (&v)[kNS]) {
+      const float4 x = reinterpret_cast<const float4 *>(p)[0];
+      const float4 z = reinterpret_cast<const float4 *>(p)[1];
+      v[0] = lo(x); v[1] = hi(x); v[2] = lo(z); v[3] = hi(z);
+    };
+    float2 dec[kQ][2][kNS], h[kQ][2][kNS], bv[kNS], cv[kNS];
     {
-      float sum[kND];
+      float2 sum[2], loc[2][kNS];
 #pragma unroll
-      for (int i = 0; i < kST; ++i) loc[i] = 0.f;
+      for (int p = 0; p < 2; ++p) {
+        sum[p] = both(0.f);
 #pragma unroll
-      for (int j = 0; j < kND; ++j) sum[j] = 0.f;
+        for (int i = 0; i < kNS; ++i) loc[p][i] = both(0.f);
+      }
 #pragma unroll
       for (int q = 0; q < kQ; ++q) {
-        const int t = warp * kQ + q;
-        const float4 dt = *reinterpret_cast<const float4 *>(m.dt + t * CT + c0);
-        const float4 uv = *reinterpret_cast<const float4 *>(m.u + t * CT + c0);
-        const float4 bv = *reinterpret_cast<const float4 *>(m.b + t * NP + n0);
+        const float4 dt = four(sdt + q * CT);
+        float4 du;
+        if (!PRE) {
+          du = four(sdu + q * CT);
+          pairs(sb2 + q * NP, bv);
+        }
 #pragma unroll
-        for (int j = 0; j < kND; ++j) {
-          const float dtj = (&dt.x)[j], du = dtj * (&uv.x)[j];
-          sum[j] += dtj;
+        for (int p = 0; p < 2; ++p) {
+          const float2 dtp = p ? hi(dt) : lo(dt), dup = p ? hi(du) : lo(du);
+          sum[p] = __fadd2_rn(sum[p], dtp);
 #pragma unroll
           for (int i = 0; i < kNS; ++i) {
-            const int e = j * kNS + i;
-            dec[q][e] = decay<T>(dtj * A[e]);
-            loc[e] = fmaf(dec[q][e], loc[e], du * (&bv.x)[i]);
+            const float2 x = __fmul2_rn(dtp, A[p][i]);
+            dec[q][p][i] = make_float2(decay<T>(x.x), decay<T>(x.y));
+            if (!PRE) loc[p][i] = __ffma2_rn(dec[q][p][i], loc[p][i], __fmul2_rn(dup, bv[i]));
           }
         }
       }
-      put(m.end + warp * kND * 32, loc);
+      if (!PRE) put(m.end + warp * kND * 32, loc);
 #pragma unroll
-      for (int e = 0; e < kST; ++e) loc[e] = decay<T>(sum[e / kNS] * A[e]);
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int i = 0; i < kNS; ++i) {
+          const float2 x = __fmul2_rn(sum[p], A[p][i]);
+          loc[p][i] = make_float2(decay<T>(x.x), decay<T>(x.y));
+        }
       put(m.prod + warp * kND * 32, loc);
 #pragma unroll
-      for (int e = 0; e < kST; ++e) loc[e] = 0.f;
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int i = 0; i < kNS; ++i) loc[p][i] = both(0.f);
 #pragma unroll
       for (int q = kQ - 1; q >= 0; --q) {
-        const int t = warp * kQ + q;
-        const float4 gv = *reinterpret_cast<const float4 *>(m.go + t * CT + c0);
-        const float4 cv = *reinterpret_cast<const float4 *>(m.c + t * NP + n0);
+        const float4 gv = four(sgo + q * CT);
+        pairs(sc2 + q * NP, cv);
 #pragma unroll
-        for (int e = 0; e < kST; ++e)
-          loc[e] = dec[q][e] * fmaf((&cv.x)[e % kNS], (&gv.x)[e / kNS], loc[e]);
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int i = 0; i < kNS; ++i)
+            loc[p][i] = __fmul2_rn(dec[q][p][i], __ffma2_rn(cv[i], p ? hi(gv) : lo(gv), loc[p][i]));
       }
       put(m.rend + warp * kND * 32, loc);
     }
     __syncthreads();
-    // what enters this warp's positions from the left and from the right
-    for (int w = 0; w < warp; ++w)
+    // what enters this warp's positions from the right, and from the left
 #pragma unroll
-      for (int j = 0; j < kND; ++j) {
-        const float4 p = m.prod[(w * kND + j) * 32 + lane], e = m.end[(w * kND + j) * 32 + lane];
-#pragma unroll
-        for (int i = 0; i < kNS; ++i)
-          hin[j * kNS + i] = fmaf((&p.x)[i], hin[j * kNS + i], (&e.x)[i]);
-      }
-#pragma unroll
-    for (int j = 0; j < kND; ++j) {
-      const float4 c = m.rcarry[(parity * kND + j) * 32 + lane];
-#pragma unroll
-      for (int i = 0; i < kNS; ++i) r[j * kNS + i] = (&c.x)[i];
+    for (int p = 0; p < 2; ++p) {
+      const float4 x = m.rcarry[(turn * kND + 2 * p) * 32 + lane];
+      const float4 z = m.rcarry[(turn * kND + 2 * p + 1) * 32 + lane];
+      r[p][0] = lo(x); r[p][1] = hi(x); r[p][2] = lo(z); r[p][3] = hi(z);
     }
-    for (int w = kWarps - 1; w > warp; --w)
+    for (int w = kWarps - 1; w > (PRE ? (warp ? kWarps : -1) : warp); --w)
+      fold(r, m.rend + w * kND * 32, m.prod + w * kND * 32);
+    if (PRE) {
+      if (warp == 0) put(m.rcarry + (turn ^ 1) * kND * 32, r);
+      continue;
+    }
 #pragma unroll
-      for (int j = 0; j < kND; ++j) {
-        const float4 p = m.prod[(w * kND + j) * 32 + lane], e = m.rend[(w * kND + j) * 32 + lane];
-#pragma unroll
-        for (int i = 0; i < kNS; ++i)
-          r[j * kNS + i] = fmaf((&p.x)[i], r[j * kNS + i], (&e.x)[i]);
-      }
+    for (int p = 0; p < 2; ++p) {
+      const float4 x = *reinterpret_cast<const float4 *>(m.h0[turn] + (c0 + 2 * p) * NP + n0);
+      const float4 z = *reinterpret_cast<const float4 *>(m.h0[turn] + (c0 + 2 * p + 1) * NP + n0);
+      h[0][p][0] = make_float2(x.x, z.x);
+      h[0][p][1] = make_float2(x.y, z.y);
+      h[0][p][2] = make_float2(x.z, z.z);
+      h[0][p][3] = make_float2(x.w, z.w);
+    }
+    for (int w = 0; w < warp; ++w) fold(h[0], m.end + w * kND * 32, m.prod + w * kND * 32);
     // forwards: h[q] is the state before position q
 #pragma unroll
-    for (int e = 0; e < kST; ++e) h[0][e] = hin[e];
-#pragma unroll
     for (int q = 0; q + 1 < kQ; ++q) {
-      const int t = warp * kQ + q;
-      const float4 dt = *reinterpret_cast<const float4 *>(m.dt + t * CT + c0);
-      const float4 uv = *reinterpret_cast<const float4 *>(m.u + t * CT + c0);
-      const float4 bv = *reinterpret_cast<const float4 *>(m.b + t * NP + n0);
+      const float4 du = four(sdu + q * CT);
+      pairs(sb2 + q * NP, bv);
 #pragma unroll
-      for (int e = 0; e < kST; ++e) {
-        const int j = e / kNS;
-        h[q + 1][e] = fmaf(dec[q][e], h[q][e], (&dt.x)[j] * (&uv.x)[j] * (&bv.x)[e % kNS]);
-      }
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int i = 0; i < kNS; ++i)
+          h[q + 1][p][i] =
+              __ffma2_rn(dec[q][p][i], h[q][p][i], __fmul2_rn(p ? hi(du) : lo(du), bv[i]));
     }
     // backwards
 #pragma unroll
     for (int q = kQ - 1; q >= 0; --q) {
       const int t = warp * kQ + q;
-      const float4 dt = *reinterpret_cast<const float4 *>(m.dt + t * CT + c0);
-      const float4 uv = *reinterpret_cast<const float4 *>(m.u + t * CT + c0);
-      const float4 gv = *reinterpret_cast<const float4 *>(m.go + t * CT + c0);
-      const float4 bv = *reinterpret_cast<const float4 *>(m.b + t * NP + n0);
-      const float4 cv = *reinterpret_cast<const float4 *>(m.c + t * NP + n0);
-      float db[kNS], dc[kNS], sb[kND], sa[kND];
+      const float4 dt = four(sdt + q * CT), du = four(sdu + q * CT), gv = four(sgo + q * CT);
+      pairs(sb2 + q * NP, bv);
+      pairs(sc2 + q * NP, cv);
+      float2 db[kNS], dc[kNS], sb[2], sa[2];
 #pragma unroll
-      for (int i = 0; i < kNS; ++i) db[i] = dc[i] = 0.f;
+      for (int i = 0; i < kNS; ++i) db[i] = dc[i] = both(0.f);
 #pragma unroll
-      for (int j = 0; j < kND; ++j) {
-        const float dtj = (&dt.x)[j], du = dtj * (&uv.x)[j], gy = (&gv.x)[j];
-        sb[j] = sa[j] = 0.f;
+      for (int p = 0; p < 2; ++p) {
+        const float2 dtp = p ? hi(dt) : lo(dt), dup = p ? hi(du) : lo(du);
+        const float2 gy = p ? hi(gv) : lo(gv);
+        sb[p] = sa[p] = both(0.f);
 #pragma unroll
         for (int i = 0; i < kNS; ++i) {
-          const int e = j * kNS + i;
-          const float gg = fmaf((&cv.x)[i], gy, r[e]);
-          const float ah = dec[q][e] * h[q][e];
-          const float ht = fmaf(du, (&bv.x)[i], ah);
-          const float w = gg * ah;
-          dc[i] = fmaf(gy, ht, dc[i]);
-          db[i] = fmaf(gg, du, db[i]);
-          sb[j] = fmaf(gg, (&bv.x)[i], sb[j]);
-          sa[j] = fmaf(w, A[e], sa[j]);
-          dA[e] = fmaf(w, dtj, dA[e]);
-          r[e] = dec[q][e] * gg;
+          const float2 gg = __ffma2_rn(cv[i], gy, r[p][i]);
+          const float2 ah = __fmul2_rn(dec[q][p][i], h[q][p][i]);
+          const float2 w = __fmul2_rn(gg, ah);
+          dc[i] = __ffma2_rn(gy, __ffma2_rn(dup, bv[i], ah), dc[i]);
+          db[i] = __ffma2_rn(gg, dup, db[i]);
+          sb[p] = __ffma2_rn(gg, bv[i], sb[p]);
+          sa[p] = __ffma2_rn(w, A[p][i], sa[p]);
+          dA[p][i] = __ffma2_rn(w, dtp, dA[p][i]);
+          r[p][i] = __fmul2_rn(dec[q][p][i], gg);
         }
       }
+      // dB, dC: over the lanes across channels; lane ld ends with values ld * left ..
+      float v[2 * kNS];
 #pragma unroll
-      for (int o = 16; o >= LPC; o >>= 1)
+      for (int i = 0; i < kNS; ++i) {
+        v[i] = db[i].x + db[i].y;
+        v[kNS + i] = dc[i].x + dc[i].y;
+      }
+      using SumD = Scatter<LPC, 32 / LPC, 2 * kNS>;
+      SumD::sum(v, lane);
+      constexpr int kLeftD = SumD::kLeft, kGroups = 2 * kNS / kLeftD;
+      constexpr int kSame = 32 / LPC / kGroups;  // lanes that hold the same values
+      if (ld % kSame == 0) {
 #pragma unroll
-        for (int i = 0; i < kNS; ++i) {
-          db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
-          dc[i] += __shfl_xor_sync(0xffffffffu, dc[i], o);
-        }
-      if (ld == 0) {
-#pragma unroll
-        for (int i = 0; i < kNS; ++i) {
-          m.gb[(n0 + i) * OP + t] = db[i];
-          m.gc[(n0 + i) * OP + t] = dc[i];
+        for (int i = 0; i < kLeftD; ++i) {
+          const int at = ld / kSame * kLeftD + i;
+          (at < kNS ? m.gb : m.gc)[(n0 + at % kNS) * kOP + t] = v[i];
         }
       }
+      // the sums over states: a channel's two values stay together
+      float z[2 * kND];
 #pragma unroll
-      for (int o = LPC / 2; o > 0; o >>= 1)
+      for (int p = 0; p < 2; ++p) {
+        z[4 * p] = sb[p].x; z[4 * p + 1] = sa[p].x;
+        z[4 * p + 2] = sb[p].y; z[4 * p + 3] = sa[p].y;
+      }
+      using SumN = Scatter<1, LPC, 2 * kND, 2>;
+      SumN::sum(z, lane);
+      constexpr int kLeftN = SumN::kLeft / 2, kOwners = kND / kLeftN, kEach = LPC / kOwners;
+      if (ln % kEach == 0) {
 #pragma unroll
-        for (int j = 0; j < kND; ++j) {
-          sb[j] += __shfl_xor_sync(0xffffffffu, sb[j], o);
-          sa[j] += __shfl_xor_sync(0xffffffffu, sa[j], o);
-        }
-      if (ln == 0) {
-        const float4 sl = *reinterpret_cast<const float4 *>(m.slope + t * CT + c0);
-#pragma unroll
-        for (int j = 0; j < kND; ++j) {
-          const float gy = (&gv.x)[j], uj = (&uv.x)[j];
-          const float dd = fmaf(uj, sb[j], sa[j]) * (&sl.x)[j];
-          m.gu[(c0 + j) * OP + t] = fmaf((&dt.x)[j], sb[j], skip[j] * gy);
-          m.gd[(c0 + j) * OP + t] = dd;
-          dskip[j] = fmaf(gy, uj, dskip[j]);
-          dbias[j] += dd;
+        for (int i = 0; i < kLeftN; ++i) {
+          const int c = c0 + ln / kEach * kLeftN + i, at = t * CT + c;
+          const float gy = m.go[at], uj = m.u[at];
+          const float sbv = z[2 * i], dd = fmaf(uj, sbv, z[2 * i + 1] * unscaled<T>()) * m.slope[at];
+          m.u[at] = m.dt[at] * sbv;
+          m.slope[at] = dd;
+          (i & 1 ? dskip[i / 2].y : dskip[i / 2].x) += gy * uj;
+          (i & 1 ? dbias[i / 2].y : dbias[i / 2].x) += dd;
         }
       }
     }
-    if (warp == 0) put(m.rcarry + (parity ^ 1) * kND * 32, r);
+    if (warp == 0) put(m.rcarry + (turn ^ 1) * kND * 32, r);
     __syncthreads();
     // the superchunk's results
-    for (int i = threadIdx.x; i < chans * kTS; i += kThreads) {
-      const int d = i / kTS, t = i % kTS;
-      if (t0 + t >= s.L) continue;
-      const bool inside = t0 + t < len;
-      stf(gu + d * s.L + t0 + t, inside ? m.gu[d * OP + t] : 0.f);
-      stf(gdelta + d * s.L + t0 + t, inside ? m.gd[d * OP + t] : 0.f);
+    for (int i = threadIdx.x; i < 2 * CT * (kTS / 8); i += kThreads) {
+      const int x = i / CT, d = i % CT, c = x / 2 * 8;
+      if (d >= chans) continue;
+      const int64_t t = t0 + c;
+      const float *src = (x & 1 ? m.slope : m.u) + c * CT + d;
+      const float skip = !(x & 1) && a.skip ? a.skip[d0 + d] : 0.f;
+      float o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        o[j] = src[j * CT];
+        if (!(x & 1)) o[j] = fmaf(skip, m.go[(c + j) * CT + d], o[j]);
+        if (t + j >= end) o[j] = 0.f;
+      }
+      T *row = (x & 1 ? gdelta : gu) + d * s.L;
+      if (a.vec) row_store8_until<T, true>(row, t, to, o);
+      else row_store8_until<T, false>(row, t, to, o);
     }
-    for (int i = threadIdx.x; i < s.N * kTS; i += kThreads) {
-      const int n = i / kTS, t = i % kTS;
-      if (t0 + t >= s.L) continue;
-      const bool inside = t0 + t < len;
-      pb[n * s.L + t0 + t] = inside ? m.gb[n * OP + t] : 0.f;
-      pc[n * s.L + t0 + t] = inside ? m.gc[n * OP + t] : 0.f;
+    for (int i = threadIdx.x; i < 2 * s.N * (kTS / 8); i += kThreads) {
+      const int x = i / (kTS / 8), n = x >> 1, c = i % (kTS / 8) * 8;
+      const int64_t t = t0 + c;
+      const float *src = (x & 1 ? m.gc : m.gb) + n * kOP + c;
+      alignas(16) float o[8];
+      *reinterpret_cast<float4 *>(o) = *reinterpret_cast<const float4 *>(src);
+      *reinterpret_cast<float4 *>(o + 4) = *reinterpret_cast<const float4 *>(src + 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (t + j >= end) o[j] = 0.f;
+      float *row = (x & 1 ? pc : pb) + n * s.L;
+      if (s.L % 8 == 0) row_store8_until<float, true>(row, t, to, o);
+      else row_store8_until<float, false>(row, t, to, o);
     }
   }
+  if (PRE) {
+    if (warp) return;
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int i = 0; i < kNS; ++i)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int c = c0 + 2 * p + x;
+          if (c >= chans || n0 + i >= s.N) continue;
+          const int64_t at = split * nst + (row0 + c) * s.N + n0 + i;
+          a.rend[at] = x ? r[p][i].y : r[p][i].x;
+          a.prod[at] = x ? total[p][i].y : total[p][i].x;
+        }
+    return;
+  }
   // padded positions behind the last superchunk
-  const int64_t from = (int64_t)supers * kTS;
-  if (from < s.L) {
+  const int64_t rest = from + (int64_t)supers * kTS;
+  if (rest < to) {
     for (int d = warp; d < chans; d += kWarps)
-      for (int64_t t = from + lane; t < s.L; t += 32) {
+      for (int64_t t = rest + lane; t < to; t += 32) {
         stf(gu + d * s.L + t, 0.f);
         stf(gdelta + d * s.L + t, 0.f);
       }
     for (int n = warp; n < s.N; n += kWarps)
-      for (int64_t t = from + lane; t < s.L; t += 32) pb[n * s.L + t] = pc[n * s.L + t] = 0.f;
+      for (int64_t t = rest + lane; t < to; t += 32) pb[n * s.L + t] = pc[n * s.L + t] = 0.f;
   }
-  if (a.ginit && warp == 0) {
+  if (a.ginit && split == 0 && warp == 0) {
 #pragma unroll
-    for (int e = 0; e < kST; ++e) {
-      const int j = e / kNS, n = n0 + e % kNS;
-      if (c0 + j < chans && n < s.N) a.ginit[(row0 + c0 + j) * s.N + n] = r[e];
-    }
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int i = 0; i < kNS; ++i)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int c = c0 + 2 * p + x;
+          if (c < chans && n0 + i < s.N)
+            a.ginit[(row0 + c) * s.N + n0 + i] = x ? r[p][i].y : r[p][i].x;
+        }
   }
   // sums over the warps
   __syncthreads();
   put(m.end + warp * kND * 32, dA);
-  m.prod[warp * 32 + lane] = make_float4(dskip[0], dskip[1], dskip[2], dskip[3]);
-  m.rend[warp * 32 + lane] = make_float4(dbias[0], dbias[1], dbias[2], dbias[3]);
+  m.prod[warp * 32 + lane] = quad(dskip[0], dskip[1]);
+  m.rend[warp * 32 + lane] = quad(dbias[0], dbias[1]);
   __syncthreads();
+  float *pa = a.part_a + (split * s.B + b) * s.D * s.N;
   for (int i = threadIdx.x; i < CT * NP; i += kThreads) {
     const int d = i / NP, n = i % NP;
     if (d >= chans || n >= s.N) continue;
-    const int j = d % kND, l = d / kND * LPC + n / kNS;
+    // put's place of pair p, state n % 4, channel d % 2
+    const int p = d % kND / 2, j = n % kNS, l = d / kND * LPC + n / kNS;
     float v = 0.f;
     for (int w = 0; w < kWarps; ++w)
-      v += reinterpret_cast<const float *>(m.end + (w * kND + j) * 32 + l)[n % kNS];
-    a.part_a[b * s.D * s.N + (d0 + d) * s.N + n] = v;
+      v += reinterpret_cast<const float *>(m.end + (w * kND + 2 * p + j / 2) * 32 + l)[j % 2 * 2 + d % 2];
+    pa[(d0 + d) * s.N + n] = v;
   }
+  using SumN = Scatter<1, LPC, 2 * kND, 2>;
+  constexpr int kLeftN = SumN::kLeft / 2, kOwners = kND / kLeftN, kEach = LPC / kOwners;
   for (int d = threadIdx.x; d < chans; d += kThreads) {
-    const int j = d % kND, l = d / kND * LPC;
+    const int l = d / kND * LPC + d % kND / kLeftN * kEach, j = d % kND % kLeftN;
     float v = 0.f, w = 0.f;
     for (int k = 0; k < kWarps; ++k) {
       v += reinterpret_cast<const float *>(m.prod + k * 32 + l)[j];
       w += reinterpret_cast<const float *>(m.rend + k * 32 + l)[j];
     }
-    a.part_d[b * s.D + d0 + d] = v;
-    a.part_d[(s.B + b) * s.D + d0 + d] = w;
+    a.part_d[(split * s.B + b) * s.D + d0 + d] = v;
+    a.part_d[((a.splits + split) * s.B + b) * s.D + d0 + d] = w;
   }
 }
 
@@ -378,21 +477,21 @@ scan_sum_parts_kernel(const float *__restrict__ pb, const float *__restrict__ pc
   }
 }
 
-// dA, dskip, ddelta_bias: the sum over the batch, in order
+// dA, dskip, ddelta_bias: the sum over batch and chunks, in order
 __global__ void __launch_bounds__(256)
 scan_param_kernel(const float *__restrict__ pa, const float *__restrict__ pd, float *ga,
-                  float *gskip, float *gbias, int64_t B, int64_t D, int64_t N) {
+                  float *gskip, float *gbias, int64_t parts, int64_t D, int64_t N) {
   const int64_t i = blockIdx.x * 256ll + threadIdx.x;
   if (i < D * N) {
     float v = 0.f;
-    for (int64_t b = 0; b < B; ++b) v += pa[b * D * N + i];
+    for (int64_t b = 0; b < parts; ++b) v += pa[b * D * N + i];
     ga[i] = v;
   }
   if (i < D) {
     float v = 0.f, w = 0.f;
-    for (int64_t b = 0; b < B; ++b) {
+    for (int64_t b = 0; b < parts; ++b) {
       v += pd[b * D + i];
-      w += pd[(B + b) * D + i];
+      w += pd[(parts + b) * D + i];
     }
     if (gskip) gskip[i] = v;
     if (gbias) gbias[i] = w;
@@ -403,6 +502,30 @@ int64_t channel_tiles(int64_t D, int64_t N, int64_t G) {
   return cdiv(D / G, 32 / lanes_per_channel(N) * kND);
 }
 
+// as the forward's chunks, with one block to an SM
+int bwd_splits(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G, int64_t *chunk) {
+  const int64_t blocks = B * G * channel_tiles(D, N, G), places = sm_count();
+  const int64_t supers = cdiv(L, kTS);
+  int64_t n = blocks * 2 <= places ? places / blocks : 1;
+  if (n > supers) n = supers;
+  *chunk = cdiv(supers, n) * kTS;
+  return (int)cdiv(L, *chunk);
+}
+
+struct Sizes {
+  int64_t chunk, splits, bc, a, d, st;  // floats: each of part_b, part_c; part_a; part_d; rend, prod
+  size_t bytes() const { return (size_t)(2 * bc + a + d + 2 * st) * sizeof(float); }
+};
+Sizes bwd_sizes(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G) {
+  Sizes z;
+  z.splits = bwd_splits(B, D, L, N, G, &z.chunk);
+  z.bc = cdiv(channel_tiles(D, N, G) * B * G * N * L, 4) * 4;
+  z.a = z.splits * B * D * N;
+  z.d = 2 * z.splits * B * D;
+  z.st = z.splits > 1 ? z.splits * B * D * N : 0;
+  return z;
+}
+
 struct Outs {
   void *gB, *gC;
   float *gA, *gskip, *gbias;
@@ -410,12 +533,19 @@ struct Outs {
 
 template <typename T, int LPC>
 int bwd_launch(const Bwd &a, const Outs &o, const Shape &s, cudaStream_t st) {
-  const size_t smem = sizeof(BwdSmem<T, LPC>);
-  auto kern = scan_bwd_kernel<T, LPC>;
-  if (set_smem_once((const void *)kern, (int)smem) != cudaSuccess)
-    return check_launch("scan_bwd_kernel shared memory");
+  const int smem = (int)sizeof(BwdTile<T, LPC>);
+  auto main = scan_bwd_kernel<T, LPC, false>, pre = scan_bwd_kernel<T, LPC, true>;
   const int64_t tiles = channel_tiles(s.D, s.N, s.G);
-  kern<<<(unsigned)(s.B * s.G * tiles), kThreads, smem, st>>>(a, s);
+  const unsigned blocks = (unsigned)(s.B * s.G * tiles * a.splits);
+  if (a.splits > 1) {
+    if (set_smem_once((const void *)pre, smem) != cudaSuccess)
+      return check_launch("scan_bwd_kernel shared memory");
+    pre<<<blocks, kThreads, smem, st>>>(a, s);
+    if (int rc = check_launch("scan_bwd_kernel (chunk ends)")) return rc;
+  }
+  if (set_smem_once((const void *)main, smem) != cudaSuccess)
+    return check_launch("scan_bwd_kernel shared memory");
+  main<<<blocks, kThreads, smem, st>>>(a, s);
   if (int rc = check_launch("scan_bwd_kernel")) return rc;
   const int64_t n = s.B * s.G * s.N * s.L, cap = 8 * (int64_t)sm_count();
   const dim3 grid((unsigned)(cdiv(n, 256) < cap ? cdiv(n, 256) : cap), 2);
@@ -423,7 +553,7 @@ int bwd_launch(const Bwd &a, const Outs &o, const Shape &s, cudaStream_t st) {
                                                   tiles);
   if (int rc = check_launch("scan_sum_parts_kernel")) return rc;
   scan_param_kernel<<<(unsigned)cdiv(s.D * s.N, 256), 256, 0, st>>>(
-      a.part_a, a.part_d, o.gA, o.gskip, o.gbias, s.B, s.D, s.N);
+      a.part_a, a.part_d, o.gA, o.gskip, o.gbias, s.B * a.splits, s.D, s.N);
   return check_launch("scan_param_kernel");
 }
 
@@ -437,8 +567,7 @@ size_t dudy_selective_scan_backward_workspace_size(int64_t B, int64_t D, int64_t
                                                    int64_t G, int dtype) {
   using namespace dudy;
   if (scan::validate(B, D, L, N, G, dtype)) return 0;
-  const int64_t parts = 2 * scan::channel_tiles(D, N, G) * B * G * N * L;
-  return ((size_t)(parts + B * D * N + 2 * B * D) * sizeof(float) + 255) & ~size_t(255);
+  return (scan::bwd_sizes(B, D, L, N, G).bytes() + 255) & ~size_t(255);
 }
 
 int dudy_selective_scan_backward(const void *go, const float *grad_final, const void *u,
@@ -460,13 +589,14 @@ int dudy_selective_scan_backward(const void *go, const float *grad_final, const 
                                  dudy_selective_scan_backward_workspace_size(B, D, L, N, G, dtype)))
     return rc;
   if (int rc = require_sm100()) return rc;
-  const int64_t tiles = scan::channel_tiles(D, N, G), n = B * G * N * L;
-  float *ws = (float *)workspace;
+  const scan::Sizes z = scan::bwd_sizes(B, D, L, N, G);
+  float *pb = (float *)workspace, *pa = pb + 2 * z.bc, *pd = pa + z.a, *rend = pd + z.d;
   const int vec = L % 8 == 0 && aligned_to_16(u) && aligned_to_16(delta) && aligned_to_16(go) &&
-                  aligned_to_16(Bm) && aligned_to_16(Cm);
+                  aligned_to_16(Bm) && aligned_to_16(Cm) && aligned_to_16(grad_u) &&
+                  aligned_to_16(grad_delta);
   const scan::Bwd a{go, u, delta, Bm, Cm, grad_final, A, skip, delta_bias, checkpoints, lengths,
-                    grad_u, grad_delta, grad_state, ws, ws + tiles * n, ws + 2 * tiles * n,
-                    ws + 2 * tiles * n + B * D * N, vec};
+                    grad_u, grad_delta, grad_state, pb, pb + z.bc, pa, pd, rend, rend + z.st,
+                    z.chunk, (int)z.splits, vec};
   const scan::Outs o{grad_B, grad_C, grad_A, grad_skip, grad_delta_bias};
   const scan::Shape s{B, D, L, (int)N, (int)G, softplus};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
