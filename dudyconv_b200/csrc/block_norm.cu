@@ -241,55 +241,12 @@ constexpr int kTileThreads = 512;
 constexpr int kV = 4;  // tokens of a thread
 
 template <typename T>
-struct Four {  // four neighbouring elements as they lie in memory
-  uint2 q;
-  __device__ __forceinline__ void get(float (&v)[kV]) const {
-    const T *e = reinterpret_cast<const T *>(&q);
-#pragma unroll
-    for (int i = 0; i < kV; ++i) v[i] = Elem<T>::to_f(e[i]);
-  }
-  __device__ __forceinline__ void set(const float (&v)[kV]) {
-    T *e = reinterpret_cast<T *>(&q);
-#pragma unroll
-    for (int i = 0; i < kV; ++i) e[i] = Elem<T>::from_f(v[i]);
-  }
-};
-template <>
-struct Four<float> {
-  float4 q;
-  __device__ __forceinline__ void get(float (&v)[kV]) const {
-    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-  }
-  __device__ __forceinline__ void set(const float (&v)[kV]) {
-    q = make_float4(v[0], v[1], v[2], v[3]);
-  }
-};
-
-// vec: rows start on a four-element boundary, so all four tokens exist or none does.
-template <typename T>
-__device__ __forceinline__ Four<T> load4(const T *p, int64_t left, bool vec) {
-  Four<T> f;
-  if (vec) {
-    f = *reinterpret_cast<const Four<T> *>(p);
-  } else {
-    T *e = reinterpret_cast<T *>(&f);
-#pragma unroll
-    for (int i = 0; i < kV; ++i) e[i] = i < left ? p[i] : Elem<T>::from_f(0.f);
-  }
-  return f;
-}
+using Four = RowFour<T>;
 
 template <typename T>
-__device__ __forceinline__ void store4(T *p, int64_t left, const float (&v)[kV], bool vec) {
-  if (vec) {
-    Four<T> f;
-    f.set(v);
-    *reinterpret_cast<Four<T> *>(p) = f;
-  } else {
+__device__ __forceinline__ void get4(const Four<T> &f, float (&v)[kV]) {
 #pragma unroll
-    for (int i = 0; i < kV; ++i)
-      if (i < left) stf(p + i, v[i]);
-  }
+  for (int i = 0; i < kV; ++i) v[i] = f.get(i);
 }
 
 struct TileRed {
@@ -344,9 +301,9 @@ block_norm_fwd_tile_kernel(NormFwd a, NormShape s, bool vec) {
   for (int i = 0; i < ROWS; ++i) {
     const int64_t d = ty + i * TY;
     if (in && d < s.D) {
-      xr[i] = load4(xp + d * s.L, left, vec);
-      if (zp) zr[i] = load4(zp + d * s.L, left, vec);
-      rr[i] = load4(rp + d * s.L, left, vec);
+      row_load4(xr[i], xp + d * s.L, 0, left, vec);
+      if (zp) row_load4(zr[i], zp + d * s.L, 0, left, vec);
+      row_load4(rr[i], rp + d * s.L, 0, left, vec);
     }
   }
   float g[ROWS][kV], m1[kV], m2[kV], q[kV];
@@ -356,10 +313,10 @@ block_norm_fwd_tile_kernel(NormFwd a, NormShape s, bool vec) {
   for (int i = 0; i < ROWS; ++i) {
     const bool ok = in && ty + i * TY < s.D;
     if (ok) {
-      xr[i].get(g[i]);
+      get4(xr[i], g[i]);
       if (zp) {
         float z[kV];
-        zr[i].get(z);
+        get4(zr[i], z);
 #pragma unroll
         for (int k = 0; k < kV; ++k) g[i][k] *= z[k] * sigmoid_for<T>(z[k]);
       }
@@ -402,11 +359,11 @@ block_norm_fwd_tile_kernel(NormFwd a, NormShape s, bool vec) {
       const float w = ldf((const T *)a.w1 + d), o = LAYER ? opt((const T *)a.b1, d, 0.f) : 0.f;
       const float c = opt((const T *)a.scale, d, 1.f);
       float r[kV];
-      rr[i].get(r);
+      get4(rr[i], r);
 #pragma unroll
       for (int k = 0; k < kV; ++k)
         g[i][k] = fmaf(c, fmaf((g[i][k] - m1[k]) * inv1[k], w, o), r[k]);
-      store4((R *)a.rout + base + d * s.L, left, g[i], vec);
+      row_store4((R *)a.rout + base + d * s.L, 0, left, g[i], vec);
     }
 #pragma unroll
     for (int k = 0; k < kV; ++k) m2[k] += g[i][k];
@@ -428,7 +385,7 @@ block_norm_fwd_tile_kernel(NormFwd a, NormShape s, bool vec) {
     float y[kV];
 #pragma unroll
     for (int k = 0; k < kV; ++k) y[k] = fmaf((g[i][k] - m2[k]) * q[k], w, o);
-    store4((T *)a.y + base + d * s.L, left, y, vec);
+    row_store4((T *)a.y + base + d * s.L, 0, left, y, vec);
   }
   if (a.stats && ty == 0) {
     const int64_t n = s.B * s.L, at = b * s.L + t;
@@ -511,11 +468,11 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, int64_t ntiles, bool vec) {
           cp_async<sizeof(Four<T>)>(&m.gy[i][tid], (const T *)a.gy + o);
           if (a.grout) cp_async<sizeof(Four<R>)>(&m.gr[i][tid], (const R *)a.grout + o);
         } else {
-          m.x[i][tid] = load4((const T *)a.x + o, left, false);
-          if (a.gate) m.z[i][tid] = load4((const T *)a.gate + o, left, false);
-          m.r[i][tid] = load4((const R *)a.residual + o, left, false);
-          m.gy[i][tid] = load4((const T *)a.gy + o, left, false);
-          if (a.grout) m.gr[i][tid] = load4((const R *)a.grout + o, left, false);
+          row_load4(m.x[i][tid], (const T *)a.x + o, 0, left, false);
+          if (a.gate) row_load4(m.z[i][tid], (const T *)a.gate + o, 0, left, false);
+          row_load4(m.r[i][tid], (const R *)a.residual + o, 0, left, false);
+          row_load4(m.gy[i][tid], (const T *)a.gy + o, 0, left, false);
+          if (a.grout) row_load4(m.gr[i][tid], (const R *)a.grout + o, 0, left, false);
         }
       }
     cp_async_commit();
@@ -550,10 +507,10 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, int64_t ntiles, bool vec) {
     for (int i = 0; i < ROWS; ++i) {
       const bool ok = in && ty + i * TY < s.D;
       float x[kV], z[kV], r[kV], gy[kV];
-      m.x[i][tid].get(x);
-      m.r[i][tid].get(r);
-      m.gy[i][tid].get(gy);
-      if (a.gate) m.z[i][tid].get(z);
+      get4(m.x[i][tid], x);
+      get4(m.r[i][tid], r);
+      get4(m.gy[i][tid], gy);
+      if (a.gate) get4(m.z[i][tid], z);
 #pragma unroll
       for (int k = 0; k < kV; ++k) {
         float g = x[k];
@@ -587,8 +544,8 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, int64_t ntiles, bool vec) {
       const int64_t d = ty + i * TY;
       const bool ok = in && d < s.D;
       float gy[kV], gr[kV], dr[kV];
-      m.gy[i][tid].get(gy);
-      if (a.grout) m.gr[i][tid].get(gr);
+      get4(m.gy[i][tid], gy);
+      if (a.grout) get4(m.gr[i][tid], gr);
 #pragma unroll
       for (int k = 0; k < kV; ++k) {
         const float up = a.grout ? gr[k] : 0.f;
@@ -601,7 +558,7 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, int64_t ntiles, bool vec) {
         acc[2][i] = fmaf(dr[k], fmaf(hat1[i][k], w1[i], b1[i]), acc[2][i]);
         if (LAYER) acc[3][i] += dp;
       }
-      if (ok) store4((R *)a.gresidual + base + d * s.L, left, dr, vec);
+      if (ok) row_store4((R *)a.gresidual + base + d * s.L, 0, left, dr, vec);
     }
     tile_sum4<TX>(v, red, turn);
     if (LAYER) tile_sum4<TX>(u, red, turn);
@@ -615,8 +572,8 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, int64_t ntiles, bool vec) {
       const int64_t d = ty + i * TY;
       if (!in || d >= s.D) continue;
       float x[kV], z[kV], gx[kV], gz[kV];
-      m.x[i][tid].get(x);
-      if (a.gate) m.z[i][tid].get(z);
+      get4(m.x[i][tid], x);
+      if (a.gate) get4(m.z[i][tid], z);
 #pragma unroll
       for (int k = 0; k < kV; ++k) {
         const float dg = inv1[k] * (fmaf(-hat1[i][k], v[k], hat2[i][k]) - u[k]);
@@ -627,8 +584,8 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, int64_t ntiles, bool vec) {
           gz[k] = h * x[k] * fmaf(z[k], 1.f - sg[i][k], 1.f);
         }
       }
-      store4((T *)a.gx + base + d * s.L, left, gx, vec);
-      if (a.gate) store4((T *)a.ggate + base + d * s.L, left, gz, vec);
+      row_store4((T *)a.gx + base + d * s.L, 0, left, gx, vec);
+      if (a.gate) row_store4((T *)a.ggate + base + d * s.L, 0, left, gz, vec);
     }
     if (Tile::kStages == 2) at ^= 1;
     else if (tile + gridDim.x < ntiles) fetch(tile + gridDim.x, stage[0]);

@@ -62,6 +62,85 @@ __device__ __forceinline__ void row_store8_until(T *row, int64_t t, int64_t end,
     if (t + i < end) stf(row + t + i, v[i]);
 }
 
+// ---- four positions of a row, as they lie in memory --------------------------------------------
+// Kept in whole 32-bit words from the load on, also where the elements are loaded one by one: the
+// conversion waits until get(), so loads that come early stay in flight.
+template <typename T>
+struct RowFour;
+template <>
+struct RowFour<float> {
+  uint32_t w[4];
+  __device__ __forceinline__ float get(int i) const { return __uint_as_float(w[i]); }
+  __device__ __forceinline__ void load_all(const float *p) {
+    const uint4 q = *reinterpret_cast<const uint4 *>(p);
+    w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+  }
+  __device__ __forceinline__ void load_some(const float *p, int n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = i < n ? reinterpret_cast<const uint32_t *>(p)[i] : 0u;
+  }
+};
+template <typename T>
+struct RowFour {
+  uint32_t w[2];
+  __device__ __forceinline__ float get(int i) const {
+    const uint16_t h = (uint16_t)(w[i >> 1] >> (i & 1 ? 16 : 0));
+    return Elem<T>::to_f(*reinterpret_cast<const T *>(&h));
+  }
+  __device__ __forceinline__ void load_all(const T *p) {
+    const uint2 q = *reinterpret_cast<const uint2 *>(p);
+    w[0] = q.x; w[1] = q.y;
+  }
+  __device__ __forceinline__ void load_some(const T *p, int n) {
+    const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+    w[0] = (n > 0 ? (uint32_t)h[0] : 0u) | (n > 1 ? (uint32_t)h[1] << 16 : 0u);
+    w[1] = (n > 2 ? (uint32_t)h[2] : 0u) | (n > 3 ? (uint32_t)h[3] << 16 : 0u);
+  }
+  __device__ __forceinline__ void set(const float (&v)[4]) {
+    T e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = Elem<T>::from_f(v[i]);
+    const uint16_t *h = reinterpret_cast<const uint16_t *>(e);
+    w[0] = (uint32_t)h[0] | (uint32_t)h[1] << 16;
+    w[1] = (uint32_t)h[2] | (uint32_t)h[3] << 16;
+  }
+  __device__ __forceinline__ void store_all(T *p) const {
+    *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+  }
+};
+
+// row[t .. t+4), zero at and behind `end`, which is not read. `vec`: rows and t start on four
+// elements.
+template <typename T>
+__device__ __forceinline__ void row_load4(RowFour<T> &f, const T *row, int64_t t, int64_t end,
+                                          bool vec) {
+  if (vec && t + 4 <= end) {
+    f.load_all(row + t);
+  } else {
+    const int64_t n = end - t;
+    f.load_some(row + t, n < 0 ? 0 : (n > 4 ? 4 : (int)n));
+  }
+}
+
+// row[t .. t+4) = v, before `end`
+template <typename T>
+__device__ __forceinline__ void row_store4(T *row, int64_t t, int64_t end, const float (&v)[4],
+                                           bool vec) {
+  if (vec && t + 4 <= end) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4 *>(row + t) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      RowFour<T> f;
+      f.set(v);
+      f.store_all(row + t);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (t + i < end) stf(row + t + i, v[i]);
+  }
+}
+
 // ---- activations --------------------------------------------------------------------------
 // 1 / (1 + exp(-v)); 16-bit tensors use the fast exponential and division (relative error
 // about 2^-21, far below the rounding of the result), fp32 tensors the accurate ones.

@@ -4,18 +4,25 @@
 //   h[t] = exp(dt A) h[t-1] + dt u B[t]           per channel d and state n
 //   y[t] = sum_n C[t] h[t] + skip u
 // A thread owns four neighbouring states n of two or four channels; LPC lanes hold a channel's
-// states (N <= 4 LPC, padded with A = B = C = 0, which add nothing). Time is cut into
-// superchunks: the warps of a block take consecutive pieces of one, run the recurrence from
-// zero, exchange their end states and decay products through shared memory and run it again
-// from the state that enters their piece, with the decays kept in registers. So each
-// exponential is computed once: the special function unit (16 a clock and SM, 59 us for the
-// 268 M of B=16, D=256, L=4096, N=16) bounds the forward, not HBM (17 us).
+// states (N <= 4 LPC, padded with A = B = C = 0, which add nothing). The warps of a block take
+// consecutive pieces of its sequence in turn, each on its own: a warp copies its piece's
+// inputs, forms the decays exp(dt A) of all its positions (in registers), runs the recurrence
+// from zero, and only then waits for the state that enters the piece. One multiply-add a state
+// (the piece's decay product times what enters, plus its own end state) gives what it hands on
+// to the next warp; it runs the recurrence again from the true state, for its outputs or
+// gradients, while that one goes on. So each exponential is computed once, the chain from warp
+// to warp is a few dozen instructions a piece, and no barrier joins the whole block:
+// consecutive warps meet in pairs (bar.arrive / bar.sync on a barrier per neighbours, never two
+// arrivals ahead, since the chain goes round the block before a warp arrives there again).
+// Waiting before the recurrence instead, and running it once, made the chain the bound: 222
+// and 861 us at the sizes below.
+// The special function unit (16 a clock and SM, 59 us for the 268 M exponentials of B=16,
+// D=256, L=4096, N=16) bounds the forward, not HBM (17 us).
 //
-// Where there are too few rows of channels to fill the GPU, the sequence is cut once more, into
-// `splits` chunks of whole superchunks, a block to each: a first kernel finds each chunk's end
-// state from zero and its decay product, and the main kernel's block folds those of the chunks
-// before its own into the state that it starts from. That doubles the exponentials and divides
-// the steps in a row by `splits`.
+// Where there are too few rows of channels to fill the GPU, the sequence is cut into `splits`
+// chunks, a block to each: a first kernel finds each chunk's end state from zero and its decay
+// product, and the main kernel's block folds those of the chunks before its own into the state
+// that it starts from. That doubles the exponentials and divides the steps in a row by `splits`.
 //
 // All arithmetic is fp32, two at a time where pairs lie side by side (__ffma2_rn).
 #pragma once
@@ -30,7 +37,7 @@ namespace scan {
 constexpr int kNS = 4;        // states of a thread, neighbours in n
 constexpr int kWarps = 8;     // warps of a block: consecutive pieces of a superchunk
 constexpr int kThreads = 32 * kWarps;
-constexpr int kCkpt = 32;     // positions between saved states
+constexpr int kCkpt = 4;      // positions between saved states: a piece of the backward
 constexpr int kMaxN = DUDY_SCAN_MAX_STATE;
 
 struct Shape {
@@ -141,43 +148,12 @@ struct Scatter<STRIDE, 1, N, KEEP> {
   static __device__ __forceinline__ void sum(float *, int) {}
 };
 
-// Copies a tile of `rows` rows x TS positions of a [.., L] tensor into shared memory as it is
-// (pitch PITCH elements): positions [t0, t0 + TS), zero at and behind `end`, and zero rows at
-// and behind `valid`. 16-byte asynchronous copies where rows start on 16 bytes (`vec`).
-template <typename T, int TS, int PITCH>
-__device__ __forceinline__ void stage_rows(T *dst, const T *src, int rows, int valid, int64_t L,
-                                           int64_t t0, int64_t end, bool vec) {
-  constexpr int V = 16 / sizeof(T), VPR = TS / V;
-  for (int i = threadIdx.x; i < rows * VPR; i += kThreads) {
-    const int r = i / VPR, c = (i % VPR) * V;
-    T *to = dst + r * PITCH + c;
-    const int64_t t = t0 + c;
-    if (r < valid && vec && t + V <= end) {
-      cp_async16(to, src + (int64_t)r * L + t);
-    } else {
-#pragma unroll
-      for (int k = 0; k < V; ++k)
-        to[k] = r < valid && t + k < end ? src[(int64_t)r * L + t + k] : Elem<T>::from_f(0.f);
-    }
-  }
+// Two warps meet: one arrives and goes on, the other waits for it.
+__device__ __forceinline__ void pair_wait(int id) {
+  asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory");
 }
-
-// dst[r * PITCH + c] = row r of an fp32 [rows, N] matrix, zero behind N and behind `valid` rows.
-// Asynchronous where N is a multiple of four and src starts on 16 bytes.
-template <int NP>
-__device__ __forceinline__ void stage_states(float *dst, const float *src, int rows, int valid,
-                                             int N) {
-  const bool vec = N % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
-  for (int i = threadIdx.x; i < rows * (NP / 4); i += kThreads) {
-    const int r = i / (NP / 4), c = i % (NP / 4) * 4;
-    float *to = dst + r * NP + c;
-    if (vec && r < valid && c < N) {
-      cp_async16(to, src + r * N + c);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) to[k] = r < valid && c + k < N ? src[r * N + c + k] : 0.f;
-    }
-  }
+__device__ __forceinline__ void pair_arrive(int id) {
+  asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory");
 }
 
 inline int lanes_per_channel(int64_t N) {

@@ -4,10 +4,10 @@
 //   dC[n,t] = sum_d h dy                 dB[n,t] = sum_d g dt u        (channels of the group)
 //   dA[d,n] = sum_{b,t} dt g a h[t-1]    ddt = u sum_n g B + sum_n A g a h[t-1]
 //   du = dt sum_n g B + skip dy          ddelta = ddt softplus'        dskip = sum_{b,t} dy u
-// Superchunks go from the right end of a sequence to its left. Within one, each warp runs its
-// four positions forwards and backwards from zero, the end states of both directions are
-// exchanged together, and it runs both again: forwards keeping the states, backwards forming
-// the gradients. The state that enters a superchunk was saved by the forward.
+// Pieces of four positions go from the right end of a sequence to its left, from warp to warp
+// of a block. The state that enters each was saved by the forward (16 bytes a state for every
+// four positions: HBM has the time, and recovering them here would take a second chain in the
+// other direction), so only g's recurrence runs from piece to piece.
 //
 // The sums over channels set the layout: a thread holds four channels x four states, so that
 // most of a sum over channels or states happens in its registers and only the rest by
@@ -21,10 +21,8 @@ namespace scan {
 namespace {
 
 constexpr int kND = 4;                 // channels of a thread
-constexpr int kQ = 4;                  // positions of a warp in a superchunk
-constexpr int kTS = kWarps * kQ;       // positions of a superchunk
-constexpr int kOP = kTS + 4;
-static_assert(kTS == kCkpt, "a state is saved at each superchunk's start");
+constexpr int kQ = 4;                  // positions of a piece
+static_assert(kQ == kCkpt, "a state is saved at each piece's start");
 
 struct Bwd {
   const void *go, *u, *delta, *Bm, *Cm;
@@ -37,26 +35,28 @@ struct Bwd {
   float *part_d;           // [2][splits][B][D]: skip, delta_bias
   float *rend, *prod;      // [splits][B*D][N]: what a chunk passes to its left from zero, and its
                            // decays' product
-  int64_t chunk;           // positions of a chunk, a multiple of kTS
+  int64_t chunk;           // positions of a chunk, a multiple of kQ
   int splits, vec;
 };
 
-template <typename T, int LPC>
-struct BwdTile {
+// a warp's own piece, positions outermost
+template <int LPC>
+struct BwdPiece {
   static constexpr int CT = 32 / LPC * kND;      // channels of a block
   static constexpr int NP = kNS * LPC;
-  static constexpr int PITCH = kTS + 16 / (int)sizeof(T);
-  T raw_u[CT * PITCH], raw_d[CT * PITCH], raw_g[CT * PITCH];
-  T raw_b[NP * PITCH], raw_c[NP * PITCH];
-  float dt[kTS * CT], du[kTS * CT], go[kTS * CT];
-  float u[kTS * CT], slope[kTS * CT];            // du's and ddelta's results take their places
-  float2 b[kTS * NP], c[kTS * NP];               // each twice side by side
-  float gb[NP * kOP], gc[NP * kOP];
-  float h0[2][CT * NP];                          // the states saved at the superchunk's start
-  // exchanged states, [warp][four of the thread's states][lane]: forward end, decay product and
-  // backward end; the sums over warps at the end use the same room
-  float4 end[kWarps * kND * 32], prod[kWarps * kND * 32], rend[kWarps * kND * 32];
-  float4 rcarry[2 * kND * 32];
+  static constexpr int UI = (CT + 31) / 32;      // rows of u, delta and dy that a lane copies
+  static constexpr int BI = (2 * NP + 31) / 32;  // rows of B and C
+  float dt[kQ * CT], du[kQ * CT], go[kQ * CT];
+  float u[kQ * CT], slope[kQ * CT];              // du's and ddelta's results take their places
+  float bc[kQ * 2 * NP];                         // B and C of a position side by side
+  float h0[2][CT * NP];                          // the states that enter this piece and the next
+};
+template <int LPC>
+struct BwdSmem {
+  BwdPiece<LPC> piece[kWarps];
+  // handed on to the left, [warp][four of the thread's states][lane] (with the chunk's decay
+  // product so far); the sums over warps at the end use the same room
+  float4 pass[kWarps * kND * 32], total[kWarps * kND * 32];
 };
 
 // A thread's states lie in pairs of channels: e[p][n] holds channels 2p and 2p + 1 of state n,
@@ -64,12 +64,13 @@ struct BwdTile {
 template <typename T, int LPC, bool PRE>
 __global__ void __launch_bounds__(kThreads, 1)
 scan_bwd_kernel(Bwd a, Shape s) {
-  using Tile = BwdTile<T, LPC>;
-  constexpr int CT = Tile::CT, NP = Tile::NP, PITCH = Tile::PITCH;
+  using Mine = BwdPiece<LPC>;
+  constexpr int CT = Mine::CT, NP = Mine::NP;
   extern __shared__ __align__(16) char smem_raw[];
-  Tile &m = *reinterpret_cast<Tile *>(smem_raw);
+  BwdSmem<LPC> &all = *reinterpret_cast<BwdSmem<LPC> *>(smem_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ln = lane % LPC, ld = lane / LPC, n0 = ln * kNS, c0 = ld * kND;
+  Mine &m = all.piece[warp];
 
   const int split = blockIdx.x % a.splits;
   if (PRE && split == 0) return;  // nothing lies to the left of the first chunk
@@ -88,8 +89,8 @@ scan_bwd_kernel(Bwd a, Shape s) {
   const T *Bm = (const T *)a.Bm + bg * s.N * s.L, *Cm = (const T *)a.Cm + bg * s.N * s.L;
   T *gu = (T *)a.gu + row0 * s.L, *gdelta = (T *)a.gdelta + row0 * s.L;
   const int64_t nbc = s.B * s.G * s.N * s.L, nst = s.B * s.D * s.N;
-  float *pb = a.part_b + tile * nbc + bg * s.N * s.L;
-  float *pc = a.part_c + tile * nbc + bg * s.N * s.L;
+  float *gB = a.part_b + tile * nbc + bg * s.N * s.L;
+  float *gC = a.part_c + tile * nbc + bg * s.N * s.L;
 
   float2 A[2][kNS], dA[2][kNS], r[2][kNS], dskip[2], dbias[2], total[2][kNS];
 #pragma unroll
@@ -105,7 +106,7 @@ scan_bwd_kernel(Bwd a, Shape s) {
         const int64_t at = (row0 + c) * s.N + n0 + i;
         av[x] = ok ? scaled<T>(a.A[(d0 + c) * s.N + n0 + i]) : 0.f;
         rv[x] = 0.f;
-        if (!PRE && ok) {
+        if (!PRE && ok && warp == 0) {
           if (a.gfinal) rv[x] = a.gfinal[at];
           for (int k = a.splits - 1; k > split; --k)
             rv[x] = fmaf(a.prod[k * nst + at], rv[x], a.rend[k * nst + at]);
@@ -124,164 +125,171 @@ scan_bwd_kernel(Bwd a, Shape s) {
       dst[(2 * p + 1) * 32 + lane] = quad(v[p][2], v[p][3]);
     }
   };
-  // v = prod v + add over what a warp put
-  auto fold = [&](float2 (&v)[2][kNS], const float4 *add, const float4 *prod) {
+  auto take = [&](float2 (&v)[2][kNS], const float4 *src) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const float4 x = src[(2 * p) * 32 + lane], z = src[(2 * p + 1) * 32 + lane];
+      v[p][0] = lo(x); v[p][1] = hi(x); v[p][2] = lo(z); v[p][3] = hi(z);
+    }
+  };
+
+  // a lane's channels where it copies them
+  float bias[Mine::UI], skip[Mine::UI];
+#pragma unroll
+  for (int k = 0; k < Mine::UI; ++k) {
+    const int d = lane + k * 32;
+    bias[k] = d < chans && a.delta_bias ? a.delta_bias[d0 + d] : 0.f;
+    skip[k] = !PRE && d < chans && a.skip ? a.skip[d0 + d] : 0.f;
+  }
+  // the warp's next piece, in registers while this one is worked on
+  RowFour<T> pu[Mine::UI], pd[Mine::UI], pg[Mine::UI], pb[Mine::BI];
+  auto fetch = [&](int64_t t0) {
+#pragma unroll
+    for (int k = 0; k < Mine::UI; ++k) {
+      const int d = lane + k * 32;
+      if (d >= CT) break;
+      const int64_t lim = d < chans ? end : 0;
+      if (!PRE) row_load4(pu[k], u + d * s.L, t0, lim, a.vec);
+      row_load4(pd[k], delta + d * s.L, t0, lim, a.vec);
+      row_load4(pg[k], go + d * s.L, t0, lim, a.vec);
+    }
+#pragma unroll
+    for (int k = 0; k < Mine::BI; ++k) {
+      const int r = lane + k * 32, n = r % NP;
+      if (r >= 2 * NP) break;
+      row_load4(pb[k], (r < NP ? Bm : Cm) + n * s.L, t0, n < s.N ? end : 0, a.vec);
+    }
+  };
+  using SumD = Scatter<LPC, 32 / LPC, 2 * kNS>;
+  constexpr int kLeftD = SumD::kLeft, kGroups = 2 * kNS / kLeftD;
+  constexpr int kSame = 32 / LPC / kGroups;  // lanes that end with the same values
+  using SumN = Scatter<1, LPC, 2 * kND, 2>;
+  constexpr int kLeftN = SumN::kLeft / 2, kOwners = kND / kLeftN, kEach = LPC / kOwners;
+  // the states that enter the piece of positions from t0 on
+  auto fetch_states = [&](int64_t t0, float *dst) {
+    const float *src = a.ckpt + ((b * s.ckpts() + t0 / kCkpt) * s.D + d0) * s.N;
+    const bool vec = s.N % 4 == 0;
+#pragma unroll
+    for (int i = lane; i < CT * (NP / 4); i += 32) {
+      const int c = i / (NP / 4), n = i % (NP / 4) * 4;
+      float *to = dst + c * NP + n;
+      if (vec && c < chans && n < s.N) {
+        cp_async16(to, src + c * s.N + n);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = c < chans && n + e < s.N ? src[c * s.N + n + e] : 0.f;
+      }
+    }
+  };
+  // piece k, counted from the right, is warp k % kWarps's
+  const int pieces = end > from ? (int)((end - from + kQ - 1) / kQ) : 0;
+  auto start = [&](int k) { return from + (int64_t)(pieces - 1 - k) * kQ; };
+  int turn = 0;
+  if (warp < pieces) {
+    fetch(start(warp));
+    if (!PRE) fetch_states(start(warp), m.h0[0]);
+  }
+  for (int k = warp; k < pieces; k += kWarps, turn ^= 1) {
+    const int64_t t0 = start(k);
+    if (!PRE) cp_async_wait_all();
+    __syncwarp();
+#pragma unroll
+    for (int p = 0; p < Mine::UI; ++p) {
+      const int d = lane + p * 32;
+      if (d >= CT) break;
+#pragma unroll
+      for (int j = 0; j < kQ; ++j) {
+        float dt = pd[p].get(j) + bias[p], slope = 1.f;
+        if (s.softplus) dt = softplus<T>(dt, slope);
+        if (t0 + j >= end) dt = slope = 0.f;
+        m.dt[j * CT + d] = dt;
+        m.go[j * CT + d] = pg[p].get(j);
+        if (PRE) continue;
+        const float uv = pu[p].get(j);
+        m.du[j * CT + d] = dt * uv;
+        m.u[j * CT + d] = uv;
+        m.slope[j * CT + d] = slope;
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < Mine::BI; ++p) {
+      const int r = lane + p * 32;
+      if (r >= 2 * NP) break;
+#pragma unroll
+      for (int j = 0; j < kQ; ++j) m.bc[j * 2 * NP + r] = pb[p].get(j);
+    }
+    __syncwarp();
+    if (k + kWarps < pieces) {
+      fetch(start(k + kWarps));
+      if (!PRE) fetch_states(start(k + kWarps), m.h0[turn ^ 1]);
+    }
+
+    auto four = [](const float *p) { return *reinterpret_cast<const float4 *>(p); };
+    auto twice = [&](int q, int which, float2 (&v)[kNS]) {
+      const float4 x = four(m.bc + q * 2 * NP + which * NP + n0);
+      v[0] = both(x.x); v[1] = both(x.y); v[2] = both(x.z); v[3] = both(x.w);
+    };
+    // dec[q]: position q's decay
+    float2 dec[kQ][2][kNS], own[2][kNS], prod[2][kNS], bv[kNS], cv[kNS];
+#pragma unroll
+    for (int q = kQ - 1; q >= 0; --q) {
+      const float4 dt = four(m.dt + q * CT + c0), gv = four(m.go + q * CT + c0);
+      twice(q, 1, cv);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const float2 dtp = p ? hi(dt) : lo(dt), gy = p ? hi(gv) : lo(gv);
+#pragma unroll
+        for (int i = 0; i < kNS; ++i) {
+          const float2 x = __fmul2_rn(dtp, A[p][i]);
+          const float2 e = make_float2(decay<T>(x.x), decay<T>(x.y));
+          dec[q][p][i] = e;
+          own[p][i] = __fmul2_rn(e, q == kQ - 1 ? __fmul2_rn(cv[i], gy)
+                                                 : __ffma2_rn(cv[i], gy, own[p][i]));
+          prod[p][i] = q == kQ - 1 ? e : __fmul2_rn(prod[p][i], e);
+        }
+      }
+    }
+    // what enters the piece from the right, and what leaves it to the left
+    if (k > 0) {
+      const int before = (warp + kWarps - 1) % kWarps;
+      pair_wait(1 + before);
+      take(r, all.pass + before * kND * 32);
+      if (PRE) take(total, all.total + before * kND * 32);
+    }
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float4 x = prod[(2 * p + i) * 32 + lane], e = add[(2 * p + i) * 32 + lane];
-        v[p][2 * i] = __ffma2_rn(lo(x), v[p][2 * i], lo(e));
-        v[p][2 * i + 1] = __ffma2_rn(hi(x), v[p][2 * i + 1], hi(e));
-        if (PRE) {
-          total[p][2 * i] = __fmul2_rn(total[p][2 * i], lo(x));
-          total[p][2 * i + 1] = __fmul2_rn(total[p][2 * i + 1], hi(x));
-        }
+      for (int i = 0; i < kNS; ++i) {
+        own[p][i] = __ffma2_rn(prod[p][i], r[p][i], own[p][i]);
+        if (PRE) total[p][i] = __fmul2_rn(total[p][i], prod[p][i]);
       }
-  };
-  if (warp == 0) put(m.rcarry, r);
-
-  auto stage = [&](int64_t t0, int turn) {
-    stage_rows<T, kTS, PITCH>(m.raw_d, delta, CT, chans, s.L, t0, end, a.vec);
-    stage_rows<T, kTS, PITCH>(m.raw_g, go, CT, chans, s.L, t0, end, a.vec);
-    stage_rows<T, kTS, PITCH>(m.raw_c, Cm, NP, s.N, s.L, t0, end, a.vec);
-    if (PRE) return;
-    stage_rows<T, kTS, PITCH>(m.raw_u, u, CT, chans, s.L, t0, end, a.vec);
-    stage_rows<T, kTS, PITCH>(m.raw_b, Bm, NP, s.N, s.L, t0, end, a.vec);
-    stage_states<NP>(m.h0[turn], a.ckpt + ((b * s.ckpts() + t0 / kCkpt) * s.D + d0) * s.N, CT,
-                     chans, s.N);
-  };
-  const int supers = end > from ? (int)((end - from + kTS - 1) / kTS) : 0;
-  if (supers) stage(from + (int64_t)(supers - 1) * kTS, 0);
-  int turn = 0;
-  for (int k = supers - 1; k >= 0; --k, turn ^= 1) {
-    const int64_t t0 = from + (int64_t)k * kTS;
-    cp_async_wait_all();
-    __syncthreads();
-    for (int i = threadIdx.x; i < CT * (kTS / 4); i += kThreads) {
-      const int d = i % CT, c = i / CT * 4;
-      const T *ru = m.raw_u + d * PITCH + c, *rd = m.raw_d + d * PITCH + c;
-      const T *rg = m.raw_g + d * PITCH + c;
-      const float bias = d < chans && a.delta_bias ? a.delta_bias[d0 + d] : 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float dt = Elem<T>::to_f(rd[j]) + bias, slope = 1.f;
-        if (s.softplus) dt = softplus<T>(dt, slope);
-        if (t0 + c + j >= end) dt = slope = 0.f;
-        const int at = (c + j) * CT + d;
-        m.dt[at] = dt;
-        m.go[at] = Elem<T>::to_f(rg[j]);
-        if (PRE) continue;
-        const float uv = Elem<T>::to_f(ru[j]);
-        m.du[at] = dt * uv;
-        m.u[at] = uv;
-        m.slope[at] = slope;
-      }
+    if (k + 1 < pieces) {
+      put(all.pass + warp * kND * 32, own);
+      if (PRE) put(all.total + warp * kND * 32, total);
+      pair_arrive(1 + warp);
     }
-    for (int i = threadIdx.x; i < NP * (kTS / 4); i += kThreads) {
-      const int n = i % NP, c = i / NP * 4;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m.c[(c + j) * NP + n] = both(Elem<T>::to_f(m.raw_c[n * PITCH + c + j]));
-        if (!PRE) m.b[(c + j) * NP + n] = both(Elem<T>::to_f(m.raw_b[n * PITCH + c + j]));
-      }
-    }
-    __syncthreads();
-    if (k > 0) stage(t0 - kTS, turn ^ 1);
-
-    // both directions from zero
-    const float *sdt = m.dt + warp * kQ * CT + c0, *sdu = m.du + warp * kQ * CT + c0;
-    const float *sgo = m.go + warp * kQ * CT + c0;
-    const float2 *sb2 = m.b + warp * kQ * NP + n0, *sc2 = m.c + warp * kQ * NP + n0;
-    auto four = [](const float *p) { return *reinterpret_cast<const float4 *>(p); };
-    auto pairs = [](const float2 *p, float2 (&v)[kNS]) {
-      const float4 x = reinterpret_cast<const float4 *>(p)[0];
-      const float4 z = reinterpret_cast<const float4 *>(p)[1];
-      v[0] = lo(x); v[1] = hi(x); v[2] = lo(z); v[3] = hi(z);
-    };
-    float2 dec[kQ][2][kNS], h[kQ][2][kNS], bv[kNS], cv[kNS];
-    {
-      float2 sum[2], loc[2][kNS];
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        sum[p] = both(0.f);
-#pragma unroll
-        for (int i = 0; i < kNS; ++i) loc[p][i] = both(0.f);
-      }
-#pragma unroll
-      for (int q = 0; q < kQ; ++q) {
-        const float4 dt = four(sdt + q * CT);
-        float4 du;
-        if (!PRE) {
-          du = four(sdu + q * CT);
-          pairs(sb2 + q * NP, bv);
-        }
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const float2 dtp = p ? hi(dt) : lo(dt), dup = p ? hi(du) : lo(du);
-          sum[p] = __fadd2_rn(sum[p], dtp);
-#pragma unroll
-          for (int i = 0; i < kNS; ++i) {
-            const float2 x = __fmul2_rn(dtp, A[p][i]);
-            dec[q][p][i] = make_float2(decay<T>(x.x), decay<T>(x.y));
-            if (!PRE) loc[p][i] = __ffma2_rn(dec[q][p][i], loc[p][i], __fmul2_rn(dup, bv[i]));
-          }
-        }
-      }
-      if (!PRE) put(m.end + warp * kND * 32, loc);
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-#pragma unroll
-        for (int i = 0; i < kNS; ++i) {
-          const float2 x = __fmul2_rn(sum[p], A[p][i]);
-          loc[p][i] = make_float2(decay<T>(x.x), decay<T>(x.y));
-        }
-      put(m.prod + warp * kND * 32, loc);
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-#pragma unroll
-        for (int i = 0; i < kNS; ++i) loc[p][i] = both(0.f);
-#pragma unroll
-      for (int q = kQ - 1; q >= 0; --q) {
-        const float4 gv = four(sgo + q * CT);
-        pairs(sc2 + q * NP, cv);
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-#pragma unroll
-          for (int i = 0; i < kNS; ++i)
-            loc[p][i] = __fmul2_rn(dec[q][p][i], __ffma2_rn(cv[i], p ? hi(gv) : lo(gv), loc[p][i]));
-      }
-      put(m.rend + warp * kND * 32, loc);
-    }
-    __syncthreads();
-    // what enters this warp's positions from the right, and from the left
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const float4 x = m.rcarry[(turn * kND + 2 * p) * 32 + lane];
-      const float4 z = m.rcarry[(turn * kND + 2 * p + 1) * 32 + lane];
-      r[p][0] = lo(x); r[p][1] = hi(x); r[p][2] = lo(z); r[p][3] = hi(z);
-    }
-    for (int w = kWarps - 1; w > (PRE ? (warp ? kWarps : -1) : warp); --w)
-      fold(r, m.rend + w * kND * 32, m.prod + w * kND * 32);
     if (PRE) {
-      if (warp == 0) put(m.rcarry + (turn ^ 1) * kND * 32, r);
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int i = 0; i < kNS; ++i) r[p][i] = own[p][i];
       continue;
     }
+    // h[q]: the state before position q
+    float2 h[kQ + 1][2][kNS];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const float4 x = *reinterpret_cast<const float4 *>(m.h0[turn] + (c0 + 2 * p) * NP + n0);
-      const float4 z = *reinterpret_cast<const float4 *>(m.h0[turn] + (c0 + 2 * p + 1) * NP + n0);
+      const float4 x = four(m.h0[turn] + (c0 + 2 * p) * NP + n0);
+      const float4 z = four(m.h0[turn] + (c0 + 2 * p + 1) * NP + n0);
       h[0][p][0] = make_float2(x.x, z.x);
       h[0][p][1] = make_float2(x.y, z.y);
       h[0][p][2] = make_float2(x.z, z.z);
       h[0][p][3] = make_float2(x.w, z.w);
     }
-    for (int w = 0; w < warp; ++w) fold(h[0], m.end + w * kND * 32, m.prod + w * kND * 32);
-    // forwards: h[q] is the state before position q
 #pragma unroll
-    for (int q = 0; q + 1 < kQ; ++q) {
-      const float4 du = four(sdu + q * CT);
-      pairs(sb2 + q * NP, bv);
+    for (int q = 0; q < kQ; ++q) {
+      const float4 du = four(m.du + q * CT + c0);
+      twice(q, 0, bv);
 #pragma unroll
       for (int p = 0; p < 2; ++p)
 #pragma unroll
@@ -289,13 +297,14 @@ scan_bwd_kernel(Bwd a, Shape s) {
           h[q + 1][p][i] =
               __ffma2_rn(dec[q][p][i], h[q][p][i], __fmul2_rn(p ? hi(du) : lo(du), bv[i]));
     }
-    // backwards
+    // the gradients
+    float dbc[SumD::kLeft][kQ];
 #pragma unroll
     for (int q = kQ - 1; q >= 0; --q) {
-      const int t = warp * kQ + q;
-      const float4 dt = four(sdt + q * CT), du = four(sdu + q * CT), gv = four(sgo + q * CT);
-      pairs(sb2 + q * NP, bv);
-      pairs(sc2 + q * NP, cv);
+      const float4 dt = four(m.dt + q * CT + c0), du = four(m.du + q * CT + c0);
+      const float4 gv = four(m.go + q * CT + c0);
+      twice(q, 0, bv);
+      twice(q, 1, cv);
       float2 db[kNS], dc[kNS], sb[2], sa[2];
 #pragma unroll
       for (int i = 0; i < kNS; ++i) db[i] = dc[i] = both(0.f);
@@ -307,14 +316,13 @@ scan_bwd_kernel(Bwd a, Shape s) {
 #pragma unroll
         for (int i = 0; i < kNS; ++i) {
           const float2 gg = __ffma2_rn(cv[i], gy, r[p][i]);
-          const float2 ah = __fmul2_rn(dec[q][p][i], h[q][p][i]);
-          const float2 w = __fmul2_rn(gg, ah);
-          dc[i] = __ffma2_rn(gy, __ffma2_rn(dup, bv[i], ah), dc[i]);
+          r[p][i] = __fmul2_rn(dec[q][p][i], gg);
+          const float2 w = __fmul2_rn(r[p][i], h[q][p][i]);
+          dc[i] = __ffma2_rn(gy, h[q + 1][p][i], dc[i]);
           db[i] = __ffma2_rn(gg, dup, db[i]);
           sb[p] = __ffma2_rn(gg, bv[i], sb[p]);
           sa[p] = __ffma2_rn(w, A[p][i], sa[p]);
           dA[p][i] = __ffma2_rn(w, dtp, dA[p][i]);
-          r[p][i] = __fmul2_rn(dec[q][p][i], gg);
         }
       }
       // dB, dC: over the lanes across channels; lane ld ends with values ld * left ..
@@ -324,17 +332,9 @@ scan_bwd_kernel(Bwd a, Shape s) {
         v[i] = db[i].x + db[i].y;
         v[kNS + i] = dc[i].x + dc[i].y;
       }
-      using SumD = Scatter<LPC, 32 / LPC, 2 * kNS>;
       SumD::sum(v, lane);
-      constexpr int kLeftD = SumD::kLeft, kGroups = 2 * kNS / kLeftD;
-      constexpr int kSame = 32 / LPC / kGroups;  // lanes that hold the same values
-      if (ld % kSame == 0) {
 #pragma unroll
-        for (int i = 0; i < kLeftD; ++i) {
-          const int at = ld / kSame * kLeftD + i;
-          (at < kNS ? m.gb : m.gc)[(n0 + at % kNS) * kOP + t] = v[i];
-        }
-      }
+      for (int i = 0; i < SumD::kLeft; ++i) dbc[i][q] = v[i];
       // the sums over states: a channel's two values stay together
       float z[2 * kND];
 #pragma unroll
@@ -342,15 +342,14 @@ scan_bwd_kernel(Bwd a, Shape s) {
         z[4 * p] = sb[p].x; z[4 * p + 1] = sa[p].x;
         z[4 * p + 2] = sb[p].y; z[4 * p + 3] = sa[p].y;
       }
-      using SumN = Scatter<1, LPC, 2 * kND, 2>;
       SumN::sum(z, lane);
-      constexpr int kLeftN = SumN::kLeft / 2, kOwners = kND / kLeftN, kEach = LPC / kOwners;
       if (ln % kEach == 0) {
 #pragma unroll
         for (int i = 0; i < kLeftN; ++i) {
-          const int c = c0 + ln / kEach * kLeftN + i, at = t * CT + c;
+          const int at = q * CT + c0 + ln / kEach * kLeftN + i;
           const float gy = m.go[at], uj = m.u[at];
-          const float sbv = z[2 * i], dd = fmaf(uj, sbv, z[2 * i + 1] * unscaled<T>()) * m.slope[at];
+          const float sbv = z[2 * i];
+          const float dd = fmaf(uj, sbv, z[2 * i + 1] * unscaled<T>()) * m.slope[at];
           m.u[at] = m.dt[at] * sbv;
           m.slope[at] = dd;
           (i & 1 ? dskip[i / 2].y : dskip[i / 2].x) += gy * uj;
@@ -358,43 +357,35 @@ scan_bwd_kernel(Bwd a, Shape s) {
         }
       }
     }
-    if (warp == 0) put(m.rcarry + (turn ^ 1) * kND * 32, r);
-    __syncthreads();
-    // the superchunk's results
-    for (int i = threadIdx.x; i < 2 * CT * (kTS / 8); i += kThreads) {
-      const int x = i / CT, d = i % CT, c = x / 2 * 8;
-      if (d >= chans) continue;
-      const int64_t t = t0 + c;
-      const float *src = (x & 1 ? m.slope : m.u) + c * CT + d;
-      const float skip = !(x & 1) && a.skip ? a.skip[d0 + d] : 0.f;
-      float o[8];
+    if (ld % kSame == 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        o[j] = src[j * CT];
-        if (!(x & 1)) o[j] = fmaf(skip, m.go[(c + j) * CT + d], o[j]);
-        if (t + j >= end) o[j] = 0.f;
+      for (int i = 0; i < kLeftD; ++i) {
+        const int at = ld / kSame * kLeftD + i, n = n0 + at % kNS;
+        if (n >= s.N) continue;
+        float o[4];
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) o[q] = t0 + q < end ? dbc[i][q] : 0.f;
+        row_store4((at < kNS ? gB : gC) + n * s.L, t0, to, o, s.L % 4 == 0);
       }
-      T *row = (x & 1 ? gdelta : gu) + d * s.L;
-      if (a.vec) row_store8_until<T, true>(row, t, to, o);
-      else row_store8_until<T, false>(row, t, to, o);
     }
-    for (int i = threadIdx.x; i < 2 * s.N * (kTS / 8); i += kThreads) {
-      const int x = i / (kTS / 8), n = x >> 1, c = i % (kTS / 8) * 8;
-      const int64_t t = t0 + c;
-      const float *src = (x & 1 ? m.gc : m.gb) + n * kOP + c;
-      alignas(16) float o[8];
-      *reinterpret_cast<float4 *>(o) = *reinterpret_cast<const float4 *>(src);
-      *reinterpret_cast<float4 *>(o + 4) = *reinterpret_cast<const float4 *>(src + 4);
+    __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (t + j >= end) o[j] = 0.f;
-      float *row = (x & 1 ? pc : pb) + n * s.L;
-      if (s.L % 8 == 0) row_store8_until<float, true>(row, t, to, o);
-      else row_store8_until<float, false>(row, t, to, o);
+    for (int p = 0; p < Mine::UI; ++p) {
+      const int d = lane + p * 32;
+      if (d >= chans) break;
+      float o[4], w[4];
+#pragma unroll
+      for (int j = 0; j < kQ; ++j) {
+        const bool inside = t0 + j < end;
+        o[j] = inside ? fmaf(skip[p], m.go[j * CT + d], m.u[j * CT + d]) : 0.f;
+        w[j] = inside ? m.slope[j * CT + d] : 0.f;
+      }
+      row_store4(gu + d * s.L, t0, to, o, a.vec);
+      row_store4(gdelta + d * s.L, t0, to, w, a.vec);
     }
   }
   if (PRE) {
-    if (warp) return;
+    if (warp != (pieces ? (pieces - 1) % kWarps : 0)) return;
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
@@ -409,8 +400,8 @@ scan_bwd_kernel(Bwd a, Shape s) {
         }
     return;
   }
-  // padded positions behind the last superchunk
-  const int64_t rest = from + (int64_t)supers * kTS;
+  // padded positions behind the last piece
+  const int64_t rest = from + (int64_t)pieces * kQ;
   if (rest < to) {
     for (int d = warp; d < chans; d += kWarps)
       for (int64_t t = rest + lane; t < to; t += 32) {
@@ -418,9 +409,9 @@ scan_bwd_kernel(Bwd a, Shape s) {
         stf(gdelta + d * s.L + t, 0.f);
       }
     for (int n = warp; n < s.N; n += kWarps)
-      for (int64_t t = rest + lane; t < to; t += 32) pb[n * s.L + t] = pc[n * s.L + t] = 0.f;
+      for (int64_t t = rest + lane; t < to; t += 32) gB[n * s.L + t] = gC[n * s.L + t] = 0.f;
   }
-  if (a.ginit && split == 0 && warp == 0) {
+  if (a.ginit && split == 0 && warp == (pieces ? (pieces - 1) % kWarps : 0)) {
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
@@ -434,9 +425,9 @@ scan_bwd_kernel(Bwd a, Shape s) {
   }
   // sums over the warps
   __syncthreads();
-  put(m.end + warp * kND * 32, dA);
-  m.prod[warp * 32 + lane] = quad(dskip[0], dskip[1]);
-  m.rend[warp * 32 + lane] = quad(dbias[0], dbias[1]);
+  put(all.pass + warp * kND * 32, dA);
+  all.total[warp * 32 + lane] = quad(dskip[0], dskip[1]);
+  all.total[(kWarps + warp) * 32 + lane] = quad(dbias[0], dbias[1]);
   __syncthreads();
   float *pa = a.part_a + (split * s.B + b) * s.D * s.N;
   for (int i = threadIdx.x; i < CT * NP; i += kThreads) {
@@ -446,17 +437,15 @@ scan_bwd_kernel(Bwd a, Shape s) {
     const int p = d % kND / 2, j = n % kNS, l = d / kND * LPC + n / kNS;
     float v = 0.f;
     for (int w = 0; w < kWarps; ++w)
-      v += reinterpret_cast<const float *>(m.end + (w * kND + 2 * p + j / 2) * 32 + l)[j % 2 * 2 + d % 2];
+      v += reinterpret_cast<const float *>(all.pass + (w * kND + 2 * p + j / 2) * 32 + l)[j % 2 * 2 + d % 2];
     pa[(d0 + d) * s.N + n] = v;
   }
-  using SumN = Scatter<1, LPC, 2 * kND, 2>;
-  constexpr int kLeftN = SumN::kLeft / 2, kOwners = kND / kLeftN, kEach = LPC / kOwners;
   for (int d = threadIdx.x; d < chans; d += kThreads) {
     const int l = d / kND * LPC + d % kND / kLeftN * kEach, j = d % kND % kLeftN;
     float v = 0.f, w = 0.f;
     for (int k = 0; k < kWarps; ++k) {
-      v += reinterpret_cast<const float *>(m.prod + k * 32 + l)[j];
-      w += reinterpret_cast<const float *>(m.rend + k * 32 + l)[j];
+      v += reinterpret_cast<const float *>(all.total + k * 32 + l)[j];
+      w += reinterpret_cast<const float *>(all.total + (kWarps + k) * 32 + l)[j];
     }
     a.part_d[(split * s.B + b) * s.D + d0 + d] = v;
     a.part_d[((a.splits + split) * s.B + b) * s.D + d0 + d] = w;
@@ -505,10 +494,10 @@ int64_t channel_tiles(int64_t D, int64_t N, int64_t G) {
 // as the forward's chunks, with one block to an SM
 int bwd_splits(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G, int64_t *chunk) {
   const int64_t blocks = B * G * channel_tiles(D, N, G), places = sm_count();
-  const int64_t supers = cdiv(L, kTS);
+  const int64_t most = cdiv(L, kWarps * kQ);
   int64_t n = blocks * 2 <= places ? places / blocks : 1;
-  if (n > supers) n = supers;
-  *chunk = cdiv(supers, n) * kTS;
+  if (n > most) n = most;
+  *chunk = cdiv(cdiv(L, n), kQ) * kQ;
   return (int)cdiv(L, *chunk);
 }
 
@@ -533,7 +522,7 @@ struct Outs {
 
 template <typename T, int LPC>
 int bwd_launch(const Bwd &a, const Outs &o, const Shape &s, cudaStream_t st) {
-  const int smem = (int)sizeof(BwdTile<T, LPC>);
+  const int smem = (int)sizeof(BwdSmem<LPC>);
   auto main = scan_bwd_kernel<T, LPC, false>, pre = scan_bwd_kernel<T, LPC, true>;
   const int64_t tiles = channel_tiles(s.D, s.N, s.G);
   const unsigned blocks = (unsigned)(s.B * s.G * tiles * a.splits);
@@ -591,7 +580,7 @@ int dudy_selective_scan_backward(const void *go, const float *grad_final, const 
   if (int rc = require_sm100()) return rc;
   const scan::Sizes z = scan::bwd_sizes(B, D, L, N, G);
   float *pb = (float *)workspace, *pa = pb + 2 * z.bc, *pd = pa + z.a, *rend = pd + z.d;
-  const int vec = L % 8 == 0 && aligned_to_16(u) && aligned_to_16(delta) && aligned_to_16(go) &&
+  const int vec = L % 4 == 0 && aligned_to_16(u) && aligned_to_16(delta) && aligned_to_16(go) &&
                   aligned_to_16(Bm) && aligned_to_16(Cm) && aligned_to_16(grad_u) &&
                   aligned_to_16(grad_delta);
   const scan::Bwd a{go, u, delta, Bm, Cm, grad_final, A, skip, delta_bias, checkpoints, lengths,

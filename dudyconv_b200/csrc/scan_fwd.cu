@@ -6,10 +6,9 @@ namespace scan {
 namespace {
 
 constexpr int kND = 2;                 // channels of a thread
-constexpr int kQ = 8;                  // positions of a warp in a superchunk
-constexpr int kTS = kWarps * kQ;       // positions of a superchunk
-constexpr int kYP = kTS + 4;
-static_assert(kTS % kCkpt == 0 && kCkpt % kQ == 0, "states are saved where a warp's piece starts");
+constexpr int kQ = 8;                  // positions of a piece
+constexpr int kYP = kQ + 4;
+static_assert(kQ % kCkpt == 0, "states are saved within a piece");
 
 struct Fwd {
   const void *u, *delta, *Bm, *Cm;
@@ -18,57 +17,43 @@ struct Fwd {
   void *y;
   float *final_state, *ckpt;
   float *end, *prod;   // [splits][B*D][N]: a chunk's end state from zero and its decays' product
-  int64_t chunk;       // positions of a chunk, a multiple of kTS
+  int64_t chunk;       // positions of a chunk, a multiple of kQ
   int splits, vec;
 };
 
-template <typename T, int LPC>
-struct FwdTile {
+// a warp's own piece
+template <int LPC>
+struct FwdPiece {
   static constexpr int CT = 32 / LPC * kND;     // channels of a block
   static constexpr int NP = kNS * LPC;          // padded states
-  static constexpr int UI = (CT * kTS / 4 + kThreads - 1) / kThreads;      // pieces of u a thread copies
-  static constexpr int BI = (2 * NP * kTS / 8 + kThreads - 1) / kThreads;  // pieces of B and C
-  float2 dt[kTS * CT], du[kTS * CT];            // dt and dt u, each twice side by side
-  float bc[kTS * 2 * NP];                       // B and C of a position side by side
-  float y[2][CT * kYP];
-  float4 end[kWarps * kND * 32], prod[kWarps * kND * 32];
-  float4 carry[2 * kND * 32];
+  static constexpr int UI = (CT * kQ / 4 + 31) / 32;      // fours of u and delta that a lane copies
+  static constexpr int BI = (2 * NP * kQ / 4 + 31) / 32;  // fours of B and C
+  float4 dtu[kQ * CT / 2];                      // (dt, dt', dt u, dt' u') of two channels
+  float bc[kQ * 2 * NP];                        // B and C of a position side by side
+  float y[CT * kYP];
 };
-
-// Four / eight neighbouring elements as they lie in memory; zero at and behind `end`.
-template <typename T, int N>
-struct Piece {
-  T e[N];
-  __device__ __forceinline__ void load(const T *row, int64_t t, int64_t end, bool vec) {
-    if (vec && t + N <= end) {
-      if constexpr (sizeof(e) == 8) {
-        *reinterpret_cast<uint2 *>(e) = *reinterpret_cast<const uint2 *>(row + t);
-      } else {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(e) / 16; ++i)
-          reinterpret_cast<uint4 *>(e)[i] = reinterpret_cast<const uint4 *>(row + t)[i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) e[i] = t + i < end ? row[t + i] : Elem<T>::from_f(0.f);
-    }
-  }
+template <int LPC>
+struct FwdSmem {
+  FwdPiece<LPC> piece[kWarps];
+  float4 pass[kWarps * kND * 32];               // the state that a warp hands on
+  float4 total[kWarps * kND * 32];              // and the chunk's decay product so far
 };
 
 // PRE: a chunk's end state from zero and its decay product only.
 template <typename T, int LPC, bool PRE>
 __global__ void __launch_bounds__(kThreads, 2)
 scan_fwd_kernel(Fwd a, Shape s) {
-  using Tile = FwdTile<T, LPC>;
-  constexpr int CT = Tile::CT, NP = Tile::NP;
+  using Mine = FwdPiece<LPC>;
+  constexpr int CT = Mine::CT, NP = Mine::NP;
   extern __shared__ __align__(16) char smem_raw[];
-  Tile &m = *reinterpret_cast<Tile *>(smem_raw);
+  FwdSmem<LPC> &all = *reinterpret_cast<FwdSmem<LPC> *>(smem_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ln = lane % LPC, ld = lane / LPC, n0 = ln * kNS, c0 = ld * kND;
+  Mine &m = all.piece[warp];
 
-  const int R = (int)(s.D / s.G), tiles = (R + CT - 1) / CT;
   const int split = blockIdx.x % a.splits;
   if (PRE && split == a.splits - 1) return;  // nothing starts from the last chunk's end
+  const int R = (int)(s.D / s.G), tiles = (R + CT - 1) / CT;
   const int64_t bid = blockIdx.x / a.splits;
   const int tile = (int)(bid % tiles);
   const int64_t bg = bid / tiles, b = bg / s.G, g = bg % s.G;
@@ -81,6 +66,7 @@ scan_fwd_kernel(Fwd a, Shape s) {
   const T *u = (const T *)a.u + row0 * s.L, *delta = (const T *)a.delta + row0 * s.L;
   const T *Bm = (const T *)a.Bm + bg * s.N * s.L, *Cm = (const T *)a.Cm + bg * s.N * s.L;
   T *y = (T *)a.y + row0 * s.L;
+  const int pieces = end > from ? (int)((end - from + kQ - 1) / kQ) : 0;
 
   float2 A[kND][2], h[kND][2], total[kND][2];
 #pragma unroll
@@ -92,7 +78,7 @@ scan_fwd_kernel(Fwd a, Shape s) {
       const int64_t at = (row0 + c0 + j) * s.N + n0 + i, step = s.B * s.D * s.N;
       av[i] = ok ? scaled<T>(a.A[(d0 + c0 + j) * s.N + n0 + i]) : 0.f;
       hv[i] = 0.f;
-      if (!PRE && ok) {
+      if (!PRE && ok && warp == 0) {
         if (a.init) hv[i] = a.init[at];
         for (int k = 0; k < split; ++k) hv[i] = fmaf(a.prod[k * step + at], hv[i], a.end[k * step + at]);
       }
@@ -102,191 +88,203 @@ scan_fwd_kernel(Fwd a, Shape s) {
     h[j][0] = make_float2(hv[0], hv[1]);
     h[j][1] = make_float2(hv[2], hv[3]);
     total[j][0] = total[j][1] = both(1.f);
-    if (warp == 0) m.carry[j * 32 + lane] = quad(h[j][0], h[j][1]);
   }
 
-  // the next superchunk's elements, in registers while this one is worked on
-  Piece<T, 4> pu[Tile::UI], pd[Tile::UI];
-  Piece<T, 8> pb[Tile::BI];
+  // a lane's channels where it copies them
+  float bias[Mine::UI], skip[Mine::UI];
+#pragma unroll
+  for (int k = 0; k < Mine::UI; ++k) {
+    const int d = (lane + k * 32) % CT;
+    bias[k] = d < chans && a.delta_bias ? a.delta_bias[d0 + d] : 0.f;
+    skip[k] = !PRE && d < chans && a.skip ? a.skip[d0 + d] : 0.f;
+  }
+  // the warp's next piece, in registers while this one is worked on
+  RowFour<T> pu[Mine::UI], pd[Mine::UI], pb[Mine::BI];
   auto fetch = [&](int64_t t0) {
 #pragma unroll
-    for (int k = 0; k < Tile::UI; ++k) {
-      const int i = threadIdx.x + k * kThreads, d = i % CT;
-      if (i >= CT * kTS / 4) break;
+    for (int k = 0; k < Mine::UI; ++k) {
+      const int i = lane + k * 32, d = i % CT;
+      if (i >= CT * kQ / 4) break;
       const int64_t lim = d < chans ? end : 0;
-      pu[k].load(u + d * s.L, t0 + i / CT * 4, lim, a.vec);
-      pd[k].load(delta + d * s.L, t0 + i / CT * 4, lim, a.vec);
+      row_load4(pu[k], u + d * s.L, t0 + i / CT * 4, lim, a.vec);
+      row_load4(pd[k], delta + d * s.L, t0 + i / CT * 4, lim, a.vec);
     }
 #pragma unroll
-    for (int k = 0; k < Tile::BI; ++k) {
-      const int i = threadIdx.x + k * kThreads, r = i % (2 * NP), n = r % NP;
-      if (i >= 2 * NP * kTS / 8) break;
-      pb[k].load((r < NP ? Bm : Cm) + n * s.L, t0 + i / (2 * NP) * 8, n < s.N ? end : 0, a.vec);
-    }
-  };
-  auto store_y = [&](int64_t t0, const float *ys) {
-    for (int i = threadIdx.x; i < chans * (kTS / 8); i += kThreads) {
-      const int d = i / (kTS / 8), c = i % (kTS / 8) * 8;
-      const int64_t t = t0 + c;
-      alignas(16) float o[8];
-      *reinterpret_cast<float4 *>(o) = *reinterpret_cast<const float4 *>(ys + d * kYP + c);
-      *reinterpret_cast<float4 *>(o + 4) = *reinterpret_cast<const float4 *>(ys + d * kYP + c + 4);
-      if (t + 8 > end)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = t + j < end ? o[j] : 0.f;
-      if (a.vec) row_store8_until<T, true>(y + d * s.L, t, to, o);
-      else row_store8_until<T, false>(y + d * s.L, t, to, o);
+    for (int k = 0; k < Mine::BI; ++k) {
+      const int i = lane + k * 32, r = i % (2 * NP), n = r % NP;
+      if (i >= 2 * NP * kQ / 4) break;
+      row_load4(pb[k], (r < NP ? Bm : Cm) + n * s.L, t0 + i / (2 * NP) * 4, n < s.N ? end : 0, a.vec);
     }
   };
-  const int supers = end > from ? (int)((end - from + kTS - 1) / kTS) : 0;
-  if (supers) fetch(from);
-  for (int k = 0; k < supers; ++k) {
-    const int64_t t0 = from + (int64_t)k * kTS;
-    __syncthreads();
-    // fp32 tiles, positions outermost, so that a thread reads its four states at once
+  if (warp < pieces) fetch(from + warp * kQ);
+  for (int k = warp; k < pieces; k += kWarps) {
+    const int64_t t0 = from + (int64_t)k * kQ;
+    __syncwarp();
+    // fp32, positions outermost, so that a thread reads its four states at once
+    float *dtu = reinterpret_cast<float *>(m.dtu);
 #pragma unroll
-    for (int p = 0; p < Tile::UI; ++p) {
-      const int i = threadIdx.x + p * kThreads, d = i % CT, c = i / CT * 4;
-      if (i >= CT * kTS / 4) break;
-      const bool ok = d < chans;
-      const float bias = ok && a.delta_bias ? a.delta_bias[d0 + d] : 0.f;
-      const float skip = !PRE && ok && a.skip ? a.skip[d0 + d] : 0.f;
+    for (int p = 0; p < Mine::UI; ++p) {
+      const int i = lane + p * 32, d = i % CT, c = i / CT * 4;
+      if (i >= CT * kQ / 4) break;
       alignas(16) float yv[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float uv = Elem<T>::to_f(pu[p].e[j]);
-        float dt = Elem<T>::to_f(pd[p].e[j]) + bias, slope;
+        const float uv = pu[p].get(j);
+        float dt = pd[p].get(j) + bias[p], slope;
         if (s.softplus) dt = softplus<T>(dt, slope);
         if (t0 + c + j >= end) dt = 0.f;  // the state passes a padded position unchanged
-        m.dt[(c + j) * CT + d] = both(dt);
-        m.du[(c + j) * CT + d] = both(dt * uv);
-        yv[j] = skip * uv;
+        float *to = dtu + ((c + j) * (CT / 2) + d / 2) * 4 + d % 2;
+        to[0] = dt;
+        to[2] = dt * uv;
+        yv[j] = skip[p] * uv;
       }
-      if (!PRE) *reinterpret_cast<float4 *>(m.y[k & 1] + d * kYP + c) = *reinterpret_cast<float4 *>(yv);
+      if (!PRE) *reinterpret_cast<float4 *>(m.y + d * kYP + c) = *reinterpret_cast<float4 *>(yv);
     }
 #pragma unroll
-    for (int p = 0; p < Tile::BI; ++p) {
-      const int i = threadIdx.x + p * kThreads, r = i % (2 * NP), c = i / (2 * NP) * 8;
-      if (i >= 2 * NP * kTS / 8) break;
+    for (int p = 0; p < Mine::BI; ++p) {
+      const int i = lane + p * 32, r = i % (2 * NP), c = i / (2 * NP) * 4;
+      if (i >= 2 * NP * kQ / 4) break;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m.bc[(c + j) * 2 * NP + r] = Elem<T>::to_f(pb[p].e[j]);
+      for (int j = 0; j < 4; ++j) m.bc[(c + j) * 2 * NP + r] = pb[p].get(j);
     }
-    __syncthreads();
-    if (k + 1 < supers) fetch(t0 + kTS);
-    if (!PRE && k > 0) store_y(t0 - kTS, m.y[(k - 1) & 1]);
+    __syncwarp();
+    if (k + kWarps < pieces) fetch(t0 + kWarps * kQ);
 
-    // this warp's piece from a zero state
-    const float2 *sdt = m.dt + warp * kQ * CT + c0, *sdu = m.du + warp * kQ * CT + c0;
-    const float *sbc = m.bc + warp * kQ * 2 * NP + n0;
-    float2 dec[kQ][kND][2];
-    float sum[kND];
-#pragma unroll
-    for (int j = 0; j < kND; ++j) sum[j] = 0.f, h[j][0] = h[j][1] = both(0.f);
+    const float4 *sdt = m.dtu + ld;
+    const float *sbc = m.bc + n0;
+    float2 dec[kQ][kND][2], own[kND][2], prod[kND][2];
 #pragma unroll
     for (int q = 0; q < kQ; ++q) {
-      const float4 dt = *reinterpret_cast<const float4 *>(sdt + q * CT);
-      const float4 du = *reinterpret_cast<const float4 *>(sdu + q * CT);
+      const float4 dt = sdt[q * (CT / 2)];
       const float4 bv = *reinterpret_cast<const float4 *>(sbc + q * 2 * NP);
 #pragma unroll
-      for (int j = 0; j < kND; ++j) {
-        const float2 dtj = j ? hi(dt) : lo(dt), duj = j ? hi(du) : lo(du);
-        sum[j] += dtj.x;
+      for (int j = 0; j < kND; ++j)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float2 x = __fmul2_rn(dtj, A[j][i]);
-          dec[q][j][i] = make_float2(decay<T>(x.x), decay<T>(x.y));
-          h[j][i] = __ffma2_rn(dec[q][j][i], h[j][i], __fmul2_rn(duj, i ? hi(bv) : lo(bv)));
+          const float2 x = __fmul2_rn(both(j ? dt.y : dt.x), A[j][i]);
+          const float2 e = make_float2(decay<T>(x.x), decay<T>(x.y));
+          const float2 in = __fmul2_rn(both(j ? dt.w : dt.z), i ? hi(bv) : lo(bv));
+          dec[q][j][i] = e;
+          own[j][i] = q ? __ffma2_rn(e, own[j][i], in) : in;
+          prod[j][i] = q ? __fmul2_rn(prod[j][i], e) : e;
         }
-      }
     }
-#pragma unroll
-    for (int j = 0; j < kND; ++j) {
-      const float2 x = __fmul2_rn(both(sum[j]), A[j][0]), z = __fmul2_rn(both(sum[j]), A[j][1]);
-      m.end[(warp * kND + j) * 32 + lane] = quad(h[j][0], h[j][1]);
-      m.prod[(warp * kND + j) * 32 + lane] =
-          make_float4(decay<T>(x.x), decay<T>(x.y), decay<T>(z.x), decay<T>(z.y));
-    }
-    __syncthreads();
-    // the state that enters it
-#pragma unroll
-    for (int j = 0; j < kND; ++j) {
-      const float4 c = m.carry[((k & 1) * kND + j) * 32 + lane];
-      h[j][0] = lo(c);
-      h[j][1] = hi(c);
-    }
-    const int before = PRE ? (warp == kWarps - 1 ? kWarps : 0) : warp;
-    for (int w = 0; w < before; ++w)
+    // the state that enters the piece, and the one that leaves it
+    if (k > 0) {
+      const int before = (warp + kWarps - 1) % kWarps;
+      pair_wait(1 + before);
 #pragma unroll
       for (int j = 0; j < kND; ++j) {
-        const float4 e = m.end[(w * kND + j) * 32 + lane], p = m.prod[(w * kND + j) * 32 + lane];
-        h[j][0] = __ffma2_rn(lo(p), h[j][0], lo(e));
-        h[j][1] = __ffma2_rn(hi(p), h[j][1], hi(e));
+        const float4 v = all.pass[(before * kND + j) * 32 + lane];
+        h[j][0] = lo(v);
+        h[j][1] = hi(v);
         if (PRE) {
-          total[j][0] = __fmul2_rn(total[j][0], lo(p));
-          total[j][1] = __fmul2_rn(total[j][1], hi(p));
-        }
-      }
-    if (!PRE) {
-      const int64_t tw = t0 + warp * kQ;
-      if (a.ckpt && warp * kQ % kCkpt == 0 && tw < s.L) {
-#pragma unroll
-        for (int j = 0; j < kND; ++j) {
-          float *ck = a.ckpt + ((b * s.ckpts() + tw / kCkpt) * s.D + d0 + c0 + j) * s.N + n0;
-          const float v[kNS] = {h[j][0].x, h[j][0].y, h[j][1].x, h[j][1].y};
-#pragma unroll
-          for (int i = 0; i < kNS; ++i)
-            if (c0 + j < chans && n0 + i < s.N) ck[i] = v[i];
-        }
-      }
-      // and the piece again from there: v[j][q] is this thread's part of y
-      float v[kND * kQ];
-#pragma unroll
-      for (int q = 0; q < kQ; ++q) {
-        const float4 du = *reinterpret_cast<const float4 *>(sdu + q * CT);
-        const float4 bv = *reinterpret_cast<const float4 *>(sbc + q * 2 * NP);
-        const float4 cv = *reinterpret_cast<const float4 *>(sbc + q * 2 * NP + NP);
-#pragma unroll
-        for (int j = 0; j < kND; ++j) {
-          const float2 duj = j ? hi(du) : lo(du);
-          h[j][0] = __ffma2_rn(dec[q][j][0], h[j][0], __fmul2_rn(duj, lo(bv)));
-          h[j][1] = __ffma2_rn(dec[q][j][1], h[j][1], __fmul2_rn(duj, hi(bv)));
-          const float2 p = __ffma2_rn(hi(cv), h[j][1], __fmul2_rn(lo(cv), h[j][0]));
-          v[j * kQ + q] = p.x + p.y;
-        }
-      }
-      using Sum = Scatter<1, LPC, kND * kQ>;
-      Sum::sum(v, lane);
-      constexpr int kLeft = Sum::kLeft, kV = kLeft % 4 == 0 ? 4 : kLeft;
-#pragma unroll
-      for (int i = 0; i < kLeft; i += kV) {
-        const int at = ln * kLeft + i;
-        float *to = m.y[k & 1] + (c0 + at / kQ) * kYP + warp * kQ + at % kQ;
-        if constexpr (kV == 4) {
-          float4 o = *reinterpret_cast<float4 *>(to);
-          o.x += v[i]; o.y += v[i + 1]; o.z += v[i + 2]; o.w += v[i + 3];
-          *reinterpret_cast<float4 *>(to) = o;
-        } else {
-#pragma unroll
-          for (int e = 0; e < kV; ++e) to[e] += v[i + e];
+          const float4 p = all.total[(before * kND + j) * 32 + lane];
+          total[j][0] = lo(p);
+          total[j][1] = hi(p);
         }
       }
     }
-    if (warp == kWarps - 1)
+#pragma unroll
+    for (int j = 0; j < kND; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        own[j][i] = __ffma2_rn(prod[j][i], h[j][i], own[j][i]);
+        if (PRE) total[j][i] = __fmul2_rn(total[j][i], prod[j][i]);
+      }
+    if (k + 1 < pieces) {
+#pragma unroll
+      for (int j = 0; j < kND; ++j) {
+        all.pass[(warp * kND + j) * 32 + lane] = quad(own[j][0], own[j][1]);
+        if (PRE) all.total[(warp * kND + j) * 32 + lane] = quad(total[j][0], total[j][1]);
+      }
+      pair_arrive(1 + warp);
+    }
+    if (PRE) {
+#pragma unroll
+      for (int j = 0; j < kND; ++j) h[j][0] = own[j][0], h[j][1] = own[j][1];
+      continue;
+    }
+    auto save = [&](int64_t t, const float2 (&v)[kND][2]) {
+      if (t >= end) return;
+#pragma unroll
+      for (int j = 0; j < kND; ++j) {
+        if (c0 + j >= chans) break;
+        float *ck = a.ckpt + ((b * s.ckpts() + t / kCkpt) * s.D + d0 + c0 + j) * s.N + n0;
+        if (s.N % kNS == 0 && n0 < s.N) {
+          *reinterpret_cast<float4 *>(ck) = quad(v[j][0], v[j][1]);
+        } else {
+          const float e[kNS] = {v[j][0].x, v[j][0].y, v[j][1].x, v[j][1].y};
+#pragma unroll
+          for (int i = 0; i < kNS; ++i)
+            if (n0 + i < s.N) ck[i] = e[i];
+        }
+      }
+    };
+    if (a.ckpt) save(t0, h);
+    // the recurrence from there; each state takes its decay's place
+#pragma unroll
+    for (int q = 0; q < kQ; ++q) {
+      const float4 du = sdt[q * (CT / 2)];
+      const float4 bv = *reinterpret_cast<const float4 *>(sbc + q * 2 * NP);
 #pragma unroll
       for (int j = 0; j < kND; ++j)
-        m.carry[(((k + 1) & 1) * kND + j) * 32 + lane] = quad(h[j][0], h[j][1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 in = __fmul2_rn(both(j ? du.w : du.z), i ? hi(bv) : lo(bv));
+          h[j][i] = __ffma2_rn(dec[q][j][i], h[j][i], in);
+          dec[q][j][i] = h[j][i];
+        }
+      if ((q + 1) % kCkpt == 0 && q + 1 < kQ && a.ckpt) save(t0 + q + 1, h);
+    }
+    // v[j][q] is this thread's part of y
+    float v[kND * kQ];
+#pragma unroll
+    for (int q = 0; q < kQ; ++q) {
+      const float4 cv = *reinterpret_cast<const float4 *>(sbc + q * 2 * NP + NP);
+#pragma unroll
+      for (int j = 0; j < kND; ++j) {
+        const float2 p = __ffma2_rn(hi(cv), dec[q][j][1], __fmul2_rn(lo(cv), dec[q][j][0]));
+        v[j * kQ + q] = p.x + p.y;
+      }
+    }
+    using Sum = Scatter<1, LPC, kND * kQ>;
+    Sum::sum(v, lane);
+    constexpr int kLeft = Sum::kLeft, kV = kLeft % 4 == 0 ? 4 : kLeft;
+#pragma unroll
+    for (int i = 0; i < kLeft; i += kV) {
+      const int at = ln * kLeft + i;
+      float *dst = m.y + (c0 + at / kQ) * kYP + at % kQ;
+      if constexpr (kV == 4) {
+        float4 o = *reinterpret_cast<float4 *>(dst);
+        o.x += v[i]; o.y += v[i + 1]; o.z += v[i + 2]; o.w += v[i + 3];
+        *reinterpret_cast<float4 *>(dst) = o;
+      } else {
+#pragma unroll
+        for (int e = 0; e < kV; ++e) dst[e] += v[i + e];
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int p = 0; p < Mine::UI; ++p) {
+      const int i = lane + p * 32, d = i % CT, c = i / CT * 4;
+      if (i >= CT * kQ / 4) break;
+      if (d >= chans) continue;
+      float o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = t0 + c + j < end ? m.y[d * kYP + c + j] : 0.f;
+      row_store4(y + d * s.L, t0 + c, to, o, a.vec);
+    }
   }
-  if (!PRE) {
-    __syncthreads();
-    if (supers) store_y(from + (int64_t)(supers - 1) * kTS, m.y[(supers - 1) & 1]);
-    // padded positions behind the last superchunk
-    const int64_t rest = from + (int64_t)supers * kTS;
+  if (!PRE) {  // padded positions behind the last piece
+    const int64_t rest = from + (int64_t)pieces * kQ;
     if (rest < to)
       for (int d = warp; d < chans; d += kWarps)
         for (int64_t t = rest + lane; t < to; t += 32) stf(y + d * s.L + t, 0.f);
   }
-  const bool last = split == a.splits - 1;
-  if (warp != kWarps - 1 || (!PRE && !(a.final_state && last))) return;
+  // the last piece's warp holds the end state
+  if (warp != (pieces ? (pieces - 1) % kWarps : 0)) return;
+  if (!PRE && !(a.final_state && split == a.splits - 1)) return;
 #pragma unroll
   for (int j = 0; j < kND; ++j) {
     const float v[kNS] = {h[j][0].x, h[j][0].y, h[j][1].x, h[j][1].y};
@@ -306,16 +304,16 @@ scan_fwd_kernel(Fwd a, Shape s) {
 }
 
 // Chunks of a sequence: as many as fill the GPU's places for blocks (two an SM), where the rows
-// of channels alone leave at least half of them empty; whole superchunks each.
+// of channels alone leave at least half of them empty; whole pieces each.
 int64_t fwd_blocks(const Shape &s) {
   return s.B * s.G * cdiv(s.R(), 32 / lanes_per_channel(s.N) * kND);
 }
 int fwd_splits(const Shape &s, int64_t *chunk) {
   const int64_t blocks = fwd_blocks(s), places = 2 * (int64_t)sm_count();
-  const int64_t supers = cdiv(s.L, kTS);
+  const int64_t most = cdiv(s.L, kWarps * kQ);  // a chunk has a piece for each of its warps
   int64_t n = blocks * 2 <= places ? places / blocks : 1;
-  if (n > supers) n = supers;
-  *chunk = cdiv(supers, n) * kTS;
+  if (n > most) n = most;
+  *chunk = cdiv(cdiv(s.L, n), kQ) * kQ;
   return (int)cdiv(s.L, *chunk);
 }
 size_t fwd_workspace(const Shape &s) {
@@ -326,7 +324,7 @@ size_t fwd_workspace(const Shape &s) {
 
 template <typename T, int LPC>
 int fwd_launch(const Fwd &a, const Shape &s, cudaStream_t st) {
-  const int smem = (int)sizeof(FwdTile<T, LPC>);
+  const int smem = (int)sizeof(FwdSmem<LPC>);
   auto main = scan_fwd_kernel<T, LPC, false>, pre = scan_fwd_kernel<T, LPC, true>;
   const unsigned grid = (unsigned)(fwd_blocks(s) * a.splits);
   if (a.splits > 1) {
@@ -413,7 +411,7 @@ int dudy_selective_scan_forward(const void *u, const void *delta, const float *A
                                  dudy_selective_scan_forward_workspace_size(B, D, L, N, G, dtype)))
     return rc;
   if (int rc = require_sm100()) return rc;
-  const int vec = L % 8 == 0 && aligned_to_16(u) && aligned_to_16(delta) && aligned_to_16(Bm) && aligned_to_16(Cm) &&
+  const int vec = L % 4 == 0 && aligned_to_16(u) && aligned_to_16(delta) && aligned_to_16(Bm) && aligned_to_16(Cm) &&
                   aligned_to_16(y);
   const scan::Shape s{B, D, L, (int)N, (int)G, softplus};
   int64_t chunk;

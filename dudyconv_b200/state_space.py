@@ -197,8 +197,8 @@ def fused_selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, 
 
     With ``return_final_state`` the result is ``(y, final_state)``, the state ``[B,D,N]`` (fp32)
     for the next chunk or for :func:`fused_selective_scan_step`. Differentiable in all tensors
-    but ``lengths``; a forward that will be differentiated keeps the states at every 32nd
-    position (``4 B D N L / 32`` bytes)."""
+    but ``lengths``; a forward that will be differentiated keeps the states at every fourth
+    position (``B D N L`` bytes)."""
     B, C = _grouped(B, 4), _grouped(C, 4)
     if _wants_grad(u, delta, A, B, C, skip, delta_bias, initial_state):
         return FusedSelectiveScanFunction.apply(u, delta, A, B, C, skip, delta_bias,

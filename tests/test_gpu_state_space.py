@@ -124,6 +124,9 @@ SCAN = [  # B, D, L, N, G, dtype, lengths, state, skip, delta_bias, softplus, of
     (1, 5, 296, 16, 1, "bf16", None, True, True, True, True, 1),
     (1, 130, 72, 2, 1, "fp16", None, True, True, True, True, 0),
     (1, 70, 96, 7, 2, "bf16", None, True, True, True, True, 0),
+    (2, 97, 75, 3, 1, "fp16", [75, 40], True, True, True, True, 0),
+    (1, 24, 1000, 16, 1, "bf16", None, True, True, True, True, 0),
+    (3, 24, 520, 24, 2, "fp32", [520, 33, 300], True, True, True, True, 0),
 ]
 
 

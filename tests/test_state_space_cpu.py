@@ -63,8 +63,8 @@ def test_workspace_is_checked_before_the_device():
     assert lib.dudy_short_conv_backward_workspace_size(0, 8, 10, 4, 1) == 0
     assert lib.dudy_selective_scan_backward_workspace_size(1, 8, 10, 65, 1, 1) == 0
     assert lib.dudy_block_norm_backward_workspace_size(1, 8, 10, 1, 2) == 0
-    # a saved state [B,D,N] for each 32 positions, fp32
-    assert lib.dudy_selective_scan_checkpoint_bytes(2, 8, 33, 16, 1, 1) == 2 * 8 * 2 * 16 * 4
+    # a saved state [B,D,N] for each four positions, fp32
+    assert lib.dudy_selective_scan_checkpoint_bytes(2, 8, 33, 16, 1, 1) == 2 * 8 * 9 * 16 * 4
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="checks the answer of a machine without a GPU")
