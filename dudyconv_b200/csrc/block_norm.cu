@@ -406,13 +406,6 @@ __device__ __forceinline__ void cp_async(void *smem, const void *gmem) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(gmem), "n"(BYTES)
                : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 // The tile's five tensors in shared memory, each thread's own four-token pieces side by side
 // (no thread reads another's, so its own copies' completion is all it waits for).
@@ -475,7 +468,7 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, int64_t ntiles, bool vec) {
           if (a.grout) row_load4(m.gr[i][tid], (const R *)a.grout + o, 0, left, false);
         }
       }
-    cp_async_commit();
+    copies_commit();
   };
   int at = 0;
   if (blockIdx.x < ntiles) fetch(blockIdx.x, stage[0]);
@@ -495,9 +488,9 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, int64_t ntiles, bool vec) {
     }
     if (Tile::kStages == 2 && tile + gridDim.x < ntiles) {
       fetch(tile + gridDim.x, stage[at ^ 1]);
-      cp_async_wait<1>();
+      copies_wait<1>();
     } else {
-      cp_async_wait<0>();
+      copies_wait<0>();
     }
     const Tile &m = stage[at];
     float hat1[ROWS][kV], hat2[ROWS][kV], sg[ROWS][kV], v[kV], u[kV];

@@ -120,7 +120,7 @@ int device_cc() {
   return g_cc[dev];
 }
 
-static int *device_err_word() {
+int *device_err_word() {
   const int dev = current_device();
   if (dev < 0 || dev >= kMaxDevices) return nullptr;
   init_device(dev);

@@ -160,6 +160,9 @@ __device__ __forceinline__ void pdl_trigger() {
 // and setting it costs host time on every launch of the small-chunk call path)
 cudaError_t set_smem_once(const void *kern, int bytes);
 
+// the current device's error record, which a wait that runs out writes to (capi.cu)
+int *device_err_word();
+
 // number of SMs of the current device (cached per device)
 int sm_count();
 // compute capability major*10+minor of the current device (cached per device)

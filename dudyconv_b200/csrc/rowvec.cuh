@@ -141,6 +141,25 @@ __device__ __forceinline__ void row_store4(T *row, int64_t t, int64_t end, const
   }
 }
 
+// row[t], row[t+1] = v, before `end`
+template <typename T>
+__device__ __forceinline__ void row_store2(T *row, int64_t t, int64_t end, const float (&v)[2],
+                                           bool vec) {
+  if (vec && t + 2 <= end) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float2 *>(row + t) = make_float2(v[0], v[1]);
+    } else {
+      const T e[2] = {Elem<T>::from_f(v[0]), Elem<T>::from_f(v[1])};
+      const uint16_t *h = reinterpret_cast<const uint16_t *>(e);
+      *reinterpret_cast<uint32_t *>(row + t) = (uint32_t)h[0] | (uint32_t)h[1] << 16;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (t + i < end) stf(row + t + i, v[i]);
+  }
+}
+
 // ---- activations --------------------------------------------------------------------------
 // 1 / (1 + exp(-v)); 16-bit tensors use the fast exponential and division (relative error
 // about 2^-21, far below the rounding of the result), fp32 tensors the accurate ones.
@@ -158,8 +177,10 @@ __device__ __forceinline__ void cp_async16(void *smem, const void *gmem) {
   const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(gmem) : "memory");
 }
-__device__ __forceinline__ void cp_async_wait_all() {
-  asm volatile("cp.async.wait_all;" ::: "memory");
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // ---- host side ------------------------------------------------------------------------------

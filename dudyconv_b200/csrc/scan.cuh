@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "rowvec.cuh"
+#include "sm100.cuh"
 
 namespace dudy {
 namespace scan {
@@ -74,6 +75,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 template <typename T>
 __device__ __forceinline__ float decay(float x) {
   return ex2(x);
@@ -90,14 +96,14 @@ __device__ __forceinline__ float decay<float>(float x) {
 template <typename T>
 __device__ __forceinline__ float softplus(float x, float &slope) {
   const float e = ex2(-1.4426950408889634f * fabsf(x));
-  const float s = __fdividef(e, 2.f + e), q = s * s;
+  const float s = e * rcp(2.f + e), q = s * s;
   float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
   p = fmaf(p, q, 1.f / 9.f);
   p = fmaf(p, q, 1.f / 7.f);
   p = fmaf(p, q, 1.f / 5.f);
   p = fmaf(p, q, 1.f / 3.f);
   p = fmaf(p, q, 1.f);
-  slope = __fdividef(x > 0.f ? 1.f : e, 1.f + e);
+  slope = (x > 0.f ? 1.f : e) * rcp(1.f + e);
   return fmaf(s + s, p, fmaxf(x, 0.f));
 }
 template <>
@@ -147,6 +153,60 @@ struct Scatter<STRIDE, 1, N, KEEP> {
   static constexpr int kLeft = N;
   static __device__ __forceinline__ void sum(float *, int) {}
 };
+
+// Input rows come in by stretches of one piece for each warp, copied by all the block's threads
+// into one of three buffers (rows of whole 16-byte pieces: a warp's own piece of a row is 8 to
+// 16 bytes, and copying it alone cost the load pipe eight times as many accesses). A warp that
+// begins a piece of stretch s issues its part of stretch s + 2, waits for its part of s + 1
+// (issued a stretch ago), takes what it needs of s into its own shared memory, and arrives for
+// s + 1: when all have arrived, s + 1 has landed and buffer (s + 3) % 3 is free.
+constexpr int kStages = 3;
+constexpr int kHeld = 2;        // 16-byte copies of a stretch whose places a thread keeps at hand
+constexpr int kSiteStage = 970;  // wait site of a stretch that never came
+
+// One thread's 16 bytes of a stretch: the same row and place in it for every stretch.
+template <typename T>
+struct RowCopy {
+  const T *src;  // null: nothing to copy (a padding row, zeroed once)
+  int dst, c;
+};
+template <typename T>
+__device__ __forceinline__ void row_copy(T *raw, const RowCopy<T> &x, int64_t t0, int64_t end,
+                                         bool vec) {
+  constexpr int V = 16 / sizeof(T);
+  if (!x.src) return;
+  T *to = raw + x.dst;
+  if (vec && t0 + x.c + V <= end) {
+    cp_async16(to, x.src + t0);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      to[k] = t0 + x.c + k < end ? x.src[t0 + k] : Elem<T>::from_f(0.f);
+  }
+}
+
+struct Ready {  // one barrier a buffer, an arrival a warp
+  uint64_t bar[kStages];
+  int abort;
+};
+__device__ __forceinline__ void ready_init(Ready &r) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) sm100::mbar_init(&r.bar[i], kWarps);
+    r.abort = 0;
+    sm100::fence_barrier_init();
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ void ready_arrive(Ready &r, int stretch) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) sm100::mbar_arrive(&r.bar[stretch % kStages]);
+}
+// A stretch that does not come within the library's limit is recorded; the block goes on, so
+// that every warp still meets its neighbours.
+__device__ __forceinline__ void ready_wait(Ready &r, int stretch, int *err) {
+  sm100::mbar_wait(&r.bar[stretch % kStages], (stretch / kStages) & 1, err, &r.abort, kSiteStage,
+                   stretch);
+}
 
 // Two warps meet: one arrives and goes on, the other waits for it.
 __device__ __forceinline__ void pair_wait(int id) {

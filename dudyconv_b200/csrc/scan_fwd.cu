@@ -7,6 +7,7 @@ namespace {
 
 constexpr int kND = 2;                 // channels of a thread
 constexpr int kQ = 8;                  // positions of a piece
+constexpr int kTS = kWarps * kQ;       // positions of a stretch
 constexpr int kYP = kQ + 4;
 static_assert(kQ % kCkpt == 0, "states are saved within a piece");
 
@@ -19,6 +20,7 @@ struct Fwd {
   float *end, *prod;   // [splits][B*D][N]: a chunk's end state from zero and its decays' product
   int64_t chunk;       // positions of a chunk, a multiple of kQ
   int splits, vec;
+  int *err;
 };
 
 // a warp's own piece
@@ -26,17 +28,24 @@ template <int LPC>
 struct FwdPiece {
   static constexpr int CT = 32 / LPC * kND;     // channels of a block
   static constexpr int NP = kNS * LPC;          // padded states
-  static constexpr int UI = (CT * kQ / 4 + 31) / 32;      // fours of u and delta that a lane copies
+  static constexpr int UI = (CT * kQ / 4 + 31) / 32;      // fours of u and delta that a lane takes
   static constexpr int BI = (2 * NP * kQ / 4 + 31) / 32;  // fours of B and C
   float4 dtu[kQ * CT / 2];                      // (dt, dt', dt u, dt' u') of two channels
   float bc[kQ * 2 * NP];                        // B and C of a position side by side
   float y[CT * kYP];
 };
-template <int LPC>
+template <typename T, int LPC>
 struct FwdSmem {
+  static constexpr int CT = FwdPiece<LPC>::CT, NP = FwdPiece<LPC>::NP;
+  static constexpr int PITCH = kTS + 16 / (int)sizeof(T);
+  static constexpr int V = 16 / (int)sizeof(T), VPR = kTS / V;
+  static constexpr int ROWS = 2 * CT + 2 * NP;  // u, delta, B, C as they lie in memory
+  static constexpr int ITEMS = ROWS * VPR, EACH = (ITEMS + kThreads - 1) / kThreads;
+  T raw[kStages][ROWS * PITCH];
   FwdPiece<LPC> piece[kWarps];
   float4 pass[kWarps * kND * 32];               // the state that a warp hands on
   float4 total[kWarps * kND * 32];              // and the chunk's decay product so far
+  Ready ready;
 };
 
 // PRE: a chunk's end state from zero and its decay product only.
@@ -46,7 +55,8 @@ scan_fwd_kernel(Fwd a, Shape s) {
   using Mine = FwdPiece<LPC>;
   constexpr int CT = Mine::CT, NP = Mine::NP;
   extern __shared__ __align__(16) char smem_raw[];
-  FwdSmem<LPC> &all = *reinterpret_cast<FwdSmem<LPC> *>(smem_raw);
+  using Smem = FwdSmem<T, LPC>;
+  Smem &all = *reinterpret_cast<Smem *>(smem_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ln = lane % LPC, ld = lane / LPC, n0 = ln * kNS, c0 = ld * kND;
   Mine &m = all.piece[warp];
@@ -90,7 +100,7 @@ scan_fwd_kernel(Fwd a, Shape s) {
     total[j][0] = total[j][1] = both(1.f);
   }
 
-  // a lane's channels where it copies them
+  // a lane's channels where it takes u and delta
   float bias[Mine::UI], skip[Mine::UI];
 #pragma unroll
   for (int k = 0; k < Mine::UI; ++k) {
@@ -98,44 +108,67 @@ scan_fwd_kernel(Fwd a, Shape s) {
     bias[k] = d < chans && a.delta_bias ? a.delta_bias[d0 + d] : 0.f;
     skip[k] = !PRE && d < chans && a.skip ? a.skip[d0 + d] : 0.f;
   }
-  // the warp's next piece, in registers while this one is worked on
-  RowFour<T> pu[Mine::UI], pd[Mine::UI], pb[Mine::BI];
-  auto fetch = [&](int64_t t0) {
-#pragma unroll
-    for (int k = 0; k < Mine::UI; ++k) {
-      const int i = lane + k * 32, d = i % CT;
-      if (i >= CT * kQ / 4) break;
-      const int64_t lim = d < chans ? end : 0;
-      row_load4(pu[k], u + d * s.L, t0 + i / CT * 4, lim, a.vec);
-      row_load4(pd[k], delta + d * s.L, t0 + i / CT * 4, lim, a.vec);
-    }
-#pragma unroll
-    for (int k = 0; k < Mine::BI; ++k) {
-      const int i = lane + k * 32, r = i % (2 * NP), n = r % NP;
-      if (i >= 2 * NP * kQ / 4) break;
-      row_load4(pb[k], (r < NP ? Bm : Cm) + n * s.L, t0 + i / (2 * NP) * 4, n < s.N ? end : 0, a.vec);
-    }
+  const int stretches = (pieces + kWarps - 1) / kWarps;
+  auto item = [&](int i) {
+    const int row = i / Smem::VPR, c = i % Smem::VPR * Smem::V;
+    const bool chan = row < 2 * CT;
+    const int r = chan ? row % CT : (row - 2 * CT) % NP;
+    const T *base = row < CT ? u : chan ? delta : row < 2 * CT + NP ? Bm : Cm;
+    const bool ok = i < Smem::ITEMS && r < (chan ? chans : s.N);
+    return RowCopy<T>{ok ? base + r * s.L + c : nullptr, row * Smem::PITCH + c, c};
   };
-  if (warp < pieces) fetch(from + warp * kQ);
-  for (int k = warp; k < pieces; k += kWarps) {
+  constexpr int kKeep = Smem::EACH < kHeld ? Smem::EACH : kHeld;
+  RowCopy<T> held[kKeep];
+#pragma unroll
+  for (int k = 0; k < kKeep; ++k) held[k] = item(threadIdx.x + k * kThreads);
+  auto stage = [&](int st) {
+    if (st < stretches) {
+      const int64_t t0 = from + (int64_t)st * kTS;
+      T *raw = all.raw[st % kStages];
+#pragma unroll
+      for (int k = 0; k < Smem::EACH; ++k)
+        row_copy(raw, k < kKeep ? held[k < kKeep ? k : 0] : item(threadIdx.x + k * kThreads), t0,
+                 end, a.vec);
+    }
+    copies_commit();
+  };
+  for (int i = threadIdx.x; i < Smem::ITEMS; i += kThreads) {
+    const RowCopy<T> x = item(i);
+    if (!x.src)
+      for (int st = 0; st < kStages; ++st)
+        *reinterpret_cast<uint4 *>(all.raw[st] + x.dst) = make_uint4(0, 0, 0, 0);
+  }
+  ready_init(all.ready);
+  stage(0);
+  stage(1);
+  copies_wait<1>();
+  ready_arrive(all.ready, 0);
+  for (int st = 0; st < stretches; ++st) {
+    const int k = st * kWarps + warp, buf = st % kStages, at = warp * kQ;
     const int64_t t0 = from + (int64_t)k * kQ;
+    ready_wait(all.ready, st, a.err);
     __syncwarp();
+    stage(st + 2);
+    copies_wait<1>();
     // fp32, positions outermost, so that a thread reads its four states at once
     float *dtu = reinterpret_cast<float *>(m.dtu);
 #pragma unroll
     for (int p = 0; p < Mine::UI; ++p) {
       const int i = lane + p * 32, d = i % CT, c = i / CT * 4;
       if (i >= CT * kQ / 4) break;
+      RowFour<T> pu, pd;
+      pu.load_all(all.raw[buf] + d * Smem::PITCH + at + c);
+      pd.load_all(all.raw[buf] + (CT + d) * Smem::PITCH + at + c);
       alignas(16) float yv[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float uv = pu[p].get(j);
-        float dt = pd[p].get(j) + bias[p], slope;
+        const float uv = pu.get(j);
+        float dt = pd.get(j) + bias[p], slope;
         if (s.softplus) dt = softplus<T>(dt, slope);
         if (t0 + c + j >= end) dt = 0.f;  // the state passes a padded position unchanged
-        float *to = dtu + ((c + j) * (CT / 2) + d / 2) * 4 + d % 2;
-        to[0] = dt;
-        to[2] = dt * uv;
+        float *dst = dtu + ((c + j) * (CT / 2) + d / 2) * 4 + d % 2;
+        dst[0] = dt;
+        dst[2] = dt * uv;
         yv[j] = skip[p] * uv;
       }
       if (!PRE) *reinterpret_cast<float4 *>(m.y + d * kYP + c) = *reinterpret_cast<float4 *>(yv);
@@ -144,11 +177,13 @@ scan_fwd_kernel(Fwd a, Shape s) {
     for (int p = 0; p < Mine::BI; ++p) {
       const int i = lane + p * 32, r = i % (2 * NP), c = i / (2 * NP) * 4;
       if (i >= 2 * NP * kQ / 4) break;
+      RowFour<T> pb;
+      pb.load_all(all.raw[buf] + (2 * CT + r) * Smem::PITCH + at + c);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) m.bc[(c + j) * 2 * NP + r] = pb[p].get(j);
+      for (int j = 0; j < 4; ++j) m.bc[(c + j) * 2 * NP + r] = pb.get(j);
     }
-    __syncwarp();
-    if (k + kWarps < pieces) fetch(t0 + kWarps * kQ);
+    ready_arrive(all.ready, st + 1);
+    if (k >= pieces) break;
 
     const float4 *sdt = m.dtu + ld;
     const float *sbc = m.bc + n0;
@@ -324,7 +359,7 @@ size_t fwd_workspace(const Shape &s) {
 
 template <typename T, int LPC>
 int fwd_launch(const Fwd &a, const Shape &s, cudaStream_t st) {
-  const int smem = (int)sizeof(FwdSmem<LPC>);
+  const int smem = (int)sizeof(FwdSmem<T, LPC>);
   auto main = scan_fwd_kernel<T, LPC, false>, pre = scan_fwd_kernel<T, LPC, true>;
   const unsigned grid = (unsigned)(fwd_blocks(s) * a.splits);
   if (a.splits > 1) {
@@ -411,7 +446,7 @@ int dudy_selective_scan_forward(const void *u, const void *delta, const float *A
                                  dudy_selective_scan_forward_workspace_size(B, D, L, N, G, dtype)))
     return rc;
   if (int rc = require_sm100()) return rc;
-  const int vec = L % 4 == 0 && aligned_to_16(u) && aligned_to_16(delta) && aligned_to_16(Bm) && aligned_to_16(Cm) &&
+  const int vec = L % 8 == 0 && aligned_to_16(u) && aligned_to_16(delta) && aligned_to_16(Bm) && aligned_to_16(Cm) &&
                   aligned_to_16(y);
   const scan::Shape s{B, D, L, (int)N, (int)G, softplus};
   int64_t chunk;
@@ -419,7 +454,7 @@ int dudy_selective_scan_forward(const void *u, const void *delta, const float *A
   float *ws = (float *)workspace;
   const scan::Fwd a{u, delta, Bm, Cm, A, skip, delta_bias, state, lengths, y, final_state,
                     checkpoints, ws, splits > 1 ? ws + splits * B * D * N : nullptr, chunk, splits,
-                    vec};
+                    vec, device_err_word()};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return scan::by_type_and_lanes(dtype, N, [&](auto t, auto lanes) {
     return scan::fwd_launch<decltype(t), decltype(lanes)::value>(a, s, st);
