@@ -236,18 +236,16 @@ block_norm_bwd_any_kernel(NormBwd a, NormShape s) {
 // ---- D <= 1024: the tile in registers ------------------------------------------------------
 // 512 threads hold a tile of 4 TX tokens x all channels, four tokens and up to four channels to
 // a thread, so each tensor moves once. TX = 8 (rows of 64 bytes in 16-bit types) up to D = 256,
-// then 4 and 2.
+// then 4 and 2. Persistent blocks: a block's next tile is copied into shared memory while it
+// works on this one, each thread's own four-token pieces side by side (no thread reads another's,
+// so its own copies' completion is all it waits for). Arithmetic goes two tokens at a time
+// (__ffma2_rn): with one, the backward issued 91 instructions an element.
 constexpr int kTileThreads = 512;
 constexpr int kV = 4;  // tokens of a thread
 
 template <typename T>
 using Four = RowFour<T>;
-
-template <typename T>
-__device__ __forceinline__ void get4(const Four<T> &f, float (&v)[kV]) {
-#pragma unroll
-  for (int i = 0; i < kV; ++i) v[i] = f.get(i);
-}
+using Two = float2[kV / 2];
 
 struct TileRed {
   float part[2][kTileThreads / 32][32];
@@ -258,9 +256,10 @@ struct TileRed {
 // tokens: across the rows of a warp by shuffles, across the warps by sixteen lanes a token.
 // `turn` alternates between two sets of buffers, so two barriers are enough.
 template <int TX>
-__device__ __forceinline__ void tile_sum4(float (&v)[kV], TileRed &m, int &turn) {
+__device__ __forceinline__ void tile_sum4(Two &p, TileRed &m, int &turn) {
   constexpr int kW = kTileThreads / 32, TOK = TX * kV;
   const int tid = threadIdx.x, tx = tid % TX;
+  float v[kV] = {p[0].x, p[0].y, p[1].x, p[1].y};
 #pragma unroll
   for (int o = 16; o >= TX; o >>= 1)
 #pragma unroll
@@ -277,127 +276,31 @@ __device__ __forceinline__ void tile_sum4(float (&v)[kV], TileRed &m, int &turn)
   }
   __syncthreads();
   const float4 t = *reinterpret_cast<const float4 *>(&m.total[turn][tx * kV]);
-  v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+  p[0] = make_float2(t.x, t.y);
+  p[1] = make_float2(t.z, t.w);
   turn ^= 1;
 }
 
-template <typename T, typename R, int TX, int ROWS, bool LAYER>
-__global__ void __launch_bounds__(kTileThreads, ROWS <= 4 && sizeof(T) == 2 ? 2 : 1)
-block_norm_fwd_tile_kernel(NormFwd a, NormShape s, bool vec) {
-  constexpr int TY = kTileThreads / TX;
-  __shared__ __align__(16) TileRed red;
-  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
-  const int64_t tiles = (s.L + TX * kV - 1) / (TX * kV);
-  const int64_t b = blockIdx.x / tiles, t = blockIdx.x % tiles * (TX * kV) + tx * kV;
-  const int64_t left = s.L - t, base = b * s.D * s.L + t;
-  const bool in = left > 0;
-  const float rd = 1.f / (float)s.D;
-  int turn = 0;
-  const T *xp = (const T *)a.x + base, *zp = a.gate ? (const T *)a.gate + base : nullptr;
-  const R *rp = (const R *)a.residual + base;
-  Four<T> xr[ROWS], zr[ROWS];
-  Four<R> rr[ROWS];
-#pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int64_t d = ty + i * TY;
-    if (in && d < s.D) {
-      row_load4(xr[i], xp + d * s.L, 0, left, vec);
-      if (zp) row_load4(zr[i], zp + d * s.L, 0, left, vec);
-      row_load4(rr[i], rp + d * s.L, 0, left, vec);
-    }
-  }
-  float g[ROWS][kV], m1[kV], m2[kV], q[kV];
-#pragma unroll
-  for (int k = 0; k < kV; ++k) m1[k] = m2[k] = 0.f;
-#pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const bool ok = in && ty + i * TY < s.D;
-    if (ok) {
-      get4(xr[i], g[i]);
-      if (zp) {
-        float z[kV];
-        get4(zr[i], z);
-#pragma unroll
-        for (int k = 0; k < kV; ++k) g[i][k] *= z[k] * sigmoid_for<T>(z[k]);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < kV; ++k) {
-      if (!ok) g[i][k] = 0.f;
-      m1[k] += g[i][k];
-    }
-  }
-  if (LAYER) {
-    tile_sum4<TX>(m1, red, turn);
-#pragma unroll
-    for (int k = 0; k < kV; ++k) m1[k] *= rd;
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 neg2(float2 a) { return make_float2(-a.x, -a.y); }
+
+template <typename T>
+__device__ __forceinline__ float2 sigmoid2(float2 v) {
+  if constexpr (sizeof(T) == 4) {
+    return make_float2(sigmoid_for<T>(v.x), sigmoid_for<T>(v.y));
   } else {
-#pragma unroll
-    for (int k = 0; k < kV; ++k) m1[k] = 0.f;
+    const float2 e = mul2(v, both(-1.4426950408889634f));
+    const float2 d = add2(make_float2(ex2(e.x), ex2(e.y)), both(1.f));
+    return make_float2(rcp(d.x), rcp(d.y));
   }
-  auto squares = [&](const float (&m)[kV]) {
-#pragma unroll
-    for (int k = 0; k < kV; ++k) q[k] = 0.f;
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i)
-      if (!LAYER || ty + i * TY < s.D)
-#pragma unroll
-        for (int k = 0; k < kV; ++k) q[k] = fmaf(g[i][k] - m[k], g[i][k] - m[k], q[k]);
-    tile_sum4<TX>(q, red, turn);
-#pragma unroll
-    for (int k = 0; k < kV; ++k) q[k] = rsqrtf(fmaf(q[k], rd, s.eps));
-  };
-  squares(m1);
-  float inv1[kV];
-#pragma unroll
-  for (int k = 0; k < kV; ++k) inv1[k] = q[k];
-  // the residual stream takes g's place
-#pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int64_t d = ty + i * TY;
-    if (in && d < s.D) {
-      const float w = ldf((const T *)a.w1 + d), o = LAYER ? opt((const T *)a.b1, d, 0.f) : 0.f;
-      const float c = opt((const T *)a.scale, d, 1.f);
-      float r[kV];
-      get4(rr[i], r);
-#pragma unroll
-      for (int k = 0; k < kV; ++k)
-        g[i][k] = fmaf(c, fmaf((g[i][k] - m1[k]) * inv1[k], w, o), r[k]);
-      row_store4((R *)a.rout + base + d * s.L, 0, left, g[i], vec);
-    }
-#pragma unroll
-    for (int k = 0; k < kV; ++k) m2[k] += g[i][k];
-  }
-  if (LAYER) {
-    tile_sum4<TX>(m2, red, turn);
-#pragma unroll
-    for (int k = 0; k < kV; ++k) m2[k] *= rd;
-  } else {
-#pragma unroll
-    for (int k = 0; k < kV; ++k) m2[k] = 0.f;
-  }
-  squares(m2);
-#pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int64_t d = ty + i * TY;
-    if (!in || d >= s.D) continue;
-    const float w = ldf((const T *)a.w2 + d), o = LAYER ? opt((const T *)a.b2, d, 0.f) : 0.f;
-    float y[kV];
-#pragma unroll
-    for (int k = 0; k < kV; ++k) y[k] = fmaf((g[i][k] - m2[k]) * q[k], w, o);
-    row_store4((T *)a.y + base + d * s.L, 0, left, y, vec);
-  }
-  if (a.stats && ty == 0) {
-    const int64_t n = s.B * s.L, at = b * s.L + t;
-#pragma unroll
-    for (int k = 0; k < kV; ++k)
-      if (k < left) {
-        a.stats[at + k] = m1[k];
-        a.stats[n + at + k] = inv1[k];
-        a.stats[2 * n + at + k] = m2[k];
-        a.stats[3 * n + at + k] = q[k];
-      }
-  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_pairs(T *row, int64_t left, const Two &p, bool vec) {
+  const float v[kV] = {p[0].x, p[0].y, p[1].x, p[1].y};
+  row_store4(row, 0, left, v, vec);
 }
 
 template <int BYTES>
@@ -406,11 +309,172 @@ __device__ __forceinline__ void cp_async(void *smem, const void *gmem) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(gmem), "n"(BYTES)
                : "memory");
 }
+template <typename T>
+__device__ __forceinline__ void fetch4(Four<T> &to, const T *from, int64_t left, bool vec) {
+  if (vec) cp_async<sizeof(Four<T>)>(&to, from);
+  else row_load4(to, from, 0, left, false);
+}
 
-// The tile's five tensors in shared memory, each thread's own four-token pieces side by side
-// (no thread reads another's, so its own copies' completion is all it waits for).
+// where a thread's tokens of a tile are
+struct Place {
+  int64_t b, t, left, base;
+};
+template <int TX>
+__device__ __forceinline__ Place place(unsigned tile, unsigned tiles, const NormShape &s) {
+  Place p;
+  p.b = tile / tiles;
+  p.t = (int64_t)(tile % tiles) * (TX * kV) + threadIdx.x % TX * kV;
+  p.left = s.L - p.t;
+  p.base = p.b * s.D * s.L + p.t;
+  return p;
+}
+
 template <typename T, typename R, int ROWS>
-struct NormTile {
+struct FwdTile {
+  Four<T> x[ROWS][kTileThreads], z[ROWS][kTileThreads];
+  Four<R> r[ROWS][kTileThreads];
+  static constexpr int kBytes = ROWS * kTileThreads * (2 * sizeof(Four<T>) + sizeof(Four<R>));
+  // two blocks an SM (64 registers) where two tiles of each fit, else one
+  static constexpr int kBlocks = 2 * kBytes <= 104 * 1024 ? 2 : 1;
+};
+
+template <typename T, typename R, int TX, int ROWS, bool LAYER>
+__global__ void __launch_bounds__(kTileThreads, (FwdTile<T, R, ROWS>::kBlocks))
+block_norm_fwd_tile_kernel(NormFwd a, NormShape s, unsigned ntiles, bool vec) {
+  using Tile = FwdTile<T, R, ROWS>;
+  constexpr int TY = kTileThreads / TX;
+  extern __shared__ __align__(16) char smem_raw[];
+  Tile *stage = reinterpret_cast<Tile *>(smem_raw);
+  __shared__ __align__(16) TileRed red;
+  const int tid = threadIdx.x, ty = tid / TX;
+  const unsigned tiles = (unsigned)((s.L + TX * kV - 1) / (TX * kV));
+  const float rd = 1.f / (float)s.D;
+  const int D = (int)s.D;
+  int turn = 0, at = 0;
+
+  // residual + c1 hat1 + c0, y = c2 hat2 + c3
+  float c1[ROWS], c0[ROWS], c2[ROWS], c3[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int d = ty + i * TY;
+    const bool ok = d < D;
+    const float sc = ok ? opt((const T *)a.scale, d, 1.f) : 0.f;
+    c1[i] = ok ? sc * ldf((const T *)a.w1 + d) : 0.f;
+    c0[i] = LAYER && ok ? sc * opt((const T *)a.b1, d, 0.f) : 0.f;
+    c2[i] = ok ? ldf((const T *)a.w2 + d) : 0.f;
+    c3[i] = LAYER && ok ? opt((const T *)a.b2, d, 0.f) : 0.f;
+  }
+  auto fetch = [&](unsigned tile, Tile &m) {
+    const Place p = place<TX>(tile, tiles, s);
+    if (p.left > 0)
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const int d = ty + i * TY;
+        if (d >= D) continue;
+        const int64_t o = p.base + d * s.L;
+        fetch4(m.x[i][tid], (const T *)a.x + o, p.left, vec);
+        if (a.gate) fetch4(m.z[i][tid], (const T *)a.gate + o, p.left, vec);
+        fetch4(m.r[i][tid], (const R *)a.residual + o, p.left, vec);
+      }
+    copies_commit();
+  };
+  if (blockIdx.x < ntiles) fetch(blockIdx.x, stage[0]);
+  for (unsigned tile = blockIdx.x; tile < ntiles; tile += gridDim.x, at ^= 1) {
+    const Place p = place<TX>(tile, tiles, s);
+    if (tile + gridDim.x < ntiles) {
+      fetch(tile + gridDim.x, stage[at ^ 1]);
+      copies_wait<1>();
+    } else {
+      copies_wait<0>();
+    }
+    const Tile &m = stage[at];
+    float2 g[ROWS][kV / 2];
+    Two m1, m2, inv1, q;
+#pragma unroll
+    for (int k = 0; k < kV / 2; ++k) m1[k] = m2[k] = q[k] = both(0.f);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const bool ok = p.left > 0 && ty + i * TY < D;
+#pragma unroll
+      for (int k = 0; k < kV / 2; ++k) {
+        float2 v = m.x[i][tid].pair(k);
+        if (a.gate) {
+          const float2 z = m.z[i][tid].pair(k);
+          v = mul2(v, mul2(z, sigmoid2<T>(z)));
+        }
+        if (!ok) v = both(0.f);
+        g[i][k] = v;
+        if (LAYER) m1[k] = add2(m1[k], v);
+        else q[k] = fma2(v, v, q[k]);
+      }
+    }
+    // mean and 1 / sqrt(var + eps) of g; q holds the sum of squares of an rms norm
+    auto statistics = [&](Two &mean, Two &inv) {
+      if (LAYER) {
+        tile_sum4<TX>(mean, red, turn);
+#pragma unroll
+        for (int k = 0; k < kV / 2; ++k) mean[k] = mul2(mean[k], both(rd)), q[k] = both(0.f);
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+          if (ty + i * TY < D)
+#pragma unroll
+            for (int k = 0; k < kV / 2; ++k) {
+              const float2 c = add2(g[i][k], neg2(mean[k]));
+              q[k] = fma2(c, c, q[k]);
+            }
+      }
+      tile_sum4<TX>(q, red, turn);
+#pragma unroll
+      for (int k = 0; k < kV / 2; ++k) {
+        inv[k] = make_float2(rsqrtf(fmaf(q[k].x, rd, s.eps)), rsqrtf(fmaf(q[k].y, rd, s.eps)));
+        q[k] = both(0.f);
+      }
+    };
+    statistics(m1, inv1);
+    // the residual stream takes g's place
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int d = ty + i * TY;
+      const bool ok = p.left > 0 && d < D;
+#pragma unroll
+      for (int k = 0; k < kV / 2; ++k) {
+        const float2 hat = mul2(LAYER ? add2(g[i][k], neg2(m1[k])) : g[i][k], inv1[k]);
+        float2 v = m.r[i][tid].pair(k);
+        if (LAYER) v = add2(v, both(c0[i]));
+        v = fma2(hat, both(c1[i]), v);
+        if (!ok) v = both(0.f);
+        g[i][k] = v;
+        if (LAYER) m2[k] = add2(m2[k], v);
+        else q[k] = fma2(v, v, q[k]);
+      }
+      if (ok) store_pairs((R *)a.rout + p.base + d * s.L, p.left, g[i], vec);
+    }
+    Two inv2;
+    statistics(m2, inv2);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int d = ty + i * TY;
+      if (p.left <= 0 || d >= D) continue;
+      Two y;
+#pragma unroll
+      for (int k = 0; k < kV / 2; ++k) {
+        const float2 hat = mul2(LAYER ? add2(g[i][k], neg2(m2[k])) : g[i][k], inv2[k]);
+        y[k] = LAYER ? fma2(hat, both(c2[i]), both(c3[i])) : mul2(hat, both(c2[i]));
+      }
+      store_pairs((T *)a.y + p.base + d * s.L, p.left, y, vec);
+    }
+    if (a.stats && ty == 0 && p.left > 0) {
+      const int64_t n = s.B * s.L;
+      float *st = a.stats + p.b * s.L + p.t;
+      if (LAYER) store_pairs(st, p.left, m1, vec), store_pairs(st + 2 * n, p.left, m2, vec);
+      store_pairs(st + n, p.left, inv1, vec);
+      store_pairs(st + 3 * n, p.left, inv2, vec);
+    }
+  }
+}
+
+template <typename T, typename R, int ROWS>
+struct BwdTile {
   Four<T> x[ROWS][kTileThreads], z[ROWS][kTileThreads], gy[ROWS][kTileThreads];
   Four<R> r[ROWS][kTileThreads], gr[ROWS][kTileThreads];
   // two tiles where they fit beside TileRed in the 227 KB of a block
@@ -418,181 +482,195 @@ struct NormTile {
   static constexpr int kStages = 2 * kBytes <= 220 * 1024 ? 2 : 1;
 };
 
-// Persistent blocks: a block's next tile is copied while it works on this one, and the
-// parameter sums stay in registers until its last.
+// The parameter sums stay in registers until a block's last tile.
 template <typename T, typename R, int TX, int ROWS, bool LAYER>
 __global__ void __launch_bounds__(kTileThreads, 1)
-block_norm_bwd_tile_kernel(NormBwd a, NormShape s, int64_t ntiles, bool vec) {
-  using Tile = NormTile<T, R, ROWS>;
+block_norm_bwd_tile_kernel(NormBwd a, NormShape s, unsigned ntiles, bool vec) {
+  using Tile = BwdTile<T, R, ROWS>;
   constexpr int TY = kTileThreads / TX;
   extern __shared__ __align__(16) char smem_raw[];
   Tile *stage = reinterpret_cast<Tile *>(smem_raw);
   __shared__ __align__(16) TileRed red;
-  const int tid = threadIdx.x, tx = tid % TX, ty = tid / TX;
-  const int64_t tiles = (s.L + TX * kV - 1) / (TX * kV), n = s.B * s.L;
+  const int tid = threadIdx.x, ty = tid / TX;
+  const unsigned tiles = (unsigned)((s.L + TX * kV - 1) / (TX * kV));
+  const int64_t n = s.B * s.L;
+  const int D = (int)s.D;
   const float rd = 1.f / (float)s.D;
-  int turn = 0;
+  int turn = 0, at = 0;
 
   float w1[ROWS], b1[ROWS], sc[ROWS], w2[ROWS];
-  float acc[5][ROWS];
+  // sums over tokens: dr hat1, dy hat2, dr, dy
+  float2 acc[LAYER ? 4 : 2][ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const int64_t d = ty + i * TY;
-    const bool ok = d < s.D;
+    const int d = ty + i * TY;
+    const bool ok = d < D;
     w1[i] = ok ? ldf((const T *)a.w1 + d) : 0.f;
     w2[i] = ok ? ldf((const T *)a.w2 + d) : 0.f;
     b1[i] = LAYER && ok ? opt((const T *)a.b1, d, 0.f) : 0.f;
     sc[i] = ok ? opt((const T *)a.scale, d, 1.f) : 0.f;
 #pragma unroll
-    for (int j = 0; j < 5; ++j) acc[j][i] = 0.f;
+    for (int j = 0; j < (LAYER ? 4 : 2); ++j) acc[j][i] = both(0.f);
   }
-  auto fetch = [&](int64_t tile, Tile &m) {
-    const int64_t b = tile / tiles, t = tile % tiles * (TX * kV) + tx * kV;
-    const int64_t left = s.L - t, base = b * s.D * s.L + t;
-    if (left > 0)
+  auto fetch = [&](unsigned tile, Tile &m) {
+    const Place p = place<TX>(tile, tiles, s);
+    if (p.left > 0)
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
-        const int64_t d = ty + i * TY, o = base + d * s.L;
-        if (d >= s.D) continue;
-        if (vec) {
-          cp_async<sizeof(Four<T>)>(&m.x[i][tid], (const T *)a.x + o);
-          if (a.gate) cp_async<sizeof(Four<T>)>(&m.z[i][tid], (const T *)a.gate + o);
-          cp_async<sizeof(Four<R>)>(&m.r[i][tid], (const R *)a.residual + o);
-          cp_async<sizeof(Four<T>)>(&m.gy[i][tid], (const T *)a.gy + o);
-          if (a.grout) cp_async<sizeof(Four<R>)>(&m.gr[i][tid], (const R *)a.grout + o);
-        } else {
-          row_load4(m.x[i][tid], (const T *)a.x + o, 0, left, false);
-          if (a.gate) row_load4(m.z[i][tid], (const T *)a.gate + o, 0, left, false);
-          row_load4(m.r[i][tid], (const R *)a.residual + o, 0, left, false);
-          row_load4(m.gy[i][tid], (const T *)a.gy + o, 0, left, false);
-          if (a.grout) row_load4(m.gr[i][tid], (const R *)a.grout + o, 0, left, false);
-        }
+        const int d = ty + i * TY;
+        if (d >= D) continue;
+        const int64_t o = p.base + d * s.L;
+        fetch4(m.x[i][tid], (const T *)a.x + o, p.left, vec);
+        if (a.gate) fetch4(m.z[i][tid], (const T *)a.gate + o, p.left, vec);
+        fetch4(m.r[i][tid], (const R *)a.residual + o, p.left, vec);
+        fetch4(m.gy[i][tid], (const T *)a.gy + o, p.left, vec);
+        if (a.grout) fetch4(m.gr[i][tid], (const R *)a.grout + o, p.left, vec);
       }
     copies_commit();
   };
-  int at = 0;
-  if (blockIdx.x < ntiles) fetch(blockIdx.x, stage[0]);
-  for (int64_t tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
-    const int64_t b = tile / tiles, t = tile % tiles * (TX * kV) + tx * kV;
-    const int64_t left = s.L - t, base = b * s.D * s.L + t;
-    const bool in = left > 0;
-    float m1[kV], inv1[kV], m2[kV], inv2[kV];
+  Four<float> sn[4];  // the next tile's statistics
+  auto fetch_stats = [&](unsigned tile) {
+    const Place p = place<TX>(tile, tiles, s);
+    const float *st = a.stats + p.b * s.L + p.t;
+    if (LAYER) row_load4(sn[0], st, 0, p.left, vec), row_load4(sn[2], st + 2 * n, 0, p.left, vec);
+    row_load4(sn[1], st + n, 0, p.left, vec);
+    row_load4(sn[3], st + 3 * n, 0, p.left, vec);
+  };
+  if (blockIdx.x < ntiles) {
+    fetch(blockIdx.x, stage[0]);
+    fetch_stats(blockIdx.x);
+  }
+  for (unsigned tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
+    const Place p = place<TX>(tile, tiles, s);
+    Two m1, inv1, m2, inv2, v, u;
 #pragma unroll
-    for (int k = 0; k < kV; ++k) {
-      const int64_t i = b * s.L + t + k;
-      const bool ok = k < left;
-      m1[k] = LAYER && ok ? a.stats[i] : 0.f;
-      inv1[k] = ok ? a.stats[n + i] : 0.f;
-      m2[k] = LAYER && ok ? a.stats[2 * n + i] : 0.f;
-      inv2[k] = ok ? a.stats[3 * n + i] : 0.f;
+    for (int k = 0; k < kV / 2; ++k) {
+      m1[k] = LAYER ? neg2(sn[0].pair(k)) : both(0.f);
+      inv1[k] = sn[1].pair(k);
+      m2[k] = LAYER ? neg2(sn[2].pair(k)) : both(0.f);
+      inv2[k] = sn[3].pair(k);
+      v[k] = u[k] = both(0.f);
     }
-    if (Tile::kStages == 2 && tile + gridDim.x < ntiles) {
+    const bool more = tile + gridDim.x < ntiles;
+    if (Tile::kStages == 2 && more) {
       fetch(tile + gridDim.x, stage[at ^ 1]);
       copies_wait<1>();
     } else {
       copies_wait<0>();
     }
+    if (more) fetch_stats(tile + gridDim.x);
     const Tile &m = stage[at];
-    float hat1[ROWS][kV], hat2[ROWS][kV], sg[ROWS][kV], v[kV], u[kV];
-#pragma unroll
-    for (int k = 0; k < kV; ++k) v[k] = u[k] = 0.f;
+    float2 hat1[ROWS][kV / 2], hat2[ROWS][kV / 2], sg[ROWS][kV / 2];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      const bool ok = in && ty + i * TY < s.D;
-      float x[kV], z[kV], r[kV], gy[kV];
-      get4(m.x[i][tid], x);
-      get4(m.r[i][tid], r);
-      get4(m.gy[i][tid], gy);
-      if (a.gate) get4(m.z[i][tid], z);
+      const bool ok = p.left > 0 && ty + i * TY < D;
 #pragma unroll
-      for (int k = 0; k < kV; ++k) {
-        float g = x[k];
-        sg[i][k] = 0.f;
+      for (int k = 0; k < kV / 2; ++k) {
+        float2 g = m.x[i][tid].pair(k), r = m.r[i][tid].pair(k), dy = m.gy[i][tid].pair(k);
+        sg[i][k] = both(0.f);
         if (a.gate) {
-          sg[i][k] = sigmoid_for<T>(z[k]);
-          g *= z[k] * sg[i][k];
+          const float2 z = m.z[i][tid].pair(k);
+          sg[i][k] = sigmoid2<T>(z);
+          g = mul2(g, mul2(z, sg[i][k]));
         }
-        hat1[i][k] = ok ? (g - m1[k]) * inv1[k] : 0.f;
-        hat2[i][k] =
-            ok ? (fmaf(sc[i], fmaf(hat1[i][k], w1[i], b1[i]), r[k]) - m2[k]) * inv2[k] : 0.f;
-        const float dy = ok ? gy[k] : 0.f, d2 = dy * w2[i];
-        v[k] = fmaf(d2, hat2[i][k], v[k]);
-        u[k] += d2;
-        acc[1][i] = fmaf(dy, hat2[i][k], acc[1][i]);
-        if (LAYER) acc[4][i] += dy;
+        if (!ok) g = r = dy = both(0.f);
+        float2 h1 = mul2(LAYER ? add2(g, m1[k]) : g, inv1[k]);
+        if (LAYER && !ok) h1 = both(0.f);
+        float2 h2 = fma2(h1, both(sc[i] * w1[i]), r);
+        if (LAYER) h2 = add2(h2, add2(both(sc[i] * b1[i]), m2[k]));
+        h2 = mul2(h2, inv2[k]);
+        if (LAYER && !ok) h2 = both(0.f);
+        hat1[i][k] = h1;
+        hat2[i][k] = h2;
+        const float2 d2 = mul2(dy, both(w2[i]));
+        v[k] = fma2(d2, h2, v[k]);
+        acc[1][i] = fma2(dy, h2, acc[1][i]);
+        if (LAYER) {
+          u[k] = add2(u[k], d2);
+          acc[3][i] = add2(acc[3][i], dy);
+        }
       }
     }
     tile_sum4<TX>(v, red, turn);
     if (LAYER) tile_sum4<TX>(u, red, turn);
-    float c2[kV], e2[kV];
+    Two c, e;
 #pragma unroll
-    for (int k = 0; k < kV; ++k) {
-      c2[k] = v[k] * rd;
-      e2[k] = LAYER ? u[k] * rd : 0.f;
-      v[k] = u[k] = 0.f;
+    for (int k = 0; k < kV / 2; ++k) {
+      c[k] = mul2(v[k], both(-rd));
+      e[k] = mul2(u[k], both(-rd));
+      v[k] = u[k] = both(0.f);
     }
-    // the gradient of p takes hat2's place
+    // the gradient of hat1 takes hat2's place
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      const int64_t d = ty + i * TY;
-      const bool ok = in && d < s.D;
-      float gy[kV], gr[kV], dr[kV];
-      get4(m.gy[i][tid], gy);
-      if (a.grout) get4(m.gr[i][tid], gr);
+      const int d = ty + i * TY;
+      const bool ok = p.left > 0 && d < D;
+      Two dr;
 #pragma unroll
-      for (int k = 0; k < kV; ++k) {
-        const float up = a.grout ? gr[k] : 0.f;
-        dr[k] = ok ? fmaf(inv2[k], fmaf(-hat2[i][k], c2[k], gy[k] * w2[i]) - e2[k], up) : 0.f;
-        const float dp = dr[k] * sc[i], d1 = dp * w1[i];
+      for (int k = 0; k < kV / 2; ++k) {
+        float2 o = fma2(hat2[i][k], c[k], mul2(m.gy[i][tid].pair(k), both(w2[i])));
+        if (LAYER) o = add2(o, e[k]);
+        dr[k] = a.grout ? fma2(inv2[k], o, m.gr[i][tid].pair(k)) : mul2(inv2[k], o);
+        if (!ok) dr[k] = both(0.f);
+        const float2 d1 = mul2(dr[k], both(sc[i] * w1[i]));
         hat2[i][k] = d1;
-        v[k] = fmaf(d1, hat1[i][k], v[k]);
-        u[k] += d1;
-        acc[0][i] = fmaf(dp, hat1[i][k], acc[0][i]);
-        acc[2][i] = fmaf(dr[k], fmaf(hat1[i][k], w1[i], b1[i]), acc[2][i]);
-        if (LAYER) acc[3][i] += dp;
+        v[k] = fma2(d1, hat1[i][k], v[k]);
+        acc[0][i] = fma2(dr[k], hat1[i][k], acc[0][i]);
+        if (LAYER) {
+          u[k] = add2(u[k], d1);
+          acc[2][i] = add2(acc[2][i], dr[k]);
+        }
       }
-      if (ok) row_store4((R *)a.gresidual + base + d * s.L, 0, left, dr, vec);
+      if (ok) store_pairs((R *)a.gresidual + p.base + d * s.L, p.left, dr, vec);
     }
     tile_sum4<TX>(v, red, turn);
     if (LAYER) tile_sum4<TX>(u, red, turn);
 #pragma unroll
-    for (int k = 0; k < kV; ++k) {
-      v[k] *= rd;
-      u[k] = LAYER ? u[k] * rd : 0.f;
+    for (int k = 0; k < kV / 2; ++k) {
+      c[k] = mul2(v[k], both(-rd));
+      e[k] = mul2(u[k], both(-rd));
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      const int64_t d = ty + i * TY;
-      if (!in || d >= s.D) continue;
-      float x[kV], z[kV], gx[kV], gz[kV];
-      get4(m.x[i][tid], x);
-      if (a.gate) get4(m.z[i][tid], z);
+      const int d = ty + i * TY;
+      if (p.left <= 0 || d >= D) continue;
+      Two gx, gz;
 #pragma unroll
-      for (int k = 0; k < kV; ++k) {
-        const float dg = inv1[k] * (fmaf(-hat1[i][k], v[k], hat2[i][k]) - u[k]);
-        gx[k] = dg;
+      for (int k = 0; k < kV / 2; ++k) {
+        float2 o = fma2(hat1[i][k], c[k], hat2[i][k]);
+        if (LAYER) o = add2(o, e[k]);
+        gx[k] = mul2(inv1[k], o);
         if (a.gate) {
-          const float h = dg * sg[i][k];
-          gx[k] = h * z[k];
-          gz[k] = h * x[k] * fmaf(z[k], 1.f - sg[i][k], 1.f);
+          const float2 z = m.z[i][tid].pair(k), h = mul2(gx[k], sg[i][k]);
+          gx[k] = mul2(h, z);
+          gz[k] = mul2(mul2(h, m.x[i][tid].pair(k)),
+                       fma2(z, fma2(sg[i][k], both(-1.f), both(1.f)), both(1.f)));
         }
       }
-      row_store4((T *)a.gx + base + d * s.L, 0, left, gx, vec);
-      if (a.gate) row_store4((T *)a.ggate + base + d * s.L, 0, left, gz, vec);
+      store_pairs((T *)a.gx + p.base + d * s.L, p.left, gx, vec);
+      if (a.gate) store_pairs((T *)a.ggate + p.base + d * s.L, p.left, gz, vec);
     }
     if (Tile::kStages == 2) at ^= 1;
-    else if (tile + gridDim.x < ntiles) fetch(tile + gridDim.x, stage[0]);
+    else if (more) fetch(tile + gridDim.x, stage[0]);
   }
+  // post_weight: scale sum(dr hat1); pre_weight: sum(dy hat2); scale: sum(dr p) = w1 sum(dr hat1) +
+  // b1 sum(dr); post_bias: scale sum(dr); pre_bias: sum(dy)
 #pragma unroll
-  for (int j = 0; j < (LAYER ? 5 : 3); ++j)
+  for (int i = 0; i < ROWS; ++i) {
+    float q[4];
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      float q = acc[j][i];
+    for (int j = 0; j < 4; ++j) {
+      q[j] = j < (LAYER ? 4 : 2) ? acc[LAYER ? j : j & 1][i].x + acc[LAYER ? j : j & 1][i].y : 0.f;
 #pragma unroll
-      for (int o = TX / 2; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-      const int64_t d = ty + i * TY;
-      if (tx == 0 && d < s.D) a.part[(j * (int64_t)gridDim.x + blockIdx.x) * s.D + d] = q;
+      for (int o = TX / 2; o > 0; o >>= 1) q[j] += __shfl_xor_sync(0xffffffffu, q[j], o);
     }
+    const int d = ty + i * TY;
+    if (tid % TX || d >= D) continue;
+    const float out[5] = {sc[i] * q[0], q[1], fmaf(w1[i], q[0], b1[i] * q[2]), sc[i] * q[2], q[3]};
+#pragma unroll
+    for (int j = 0; j < (LAYER ? 5 : 3); ++j)
+      a.part[(j * (int64_t)gridDim.x + blockIdx.x) * s.D + d] = out[j];
+  }
 }
 
 // One column of threads per 32 channels: eight rows of threads take every eighth tile, then
@@ -669,10 +747,15 @@ int fwd_launch(const NormFwd &a, const NormShape &s, cudaStream_t st) {
   if (tile_tx(s.D, s.L)) {
     const bool vec = s.L % kV == 0 && aligned_to(a.x, sizeof(Four<T>)) &&
                      aligned_to(a.gate, sizeof(Four<T>)) && aligned_to(a.y, sizeof(Four<T>)) &&
-                     aligned_to(a.residual, sizeof(Four<R>)) && aligned_to(a.rout, sizeof(Four<R>));
+                     aligned_to(a.residual, sizeof(Four<R>)) &&
+                     aligned_to(a.rout, sizeof(Four<R>)) && aligned_to_16(a.stats);
     return by_tile(s.D, [&](auto tx, auto rows) {
-      block_norm_fwd_tile_kernel<T, R, decltype(tx)::value, decltype(rows)::value, LAYER>
-          <<<grid, kTileThreads, 0, st>>>(a, s, vec);
+      using Tile = FwdTile<T, R, decltype(rows)::value>;
+      const int smem = 2 * (int)sizeof(Tile), most = Tile::kBlocks * sm_count();
+      auto kern = block_norm_fwd_tile_kernel<T, R, decltype(tx)::value, decltype(rows)::value, LAYER>;
+      if (set_smem_once((const void *)kern, smem) != cudaSuccess)
+        return check_launch("block_norm_fwd_tile_kernel shared memory");
+      kern<<<grid < (unsigned)most ? grid : most, kTileThreads, smem, st>>>(a, s, grid, vec);
       return check_launch("block_norm_fwd_tile_kernel");
     });
   }
@@ -696,17 +779,17 @@ int bwd_main(const NormBwd &a, const NormShape &s, cudaStream_t st) {
                      aligned_to(a.gy, sizeof(Four<T>)) && aligned_to(a.gx, sizeof(Four<T>)) &&
                      aligned_to(a.residual, sizeof(Four<R>)) &&
                      aligned_to(a.grout, sizeof(Four<R>)) &&
-                     aligned_to(a.gresidual, sizeof(Four<R>));
+                     aligned_to(a.gresidual, sizeof(Four<R>)) && aligned_to_16(a.stats);
     const unsigned grid = (unsigned)part_count(s.B, s.D, s.L);
     const int64_t tiles = tile_count(s.B, s.D, s.L);
     return by_tile(s.D, [&](auto tx, auto rows) {
       constexpr int ROWS = decltype(rows)::value;
-      using Tile = NormTile<T, R, ROWS>;
+      using Tile = BwdTile<T, R, ROWS>;
       const int smem = Tile::kStages * (int)sizeof(Tile);
       auto kern = block_norm_bwd_tile_kernel<T, R, decltype(tx)::value, ROWS, LAYER>;
       if (set_smem_once((const void *)kern, smem) != cudaSuccess)
         return check_launch("block_norm_bwd_tile_kernel shared memory");
-      kern<<<grid, kTileThreads, smem, st>>>(a, s, tiles, vec);
+      kern<<<grid, kTileThreads, smem, st>>>(a, s, (unsigned)tiles, vec);
       return check_launch("block_norm_bwd_tile_kernel");
     });
   }

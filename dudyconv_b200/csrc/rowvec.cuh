@@ -7,70 +7,90 @@
 
 namespace dudy {
 
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// two neighbouring 16-bit elements of one word
+__device__ __forceinline__ float2 pair_of(uint32_t w, __half) {
+  return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+__device__ __forceinline__ float2 pair_of(uint32_t w, __nv_bfloat16) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w));
+}
+__device__ __forceinline__ uint32_t word_of(float2 v, __half) {
+  const __half2 h = __float22half2_rn(v);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t word_of(float2 v, __nv_bfloat16) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(v);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
 // ---- eight positions of a row ------------------------------------------------------------
-// 16-bit rows: one 16-byte access, fp32 rows: two. `p` is 16-byte aligned.
+// Kept in whole 32-bit words from the load on, also where the elements are loaded one by one: the
+// conversion waits until it is asked for, so loads that come early stay in flight.
 template <typename T>
-__device__ __forceinline__ void row_load8(const T *p, float (&v)[8]) {
-  const uint4 q = *reinterpret_cast<const uint4 *>(p);
-  const T *e = reinterpret_cast<const T *>(&q);
+struct RowEight {
+  static constexpr int kW = 2 * sizeof(T);
+  uint32_t w[kW];
+  // row[t .. t+8), zero at and behind `end`, which is not read. `vec`: rows and t start on eight
+  // elements.
+  __device__ __forceinline__ void load(const T *row, int t, int end, bool vec) {
+    if (vec && t + 8 <= end) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = Elem<T>::to_f(e[i]);
-}
-template <>
-__device__ __forceinline__ void row_load8<float>(const float *p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4 *>(p);
-  const float4 b = *reinterpret_cast<const float4 *>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
+      for (int i = 0; i < kW / 4; ++i) {
+        const uint4 q = reinterpret_cast<const uint4 *>(row + t)[i];
+        w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+      }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = t + i < end ? reinterpret_cast<const uint32_t *>(row)[t + i] : 0u;
+    } else {
+      const uint16_t *h = reinterpret_cast<const uint16_t *>(row);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = (t + 2 * i < end ? (uint32_t)h[t + 2 * i] : 0u) |
+               (t + 2 * i + 1 < end ? (uint32_t)h[t + 2 * i + 1] << 16 : 0u);
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 p;
+      if constexpr (sizeof(T) == 4) p = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+      else p = pair_of(w[i], T());
+      v[2 * i] = p.x;
+      v[2 * i + 1] = p.y;
+    }
+  }
+};
 
+// row[t .. t+8) = v, before `end`
 template <typename T>
-__device__ __forceinline__ void row_store8(T *p, const float (&v)[8]) {
-  uint4 q;
-  T *e = reinterpret_cast<T *>(&q);
+__device__ __forceinline__ void row_store8(T *row, int t, int end, const float (&v)[8], bool vec) {
+  if (vec && t + 8 <= end) {
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float4 *>(row + t)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4 *>(row + t)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      *reinterpret_cast<uint4 *>(row + t) =
+          make_uint4(word_of(make_float2(v[0], v[1]), T()), word_of(make_float2(v[2], v[3]), T()),
+                     word_of(make_float2(v[4], v[5]), T()), word_of(make_float2(v[6], v[7]), T()));
+    }
+  } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = Elem<T>::from_f(v[i]);
-  *reinterpret_cast<uint4 *>(p) = q;
-}
-template <>
-__device__ __forceinline__ void row_store8<float>(float *p, const float (&v)[8]) {
-  *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-}
-
-// Positions [t, t+8) of a row, zero at and after `end` (what lies there is not read).
-template <typename T, bool VEC>
-__device__ __forceinline__ void row_load8_until(const T *row, int64_t t, int64_t end,
-                                                float (&v)[8]) {
-  if (VEC && t + 8 <= end) {
-    row_load8(row + t, v);
-    return;
+    for (int i = 0; i < 8; ++i)
+      if (t + i < end) stf(row + t + i, v[i]);
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = t + i < end ? ldf(row + t + i) : 0.f;
-}
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void row_store8_until(T *row, int64_t t, int64_t end,
-                                                 const float (&v)[8]) {
-  if (VEC && t + 8 <= end) {
-    row_store8(row + t, v);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (t + i < end) stf(row + t + i, v[i]);
 }
 
 // ---- four positions of a row, as they lie in memory --------------------------------------------
-// Kept in whole 32-bit words from the load on, also where the elements are loaded one by one: the
-// conversion waits until get(), so loads that come early stay in flight.
 template <typename T>
 struct RowFour;
 template <>
 struct RowFour<float> {
   uint32_t w[4];
   __device__ __forceinline__ float get(int i) const { return __uint_as_float(w[i]); }
+  __device__ __forceinline__ float2 pair(int i) const { return make_float2(get(2 * i), get(2 * i + 1)); }
   __device__ __forceinline__ void load_all(const float *p) {
     const uint4 q = *reinterpret_cast<const uint4 *>(p);
     w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
@@ -87,6 +107,7 @@ struct RowFour {
     const uint16_t h = (uint16_t)(w[i >> 1] >> (i & 1 ? 16 : 0));
     return Elem<T>::to_f(*reinterpret_cast<const T *>(&h));
   }
+  __device__ __forceinline__ float2 pair(int i) const { return pair_of(w[i], T()); }
   __device__ __forceinline__ void load_all(const T *p) {
     const uint2 q = *reinterpret_cast<const uint2 *>(p);
     w[0] = q.x; w[1] = q.y;
@@ -97,12 +118,8 @@ struct RowFour {
     w[1] = (n > 2 ? (uint32_t)h[2] : 0u) | (n > 3 ? (uint32_t)h[3] << 16 : 0u);
   }
   __device__ __forceinline__ void set(const float (&v)[4]) {
-    T e[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = Elem<T>::from_f(v[i]);
-    const uint16_t *h = reinterpret_cast<const uint16_t *>(e);
-    w[0] = (uint32_t)h[0] | (uint32_t)h[1] << 16;
-    w[1] = (uint32_t)h[2] | (uint32_t)h[3] << 16;
+    w[0] = word_of(make_float2(v[0], v[1]), T());
+    w[1] = word_of(make_float2(v[2], v[3]), T());
   }
   __device__ __forceinline__ void store_all(T *p) const {
     *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
@@ -149,9 +166,7 @@ __device__ __forceinline__ void row_store2(T *row, int64_t t, int64_t end, const
     if constexpr (sizeof(T) == 4) {
       *reinterpret_cast<float2 *>(row + t) = make_float2(v[0], v[1]);
     } else {
-      const T e[2] = {Elem<T>::from_f(v[0]), Elem<T>::from_f(v[1])};
-      const uint16_t *h = reinterpret_cast<const uint16_t *>(e);
-      *reinterpret_cast<uint32_t *>(row + t) = (uint32_t)h[0] | (uint32_t)h[1] << 16;
+      *reinterpret_cast<uint32_t *>(row + t) = word_of(make_float2(v[0], v[1]), T());
     }
   } else {
 #pragma unroll
@@ -161,11 +176,21 @@ __device__ __forceinline__ void row_store2(T *row, int64_t t, int64_t end, const
 }
 
 // ---- activations --------------------------------------------------------------------------
-// 1 / (1 + exp(-v)); 16-bit tensors use the fast exponential and division (relative error
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// 1 / (1 + exp(-v)); 16-bit tensors use the fast exponential and reciprocal (relative error
 // about 2^-21, far below the rounding of the result), fp32 tensors the accurate ones.
 template <typename T>
 __device__ __forceinline__ float sigmoid_for(float v) {
-  return __fdividef(1.f, 1.f + __expf(-v));
+  return rcp(1.f + ex2(-1.4426950408889634f * v));
 }
 template <>
 __device__ __forceinline__ float sigmoid_for<float>(float v) {

@@ -70,16 +70,6 @@ template <typename T>
 __device__ __forceinline__ constexpr float unscaled() {
   return sizeof(T) == 4 ? 1.f : 0.6931471805599453f;
 }
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ float rcp(float x) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 template <typename T>
 __device__ __forceinline__ float decay(float x) {
   return ex2(x);
@@ -113,7 +103,6 @@ __device__ __forceinline__ float softplus<float>(float x, float &slope) {
   return fmaxf(x, 0.f) + log1pf(e);
 }
 
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float2 lo(const float4 &v) { return make_float2(v.x, v.y); }
 __device__ __forceinline__ float2 hi(const float4 &v) { return make_float2(v.z, v.w); }
 __device__ __forceinline__ float4 quad(const float2 &a, const float2 &b) {

@@ -10,13 +10,14 @@
 // Positions at and behind a sequence's length are not read, give zeros and carry no gradient.
 //
 // Both directions are bound by HBM: the forward reads and writes each row once, the backward
-// reads two rows and writes one. A warp takes 256 consecutive positions of a row, eight to a
-// lane (16-byte accesses); the S-1 <= 7 inputs before a lane's own come from the lane before
-// it by shuffles, so no row is read twice. The backward walks its 1024 positions from the
+// reads two rows and writes one. A warp takes up to 1024 positions of a row, 256 at a time, eight
+// to a lane (16-byte accesses); the S-1 <= 7 inputs before a lane's own come from the lane before
+// it by shuffles, so no row is read twice. The forward has all of a segment's loads in flight at
+// once; the backward loads the next block before it works on one. It walks its positions from the
 // right, because dx needs the S-1 values of dv behind it: those come from the next lane, and at
 // the right end of a block from the block done just before. Parameter gradients are summed in
-// registers over the 1024 positions, once across the warp, and by a second kernel over batch
-// and segments in a fixed order.
+// registers over the segment, once across the warp, and by a second kernel over batch and
+// segments in a fixed order.
 #include "rowvec.cuh"
 
 namespace dudy {
@@ -28,75 +29,96 @@ constexpr int kSegBlocks = 4;      // blocks of a backward segment
 constexpr int64_t kSegT = kBlockT * kSegBlocks;
 
 struct ConvShape {
-  int64_t B, D, L;
-  int silu;
+  int64_t rows, D, L;
+  unsigned segs;
+  int silu, vec;
 };
 
-__device__ __forceinline__ int64_t clamp_len(const int32_t *lengths, int64_t b, int64_t L) {
-  if (!lengths) return L;
+__device__ __forceinline__ int clamp_len(const int32_t *lengths, int64_t b, int64_t L) {
+  if (!lengths) return (int)L;
   const int64_t n = lengths[b];
-  return n < 0 ? 0 : (n > L ? L : n);
+  return (int)(n < 0 ? 0 : (n > L ? L : n));
 }
 
 // xe[t] for t < 0: the state's entry, or zero
 template <typename T, int S>
-__device__ __forceinline__ float before(const T *state_row, int64_t t) {
+__device__ __forceinline__ float before(const T *state_row, int t) {
   return state_row && t >= -(S - 1) ? ldf(state_row + (S - 1) + t) : 0.f;
 }
 
-// The lane's window xw[0 .. S-2] = xe[t-(S-1) .. t-1], xw[S-1 ..] = xe[t .. t+7], zero at and
-// after `len`. `t` is the lane's first position, t0 the warp's.
-template <typename T, int S, bool VEC>
-__device__ __forceinline__ void load_window(const T *row, const T *state_row, int64_t t0,
-                                            int64_t len, int lane, float (&xw)[8 + S - 1]) {
-  const int64_t t = t0 + lane * 8;
-  float x[8];
-  row_load8_until<T, VEC>(row, t, len, x);
+// The lane's window xw[0 .. S-2] = xe[t-(S-1) .. t-1], xw[S-1 ..] = xe[t .. t+7] from its own
+// eight, zero at and after `len`. `t0` is the warp's first position.
+template <typename T, int S>
+__device__ __forceinline__ void window(const RowEight<T> &x, const T *row, const T *state_row,
+                                       int t0, int len, int lane, float (&xw)[8 + S - 1]) {
+  float v[8];
+  x.get(v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) xw[S - 1 + i] = x[i];
+  for (int i = 0; i < 8; ++i) xw[S - 1 + i] = v[i];
 #pragma unroll
-  for (int i = 0; i < S - 1; ++i) {
-    const float left = __shfl_up_sync(0xffffffffu, x[8 - (S - 1) + i], 1);
-    const int64_t p = t0 - (S - 1) + i;
-    xw[i] = left;
-    if (lane == 0)
+  for (int i = 0; i < S - 1; ++i)
+    xw[i] = __shfl_up_sync(0xffffffffu, v[8 - (S - 1) + i], 1);
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) {
+      const int p = t0 - (S - 1) + i;
       xw[i] = p < 0 ? before<T, S>(state_row, p) : (p < len ? ldf(row + p) : 0.f);
+    }
   }
 }
 
-template <typename T, int S, bool VEC>
+// the row and segment of a warp; false: none
+__device__ __forceinline__ bool place(const ConvShape &s, int64_t &row, int &lo, int &hi) {
+  const unsigned seg = blockIdx.x % s.segs;
+  row = (int64_t)(blockIdx.x / s.segs) * kWarps + (threadIdx.x >> 5);
+  lo = (int)(seg * (unsigned)kSegT);
+  hi = lo + kSegT < s.L ? lo + (int)kSegT : (int)s.L;
+  return row < s.rows;
+}
+
+template <typename T, int S>
 __global__ void __launch_bounds__(kWarps * 32)
 short_conv_fwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const T *__restrict__ bias,
                       const T *__restrict__ state, const int32_t *__restrict__ lengths,
-                      T *__restrict__ out, T *__restrict__ final_state, ConvShape s,
-                      int64_t blocks_per_row, int64_t units) {
+                      T *__restrict__ out, T *__restrict__ final_state, ConvShape s) {
   const int lane = threadIdx.x & 31;
-  const int64_t unit = blockIdx.x * (int64_t)kWarps + (threadIdx.x >> 5);
-  if (unit >= units) return;
-  const int64_t row = unit / blocks_per_row, t0 = (unit % blocks_per_row) * kBlockT;
-  const int64_t b = row / s.D, d = row % s.D;
-  const int64_t len = clamp_len(lengths, b, s.L);
+  int64_t row;
+  int lo, hi;
+  if (!place(s, row, lo, hi)) return;
+  const unsigned d = (unsigned)row % (unsigned)s.D;
+  const int len = clamp_len(lengths, (unsigned)row / (unsigned)s.D, s.L);
   const T *xr = x + row * s.L;
   const T *sr = state ? state + row * (S - 1) : nullptr;
+  T *outr = out + row * s.L;
+  RowEight<T> xs[kSegBlocks];
+#pragma unroll
+  for (int k = 0; k < kSegBlocks; ++k)
+    if (lo + k * kBlockT < hi) xs[k].load(xr, lo + k * kBlockT + lane * 8, len, s.vec);
   float wt[S];
 #pragma unroll
   for (int j = 0; j < S; ++j) wt[j] = ldf(w + d * S + j);
   const float bv = bias ? ldf(bias + d) : 0.f;
-  float xw[8 + S - 1];
-  load_window<T, S, VEC>(xr, sr, t0, len, lane, xw);
-  const int64_t t = t0 + lane * 8;
-  float o[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float v = bv;
+  for (int k = 0; k < kSegBlocks; ++k) {
+    const int t0 = lo + k * kBlockT, t = t0 + lane * 8;
+    if (t0 >= hi) break;
+    float xw[8 + S - 1], o[8];
+    window<T, S>(xs[k], xr, sr, t0, len, lane, xw);
 #pragma unroll
-    for (int j = 0; j < S; ++j) v = fmaf(wt[j], xw[i + j], v);
-    if (s.silu) v *= sigmoid_for<T>(v);
-    o[i] = t + i < len ? v : 0.f;
+    for (int i = 0; i < 8; ++i) {
+      float v = bv;
+#pragma unroll
+      for (int j = 0; j < S; ++j) v = fmaf(wt[j], xw[i + j], v);
+      o[i] = s.silu ? v * sigmoid_for<T>(v) : v;
+    }
+    if (t + 8 > len) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = t + i < len ? o[i] : 0.f;
+    }
+    row_store8(outr, t, (int)s.L, o, s.vec);
   }
-  row_store8_until<T, VEC>(out + row * s.L, t, s.L, o);
-  if (final_state && t0 == 0 && lane < S - 1) {
-    const int64_t p = len - (S - 1) + lane;
+  if (final_state && lo == 0 && lane < S - 1) {
+    const int p = len - (S - 1) + lane;
     stf(final_state + row * (S - 1) + lane, p < 0 ? before<T, S>(sr, p) : ldf(xr + p));
   }
 }
@@ -109,24 +131,28 @@ __device__ __forceinline__ float dv_of(float v, float go, int silu) {
   return go * (sg * fmaf(v, 1.f - sg, 1.f));
 }
 
-template <typename T, int S, bool VEC>
+template <typename T, int S>
 __global__ void __launch_bounds__(kWarps * 32)
 short_conv_bwd_kernel(const T *__restrict__ go, const T *__restrict__ gfinal,
                       const T *__restrict__ x, const T *__restrict__ w,
                       const T *__restrict__ bias, const T *__restrict__ state,
                       const int32_t *__restrict__ lengths, T *__restrict__ gx,
-                      T *__restrict__ gstate, float *__restrict__ part, ConvShape s,
-                      int64_t segs, int64_t units) {
+                      T *__restrict__ gstate, float *__restrict__ part, ConvShape s) {
   const int lane = threadIdx.x & 31;
-  const int64_t unit = blockIdx.x * (int64_t)kWarps + (threadIdx.x >> 5);
-  if (unit >= units) return;
-  const int64_t row = unit / segs, seg = unit % segs;
-  const int64_t b = row / s.D, d = row % s.D;
-  const int64_t len = clamp_len(lengths, b, s.L);
+  int64_t row;
+  int lo, hi;
+  if (!place(s, row, lo, hi)) return;
+  const unsigned d = (unsigned)row % (unsigned)s.D, b = (unsigned)row / (unsigned)s.D;
+  const int len = clamp_len(lengths, b, s.L);
   const T *xr = x + row * s.L;
   const T *gr = go + row * s.L;
+  T *gxr = gx + row * s.L;
   const T *sr = state ? state + row * (S - 1) : nullptr;
   const T *fr = gfinal ? gfinal + row * (S - 1) : nullptr;
+  const int last = lo + (hi - lo - 1) / kBlockT * kBlockT;
+  RowEight<T> xn, gn;  // the next block
+  xn.load(xr, last + lane * 8, len, s.vec);
+  gn.load(gr, last + lane * 8, len, s.vec);
   float wt[S];
 #pragma unroll
   for (int j = 0; j < S; ++j) wt[j] = ldf(w + d * S + j);
@@ -135,18 +161,16 @@ short_conv_bwd_kernel(const T *__restrict__ go, const T *__restrict__ gfinal,
 #pragma unroll
   for (int j = 0; j < S; ++j) dw[j] = 0.f;
 
-  const int64_t lo = seg * kSegT;
-  const int64_t hi = lo + kSegT < s.L ? lo + kSegT : s.L;
   // dv at the S-1 positions behind the segment: lane i takes position hi + i
   float behind[S];
   {
     float mine = 0.f;
-    const int64_t p = hi + lane;
+    const int p = hi + lane;
     if (lane < S - 1 && p < len) {
       float v = bv;
 #pragma unroll
       for (int j = 0; j < S; ++j) {
-        const int64_t q = p - (S - 1) + j;
+        const int q = p - (S - 1) + j;
         v = fmaf(wt[j], q < 0 ? before<T, S>(sr, q) : ldf(xr + q), v);
       }
       mine = dv_of<T>(v, ldf(gr + p), s.silu);
@@ -154,18 +178,29 @@ short_conv_bwd_kernel(const T *__restrict__ go, const T *__restrict__ gfinal,
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) behind[i] = __shfl_sync(0xffffffffu, mine, i);
   }
-  for (int64_t t0 = lo + (hi - lo - 1) / kBlockT * kBlockT; t0 >= lo; t0 -= kBlockT) {
-    const int64_t t = t0 + lane * 8;
-    float xw[8 + S - 1], g[8];
-    load_window<T, S, VEC>(xr, sr, t0, len, lane, xw);
-    row_load8_until<T, VEC>(gr, t, len, g);
-    float dv[8 + S - 1];
+  for (int t0 = last; t0 >= lo; t0 -= kBlockT) {
+    const int t = t0 + lane * 8;
+    const RowEight<T> xc = xn, gc = gn;
+    if (t0 > lo) {
+      xn.load(xr, t - kBlockT, len, s.vec);
+      gn.load(gr, t - kBlockT, len, s.vec);
+    }
+    float xw[8 + S - 1], g[8], dv[8 + S - 1];
+    window<T, S>(xc, xr, sr, t0, len, lane, xw);
+    gc.get(g);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float v = bv;
 #pragma unroll
       for (int j = 0; j < S; ++j) v = fmaf(wt[j], xw[i + j], v);
-      dv[i] = t + i < len ? dv_of<T>(v, g[i], s.silu) : 0.f;
+      dv[i] = dv_of<T>(v, g[i], s.silu);
+    }
+    if (t + 8 > len) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dv[i] = t + i < len ? dv[i] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
       db += dv[i];
 #pragma unroll
       for (int j = 0; j < S; ++j) dw[j] = fmaf(dv[i], xw[i + j], dw[j]);
@@ -179,19 +214,22 @@ short_conv_bwd_kernel(const T *__restrict__ go, const T *__restrict__ gfinal,
     float o[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float v = 0.f;
+      o[i] = 0.f;
 #pragma unroll
-      for (int j = 0; j < S; ++j) v = fmaf(wt[j], dv[i + S - 1 - j], v);
-      o[i] = t + i < len ? v : 0.f;
+      for (int j = 0; j < S; ++j) o[i] = fmaf(wt[j], dv[i + S - 1 - j], o[i]);
     }
-    if (fr) {
+    if (fr && t + 8 > len - (S - 1)) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int64_t k = t + i - (len - (S - 1));
+        const int k = t + i - (len - (S - 1));
         if (k >= 0 && k < S - 1) o[i] += ldf(fr + k);
       }
     }
-    row_store8_until<T, VEC>(gx + row * s.L, t, s.L, o);
+    if (t + 8 > len) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = t + i < len ? o[i] : 0.f;
+    }
+    row_store8(gxr, t, (int)s.L, o, s.vec);
     if (gstate && t0 == 0 && lane == 0) {
 #pragma unroll
       for (int i = 0; i < S - 1; ++i) {
@@ -204,8 +242,8 @@ short_conv_bwd_kernel(const T *__restrict__ go, const T *__restrict__ gfinal,
       }
     }
   }
-  // part[(j * D + d) * (B * segs) + b * segs + seg], j = S the bias
-  const int64_t per = s.B * segs, at = b * segs + seg;
+  // part[(j * D + d) * per + b * segs + seg], j = S the bias
+  const int64_t per = s.rows / s.D * s.segs, at = (int64_t)b * s.segs + blockIdx.x % s.segs;
 #pragma unroll
   for (int j = 0; j <= S; ++j) {
     float v = j < S ? dw[j] : db;
@@ -264,8 +302,8 @@ int validate(int64_t B, int64_t D, int64_t L, int64_t S, int dtype) {
     return refuse("S must be between 2 and " + std::to_string(DUDY_SHORT_CONV_MAX_TAPS) +
                   ", got " + std::to_string(S) + ".");
   if (!dtype_known(dtype)) return refuse("Unsupported dtype.");
-  if (L >= ((int64_t)1 << 31) || D >= ((int64_t)1 << 31) || B >= ((int64_t)1 << 31) ||
-      B * D >= ((int64_t)1 << 31) || B * D * cdiv(L, kBlockT) / kWarps >= ((int64_t)1 << 31) - 1)
+  if (L >= ((int64_t)1 << 30) || D >= ((int64_t)1 << 31) || B >= ((int64_t)1 << 31) ||
+      B * D >= ((int64_t)1 << 31) || cdiv(B * D, kWarps) * cdiv(L, kSegT) >= ((int64_t)1 << 31))
     return refuse("tensor too large.");
   return DUDY_OK;
 }
@@ -287,28 +325,23 @@ struct BwdArgs {
 };
 
 template <typename T, int S>
-int fwd_launch(const FwdArgs &a, const ConvShape &s, cudaStream_t st) {
-  const int64_t per_row = cdiv(s.L, kBlockT), units = s.B * s.D * per_row;
-  const bool vec = s.L % 8 == 0 && aligned_to_16(a.x) && aligned_to_16(a.out);
-  auto kern = vec ? short_conv_fwd_kernel<T, S, true> : short_conv_fwd_kernel<T, S, false>;
-  kern<<<(unsigned)cdiv(units, kWarps), kWarps * 32, 0, st>>>(
+int fwd_launch(const FwdArgs &a, ConvShape s, cudaStream_t st) {
+  s.vec = s.L % 8 == 0 && aligned_to_16(a.x) && aligned_to_16(a.out);
+  short_conv_fwd_kernel<T, S><<<(unsigned)(cdiv(s.rows, kWarps) * s.segs), kWarps * 32, 0, st>>>(
       (const T *)a.x, (const T *)a.w, (const T *)a.bias, (const T *)a.state, a.lengths,
-      (T *)a.out, (T *)a.final_state, s, per_row, units);
+      (T *)a.out, (T *)a.final_state, s);
   return check_launch("short_conv_fwd_kernel");
 }
 
 template <typename T, int S>
-int bwd_launch(const BwdArgs &a, const ConvShape &s, cudaStream_t st) {
-  const int64_t segs = cdiv(s.L, kSegT), units = s.B * s.D * segs;
-  const bool vec = s.L % 8 == 0 && aligned_to_16(a.x) && aligned_to_16(a.go) &&
-                   aligned_to_16(a.gx);
-  auto kern = vec ? short_conv_bwd_kernel<T, S, true> : short_conv_bwd_kernel<T, S, false>;
-  kern<<<(unsigned)cdiv(units, kWarps), kWarps * 32, 0, st>>>(
+int bwd_launch(const BwdArgs &a, ConvShape s, cudaStream_t st) {
+  s.vec = s.L % 8 == 0 && aligned_to_16(a.x) && aligned_to_16(a.go) && aligned_to_16(a.gx);
+  short_conv_bwd_kernel<T, S><<<(unsigned)(cdiv(s.rows, kWarps) * s.segs), kWarps * 32, 0, st>>>(
       (const T *)a.go, (const T *)a.gfinal, (const T *)a.x, (const T *)a.w, (const T *)a.bias,
-      (const T *)a.state, a.lengths, (T *)a.gx, (T *)a.gstate, a.part, s, segs, units);
+      (const T *)a.state, a.lengths, (T *)a.gx, (T *)a.gstate, a.part, s);
   if (int rc = check_launch("short_conv_bwd_kernel")) return rc;
   short_conv_param_kernel<T><<<(unsigned)cdiv(s.D * (S + 1), kWarps), kWarps * 32, 0, st>>>(
-      a.part, (T *)a.gw, (T *)a.gb, s.D, S, s.B * segs);
+      a.part, (T *)a.gw, (T *)a.gb, s.D, S, s.rows / s.D * s.segs);
   return check_launch("short_conv_param_kernel");
 }
 
@@ -361,7 +394,7 @@ int dudy_short_conv_forward(const void *x, const void *weight, const void *bias,
   if (!x || !weight || !out) return refuse("null tensor pointer");
   if (int rc = require_sm100()) return rc;
   const FwdArgs a{x, weight, bias, state, lengths, out, final_state};
-  const ConvShape s{B, D, L, silu};
+  const ConvShape s{B * D, D, L, (unsigned)cdiv(L, kSegT), silu, 0};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (dtype) {
     case DUDY_DTYPE_F32: return fwd_by_taps<float>(a, s, S, st);
@@ -392,7 +425,7 @@ int dudy_short_conv_backward(const void *go, const void *grad_final, const void 
   if (int rc = require_sm100()) return rc;
   const BwdArgs a{go, grad_final, x, weight, bias, state, lengths, grad_x, grad_weight, grad_bias,
                   grad_state, (float *)workspace};
-  const ConvShape s{B, D, L, silu};
+  const ConvShape s{B * D, D, L, (unsigned)cdiv(L, kSegT), silu, 0};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (dtype) {
     case DUDY_DTYPE_F32: return bwd_by_taps<float>(a, s, S, st);
