@@ -234,39 +234,38 @@ block_norm_bwd_any_kernel(NormBwd a, NormShape s) {
 }
 
 // ---- D <= 1024: the tile in registers ------------------------------------------------------
-// 512 threads hold a tile of 4 TX tokens x all channels, four tokens and up to four channels to
-// a thread, so each tensor moves once. TX = 8 (rows of 64 bytes in 16-bit types) up to D = 256,
-// then 4 and 2. Persistent blocks: a block's next tile is copied into shared memory while it
-// works on this one, each thread's own four-token pieces side by side (no thread reads another's,
-// so its own copies' completion is all it waits for). Arithmetic goes two tokens at a time
-// (__ffma2_rn): with one, the backward issued 91 instructions an element.
-constexpr int kTileThreads = 512;
-constexpr int kV = 4;  // tokens of a thread
+// A block holds a tile of 8 TX tokens x all channels, eight tokens (16 bytes of a 16-bit row) and
+// up to four (backward: two) channels to a thread, so each tensor moves once. TX = 4 (rows of 64
+// bytes) up to D = 256, then 2 and 1. Persistent blocks copy their next tile into shared memory
+// while they work on one, each thread's own pieces side by side (no thread reads another's, so its
+// own copies' completion is all it waits for). Arithmetic goes two tokens at a time (__ffma2_rn). Four tokens to a thread, with
+// twice the addresses and sums a token, took 62 and 107 us at B=16, D=256, L=4096 in fp16.
+constexpr int kFwdThreads = 256, kBwdThreads = 512;
+constexpr int kV = 8;  // tokens of a thread
 
 template <typename T>
-using Four = RowFour<T>;
+using Piece = RowEight<T>;
 using Two = float2[kV / 2];
 
+template <int NT>
 struct TileRed {
-  float part[2][kTileThreads / 32][32];
+  float part[2][NT / 32][32];
   float total[2][32];
 };
 
-// Sums of the four tokens' values over the block's rows of threads, known to all threads of the
-// tokens: across the rows of a warp by shuffles, across the warps by sixteen lanes a token.
-// `turn` alternates between two sets of buffers, so two barriers are enough.
-template <int TX>
-__device__ __forceinline__ void tile_sum4(Two &p, TileRed &m, int &turn) {
-  constexpr int kW = kTileThreads / 32, TOK = TX * kV;
-  const int tid = threadIdx.x, tx = tid % TX;
-  float v[kV] = {p[0].x, p[0].y, p[1].x, p[1].y};
+// Sums of the eight tokens' values over the block's rows of threads, known to all threads of the
+// tokens: across the rows of a warp by shuffles, each lane ending with one token's, and across
+// the warps by as many lanes a token. `turn` alternates between two sets of buffers, so two
+// barriers are enough.
+template <int TX, int NT>
+__device__ __forceinline__ void tile_sum(Two &p, TileRed<NT> &m, int &turn) {
+  constexpr int kW = NT / 32, TOK = TX * kV, LY = 32 / TX, SAME = LY / kV;
+  const int tid = threadIdx.x, tx = tid % TX, ly = (tid & 31) / TX;
+  float v[kV];
 #pragma unroll
-  for (int o = 16; o >= TX; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < kV; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-  if ((tid & 31) < TX)
-    *reinterpret_cast<float4 *>(&m.part[turn][tid >> 5][tx * kV]) =
-        make_float4(v[0], v[1], v[2], v[3]);
+  for (int i = 0; i < kV / 2; ++i) v[2 * i] = p[i].x, v[2 * i + 1] = p[i].y;
+  Scatter<TX, LY, kV>::sum(v, tid & 31);
+  if (ly % SAME == 0) m.part[turn][tid >> 5][tx * kV + ly / SAME] = v[0];
   __syncthreads();
   if (tid < TOK * kW) {
     float s = m.part[turn][tid % kW][tid / kW];
@@ -276,8 +275,11 @@ __device__ __forceinline__ void tile_sum4(Two &p, TileRed &m, int &turn) {
   }
   __syncthreads();
   const float4 t = *reinterpret_cast<const float4 *>(&m.total[turn][tx * kV]);
+  const float4 u = *reinterpret_cast<const float4 *>(&m.total[turn][tx * kV + 4]);
   p[0] = make_float2(t.x, t.y);
   p[1] = make_float2(t.z, t.w);
+  p[2] = make_float2(u.x, u.y);
+  p[3] = make_float2(u.z, u.w);
   turn ^= 1;
 }
 
@@ -298,54 +300,53 @@ __device__ __forceinline__ float2 sigmoid2(float2 v) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store_pairs(T *row, int64_t left, const Two &p, bool vec) {
-  const float v[kV] = {p[0].x, p[0].y, p[1].x, p[1].y};
-  row_store4(row, 0, left, v, vec);
+__device__ __forceinline__ void store_pairs(T *row, int left, const Two &p, bool vec) {
+  float v[kV];
+#pragma unroll
+  for (int i = 0; i < kV / 2; ++i) v[2 * i] = p[i].x, v[2 * i + 1] = p[i].y;
+  row_store8(row, 0, left, v, vec);
 }
 
-template <int BYTES>
-__device__ __forceinline__ void cp_async(void *smem, const void *gmem) {
-  const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(gmem), "n"(BYTES)
-               : "memory");
-}
 template <typename T>
-__device__ __forceinline__ void fetch4(Four<T> &to, const T *from, int64_t left, bool vec) {
-  if (vec) cp_async<sizeof(Four<T>)>(&to, from);
-  else row_load4(to, from, 0, left, false);
+__device__ __forceinline__ void fetch8(Piece<T> &to, const T *from, int left, bool vec) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(Piece<T>) / 16; ++i)
+      cp_async16(reinterpret_cast<char *>(&to) + 16 * i, reinterpret_cast<const char *>(from) + 16 * i);
+  } else {
+    to.load(from, 0, left, false);
+  }
 }
 
 // where a thread's tokens of a tile are
 struct Place {
-  int64_t b, t, left, base;
+  int64_t first, base;  // of the tokens alone, and of channel 0's row
+  int left;
 };
 template <int TX>
 __device__ __forceinline__ Place place(unsigned tile, unsigned tiles, const NormShape &s) {
-  Place p;
-  p.b = tile / tiles;
-  p.t = (int64_t)(tile % tiles) * (TX * kV) + threadIdx.x % TX * kV;
-  p.left = s.L - p.t;
-  p.base = p.b * s.D * s.L + p.t;
-  return p;
+  const unsigned b = tile / tiles;
+  const int t = (int)(tile - b * tiles) * (TX * kV) + threadIdx.x % TX * kV;
+  return Place{b * s.L + t, b * s.D * s.L + t, (int)s.L - t};
 }
 
 template <typename T, typename R, int ROWS>
 struct FwdTile {
-  Four<T> x[ROWS][kTileThreads], z[ROWS][kTileThreads];
-  Four<R> r[ROWS][kTileThreads];
-  static constexpr int kBytes = ROWS * kTileThreads * (2 * sizeof(Four<T>) + sizeof(Four<R>));
-  // two blocks an SM (64 registers) where two tiles of each fit, else one
+  Piece<T> x[ROWS][kFwdThreads], z[ROWS][kFwdThreads];
+  Piece<R> r[ROWS][kFwdThreads];
+  static constexpr int kBytes = ROWS * kFwdThreads * (2 * sizeof(Piece<T>) + sizeof(Piece<R>));
+  // two blocks an SM where two tiles of each fit, else one
   static constexpr int kBlocks = 2 * kBytes <= 104 * 1024 ? 2 : 1;
 };
 
 template <typename T, typename R, int TX, int ROWS, bool LAYER>
-__global__ void __launch_bounds__(kTileThreads, (FwdTile<T, R, ROWS>::kBlocks))
+__global__ void __launch_bounds__(kFwdThreads, (FwdTile<T, R, ROWS>::kBlocks))
 block_norm_fwd_tile_kernel(NormFwd a, NormShape s, unsigned ntiles, bool vec) {
   using Tile = FwdTile<T, R, ROWS>;
-  constexpr int TY = kTileThreads / TX;
+  constexpr int TY = kFwdThreads / TX;
   extern __shared__ __align__(16) char smem_raw[];
   Tile *stage = reinterpret_cast<Tile *>(smem_raw);
-  __shared__ __align__(16) TileRed red;
+  __shared__ __align__(16) TileRed<kFwdThreads> red;
   const int tid = threadIdx.x, ty = tid / TX;
   const unsigned tiles = (unsigned)((s.L + TX * kV - 1) / (TX * kV));
   const float rd = 1.f / (float)s.D;
@@ -372,9 +373,9 @@ block_norm_fwd_tile_kernel(NormFwd a, NormShape s, unsigned ntiles, bool vec) {
         const int d = ty + i * TY;
         if (d >= D) continue;
         const int64_t o = p.base + d * s.L;
-        fetch4(m.x[i][tid], (const T *)a.x + o, p.left, vec);
-        if (a.gate) fetch4(m.z[i][tid], (const T *)a.gate + o, p.left, vec);
-        fetch4(m.r[i][tid], (const R *)a.residual + o, p.left, vec);
+        fetch8(m.x[i][tid], (const T *)a.x + o, p.left, vec);
+        if (a.gate) fetch8(m.z[i][tid], (const T *)a.gate + o, p.left, vec);
+        fetch8(m.r[i][tid], (const R *)a.residual + o, p.left, vec);
       }
     copies_commit();
   };
@@ -411,7 +412,7 @@ block_norm_fwd_tile_kernel(NormFwd a, NormShape s, unsigned ntiles, bool vec) {
     // mean and 1 / sqrt(var + eps) of g; q holds the sum of squares of an rms norm
     auto statistics = [&](Two &mean, Two &inv) {
       if (LAYER) {
-        tile_sum4<TX>(mean, red, turn);
+        tile_sum<TX>(mean, red, turn);
 #pragma unroll
         for (int k = 0; k < kV / 2; ++k) mean[k] = mul2(mean[k], both(rd)), q[k] = both(0.f);
 #pragma unroll
@@ -423,7 +424,7 @@ block_norm_fwd_tile_kernel(NormFwd a, NormShape s, unsigned ntiles, bool vec) {
               q[k] = fma2(c, c, q[k]);
             }
       }
-      tile_sum4<TX>(q, red, turn);
+      tile_sum<TX>(q, red, turn);
 #pragma unroll
       for (int k = 0; k < kV / 2; ++k) {
         inv[k] = make_float2(rsqrtf(fmaf(q[k].x, rd, s.eps)), rsqrtf(fmaf(q[k].y, rd, s.eps)));
@@ -465,7 +466,7 @@ block_norm_fwd_tile_kernel(NormFwd a, NormShape s, unsigned ntiles, bool vec) {
     }
     if (a.stats && ty == 0 && p.left > 0) {
       const int64_t n = s.B * s.L;
-      float *st = a.stats + p.b * s.L + p.t;
+      float *st = a.stats + p.first;
       if (LAYER) store_pairs(st, p.left, m1, vec), store_pairs(st + 2 * n, p.left, m2, vec);
       store_pairs(st + n, p.left, inv1, vec);
       store_pairs(st + 3 * n, p.left, inv2, vec);
@@ -475,28 +476,28 @@ block_norm_fwd_tile_kernel(NormFwd a, NormShape s, unsigned ntiles, bool vec) {
 
 template <typename T, typename R, int ROWS>
 struct BwdTile {
-  Four<T> x[ROWS][kTileThreads], z[ROWS][kTileThreads], gy[ROWS][kTileThreads];
-  Four<R> r[ROWS][kTileThreads], gr[ROWS][kTileThreads];
-  // two tiles where they fit beside TileRed in the 227 KB of a block
-  static constexpr int kBytes = ROWS * kTileThreads * (3 * sizeof(Four<T>) + 2 * sizeof(Four<R>));
-  static constexpr int kStages = 2 * kBytes <= 220 * 1024 ? 2 : 1;
+  Piece<T> x[ROWS][kBwdThreads], z[ROWS][kBwdThreads], gy[ROWS][kBwdThreads];
+  Piece<R> r[ROWS][kBwdThreads], gr[ROWS][kBwdThreads];
+  static constexpr int kBytes = ROWS * kBwdThreads * (3 * sizeof(Piece<T>) + 2 * sizeof(Piece<R>));
+  // two tiles where they fit beside the block's other shared memory
+  static constexpr int kStages = 2 * kBytes <= 216 * 1024 ? 2 : 1;
 };
 
 // The parameter sums stay in registers until a block's last tile.
 template <typename T, typename R, int TX, int ROWS, bool LAYER>
-__global__ void __launch_bounds__(kTileThreads, 1)
+__global__ void __launch_bounds__(kBwdThreads, 1)
 block_norm_bwd_tile_kernel(NormBwd a, NormShape s, unsigned ntiles, bool vec) {
   using Tile = BwdTile<T, R, ROWS>;
-  constexpr int TY = kTileThreads / TX;
+  constexpr int TY = kBwdThreads / TX;
   extern __shared__ __align__(16) char smem_raw[];
   Tile *stage = reinterpret_cast<Tile *>(smem_raw);
-  __shared__ __align__(16) TileRed red;
+  __shared__ __align__(16) TileRed<kBwdThreads> red;
   const int tid = threadIdx.x, ty = tid / TX;
   const unsigned tiles = (unsigned)((s.L + TX * kV - 1) / (TX * kV));
   const int64_t n = s.B * s.L;
   const int D = (int)s.D;
   const float rd = 1.f / (float)s.D;
-  int turn = 0, at = 0;
+  int turn = 0;
 
   float w1[ROWS], b1[ROWS], sc[ROWS], w2[ROWS];
   // sums over tokens: dr hat1, dy hat2, dr, dy
@@ -520,65 +521,60 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, unsigned ntiles, bool vec) {
         const int d = ty + i * TY;
         if (d >= D) continue;
         const int64_t o = p.base + d * s.L;
-        fetch4(m.x[i][tid], (const T *)a.x + o, p.left, vec);
-        if (a.gate) fetch4(m.z[i][tid], (const T *)a.gate + o, p.left, vec);
-        fetch4(m.r[i][tid], (const R *)a.residual + o, p.left, vec);
-        fetch4(m.gy[i][tid], (const T *)a.gy + o, p.left, vec);
-        if (a.grout) fetch4(m.gr[i][tid], (const R *)a.grout + o, p.left, vec);
+        fetch8(m.x[i][tid], (const T *)a.x + o, p.left, vec);
+        if (a.gate) fetch8(m.z[i][tid], (const T *)a.gate + o, p.left, vec);
+        fetch8(m.r[i][tid], (const R *)a.residual + o, p.left, vec);
+        fetch8(m.gy[i][tid], (const T *)a.gy + o, p.left, vec);
+        if (a.grout) fetch8(m.gr[i][tid], (const R *)a.grout + o, p.left, vec);
       }
     copies_commit();
   };
-  Four<float> sn[4];  // the next tile's statistics
-  auto fetch_stats = [&](unsigned tile) {
+  // the tile's statistics, by turns: mean1, inv1, mean2, inv2 of its tokens
+  __shared__ __align__(16) Piece<float> stat[2][4][TX];
+  auto fetch_stats = [&](unsigned tile, int buf) {
+    const int tx = tid % TX, k = tid / TX;
+    if (k >= 4 || (!LAYER && k % 2 == 0)) return;
     const Place p = place<TX>(tile, tiles, s);
-    const float *st = a.stats + p.b * s.L + p.t;
-    if (LAYER) row_load4(sn[0], st, 0, p.left, vec), row_load4(sn[2], st + 2 * n, 0, p.left, vec);
-    row_load4(sn[1], st + n, 0, p.left, vec);
-    row_load4(sn[3], st + 3 * n, 0, p.left, vec);
+    if (p.left > 0) fetch8(stat[buf][k][tx], a.stats + k * n + p.first, p.left, vec);
+    else stat[buf][k][tx].load(a.stats, 0, 0, false);
   };
+  int buf = 0;
   if (blockIdx.x < ntiles) {
+    fetch_stats(blockIdx.x, 0);
     fetch(blockIdx.x, stage[0]);
-    fetch_stats(blockIdx.x);
   }
-  for (unsigned tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
+  for (unsigned tile = blockIdx.x; tile < ntiles; tile += gridDim.x, buf ^= 1) {
     const Place p = place<TX>(tile, tiles, s);
-    Two m1, inv1, m2, inv2, v, u;
-#pragma unroll
-    for (int k = 0; k < kV / 2; ++k) {
-      m1[k] = LAYER ? neg2(sn[0].pair(k)) : both(0.f);
-      inv1[k] = sn[1].pair(k);
-      m2[k] = LAYER ? neg2(sn[2].pair(k)) : both(0.f);
-      inv2[k] = sn[3].pair(k);
-      v[k] = u[k] = both(0.f);
-    }
     const bool more = tile + gridDim.x < ntiles;
+    const Tile &m = stage[Tile::kStages == 2 ? buf : 0];
+    copies_wait<0>();
+    __syncthreads();  // for the statistics: other threads copied them
     if (Tile::kStages == 2 && more) {
-      fetch(tile + gridDim.x, stage[at ^ 1]);
-      copies_wait<1>();
-    } else {
-      copies_wait<0>();
+      fetch_stats(tile + gridDim.x, buf ^ 1);
+      fetch(tile + gridDim.x, stage[buf ^ 1]);
     }
-    if (more) fetch_stats(tile + gridDim.x);
-    const Tile &m = stage[at];
-    float2 hat1[ROWS][kV / 2], hat2[ROWS][kV / 2], sg[ROWS][kV / 2];
+    const Piece<float> &m1 = stat[buf][0][tid % TX], &inv1 = stat[buf][1][tid % TX];
+    const Piece<float> &m2 = stat[buf][2][tid % TX], &inv2 = stat[buf][3][tid % TX];
+    Two v, u;
+#pragma unroll
+    for (int k = 0; k < kV / 2; ++k) v[k] = u[k] = both(0.f);
+    float2 hat1[ROWS][kV / 2], hat2[ROWS][kV / 2];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const bool ok = p.left > 0 && ty + i * TY < D;
 #pragma unroll
       for (int k = 0; k < kV / 2; ++k) {
         float2 g = m.x[i][tid].pair(k), r = m.r[i][tid].pair(k), dy = m.gy[i][tid].pair(k);
-        sg[i][k] = both(0.f);
         if (a.gate) {
           const float2 z = m.z[i][tid].pair(k);
-          sg[i][k] = sigmoid2<T>(z);
-          g = mul2(g, mul2(z, sg[i][k]));
+          g = mul2(g, mul2(z, sigmoid2<T>(z)));
         }
         if (!ok) g = r = dy = both(0.f);
-        float2 h1 = mul2(LAYER ? add2(g, m1[k]) : g, inv1[k]);
+        float2 h1 = mul2(LAYER ? add2(g, neg2(m1.pair(k))) : g, inv1.pair(k));
         if (LAYER && !ok) h1 = both(0.f);
         float2 h2 = fma2(h1, both(sc[i] * w1[i]), r);
-        if (LAYER) h2 = add2(h2, add2(both(sc[i] * b1[i]), m2[k]));
-        h2 = mul2(h2, inv2[k]);
+        if (LAYER) h2 = add2(h2, add2(both(sc[i] * b1[i]), neg2(m2.pair(k))));
+        h2 = mul2(h2, inv2.pair(k));
         if (LAYER && !ok) h2 = both(0.f);
         hat1[i][k] = h1;
         hat2[i][k] = h2;
@@ -591,8 +587,8 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, unsigned ntiles, bool vec) {
         }
       }
     }
-    tile_sum4<TX>(v, red, turn);
-    if (LAYER) tile_sum4<TX>(u, red, turn);
+    tile_sum<TX>(v, red, turn);
+    if (LAYER) tile_sum<TX>(u, red, turn);
     Two c, e;
 #pragma unroll
     for (int k = 0; k < kV / 2; ++k) {
@@ -610,7 +606,7 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, unsigned ntiles, bool vec) {
       for (int k = 0; k < kV / 2; ++k) {
         float2 o = fma2(hat2[i][k], c[k], mul2(m.gy[i][tid].pair(k), both(w2[i])));
         if (LAYER) o = add2(o, e[k]);
-        dr[k] = a.grout ? fma2(inv2[k], o, m.gr[i][tid].pair(k)) : mul2(inv2[k], o);
+        dr[k] = a.grout ? fma2(inv2.pair(k), o, m.gr[i][tid].pair(k)) : mul2(inv2.pair(k), o);
         if (!ok) dr[k] = both(0.f);
         const float2 d1 = mul2(dr[k], both(sc[i] * w1[i]));
         hat2[i][k] = d1;
@@ -623,8 +619,8 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, unsigned ntiles, bool vec) {
       }
       if (ok) store_pairs((R *)a.gresidual + p.base + d * s.L, p.left, dr, vec);
     }
-    tile_sum4<TX>(v, red, turn);
-    if (LAYER) tile_sum4<TX>(u, red, turn);
+    tile_sum<TX>(v, red, turn);
+    if (LAYER) tile_sum<TX>(u, red, turn);
 #pragma unroll
     for (int k = 0; k < kV / 2; ++k) {
       c[k] = mul2(v[k], both(-rd));
@@ -639,19 +635,21 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, unsigned ntiles, bool vec) {
       for (int k = 0; k < kV / 2; ++k) {
         float2 o = fma2(hat1[i][k], c[k], hat2[i][k]);
         if (LAYER) o = add2(o, e[k]);
-        gx[k] = mul2(inv1[k], o);
+        gx[k] = mul2(inv1.pair(k), o);
         if (a.gate) {
-          const float2 z = m.z[i][tid].pair(k), h = mul2(gx[k], sg[i][k]);
+          const float2 z = m.z[i][tid].pair(k), sg = sigmoid2<T>(z), h = mul2(gx[k], sg);
           gx[k] = mul2(h, z);
           gz[k] = mul2(mul2(h, m.x[i][tid].pair(k)),
-                       fma2(z, fma2(sg[i][k], both(-1.f), both(1.f)), both(1.f)));
+                       fma2(z, fma2(sg, both(-1.f), both(1.f)), both(1.f)));
         }
       }
       store_pairs((T *)a.gx + p.base + d * s.L, p.left, gx, vec);
       if (a.gate) store_pairs((T *)a.ggate + p.base + d * s.L, p.left, gz, vec);
     }
-    if (Tile::kStages == 2) at ^= 1;
-    else if (more) fetch(tile + gridDim.x, stage[0]);
+    if (Tile::kStages == 1 && more) {
+      fetch_stats(tile + gridDim.x, buf ^ 1);
+      fetch(tile + gridDim.x, stage[0]);
+    }
   }
   // post_weight: scale sum(dr hat1); pre_weight: sum(dy hat2); scale: sum(dr p) = w1 sum(dr hat1) +
   // b1 sum(dr); post_bias: scale sum(dr); pre_bias: sum(dy)
@@ -715,7 +713,7 @@ int any_tokens(int64_t L) { return L >= 32 ? 32 : (L >= 8 ? 8 : 1); }
 
 int tile_tx(int64_t D, int64_t L) {
   if (D > 1024 || L < 8) return 0;
-  return D <= 256 ? 8 : (D <= 512 ? 4 : 2);
+  return D <= 256 ? 4 : (D <= 512 ? 2 : 1);
 }
 
 // tiles of the kernel that runs, and the number of parts of its parameter sums
@@ -724,38 +722,37 @@ int64_t tile_count(int64_t B, int64_t D, int64_t L) {
   return B * cdiv(L, tx ? tx * kV : any_tokens(L));
 }
 int64_t part_count(int64_t B, int64_t D, int64_t L) {
-  const int64_t n = tile_count(B, D, L), sms = sm_count();
-  return tile_tx(D, L) && n > sms ? sms : n;
+  const int64_t n = tile_count(B, D, L), most = sm_count();
+  return tile_tx(D, L) && n > most ? most : n;
 }
 
-bool aligned_to(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
-
 // calls f with the tile's lanes along tokens and the channels of a thread
-template <typename F>
+template <int NT, typename F>
 int by_tile(int64_t D, F &&f) {
   using std::integral_constant;
-  if (D <= 64) return f(integral_constant<int, 8>(), integral_constant<int, 1>());
-  if (D <= 128) return f(integral_constant<int, 8>(), integral_constant<int, 2>());
-  if (D <= 256) return f(integral_constant<int, 8>(), integral_constant<int, 4>());
-  if (D <= 512) return f(integral_constant<int, 4>(), integral_constant<int, 4>());
-  return f(integral_constant<int, 2>(), integral_constant<int, 4>());
+  constexpr int kMost = 1024 / NT;  // channels of a thread at D = 256, 512, 1024
+  if (D <= NT / 4) return f(integral_constant<int, 4>(), integral_constant<int, 1>());
+  if (kMost == 4 && D <= 128) return f(integral_constant<int, 4>(), integral_constant<int, 2>());
+  if (D <= 256) return f(integral_constant<int, 4>(), integral_constant<int, kMost>());
+  if (D <= 512) return f(integral_constant<int, 2>(), integral_constant<int, kMost>());
+  return f(integral_constant<int, 1>(), integral_constant<int, kMost>());
 }
 
 template <typename T, typename R, bool LAYER>
 int fwd_launch(const NormFwd &a, const NormShape &s, cudaStream_t st) {
   const unsigned grid = (unsigned)tile_count(s.B, s.D, s.L);
   if (tile_tx(s.D, s.L)) {
-    const bool vec = s.L % kV == 0 && aligned_to(a.x, sizeof(Four<T>)) &&
-                     aligned_to(a.gate, sizeof(Four<T>)) && aligned_to(a.y, sizeof(Four<T>)) &&
-                     aligned_to(a.residual, sizeof(Four<R>)) &&
-                     aligned_to(a.rout, sizeof(Four<R>)) && aligned_to_16(a.stats);
-    return by_tile(s.D, [&](auto tx, auto rows) {
+    const bool vec = s.L % kV == 0 && aligned_to_16(a.x) &&
+                     aligned_to_16(a.gate) && aligned_to_16(a.y) &&
+                     aligned_to_16(a.residual) &&
+                     aligned_to_16(a.rout) && aligned_to_16(a.stats);
+    return by_tile<kFwdThreads>(s.D, [&](auto tx, auto rows) {
       using Tile = FwdTile<T, R, decltype(rows)::value>;
       const int smem = 2 * (int)sizeof(Tile), most = Tile::kBlocks * sm_count();
       auto kern = block_norm_fwd_tile_kernel<T, R, decltype(tx)::value, decltype(rows)::value, LAYER>;
       if (set_smem_once((const void *)kern, smem) != cudaSuccess)
         return check_launch("block_norm_fwd_tile_kernel shared memory");
-      kern<<<grid < (unsigned)most ? grid : most, kTileThreads, smem, st>>>(a, s, grid, vec);
+      kern<<<grid < (unsigned)most ? grid : most, kFwdThreads, smem, st>>>(a, s, grid, vec);
       return check_launch("block_norm_fwd_tile_kernel");
     });
   }
@@ -774,22 +771,22 @@ struct ParamGrads {
 template <typename T, typename R, bool LAYER>
 int bwd_main(const NormBwd &a, const NormShape &s, cudaStream_t st) {
   if (tile_tx(s.D, s.L)) {
-    const bool vec = s.L % kV == 0 && aligned_to(a.x, sizeof(Four<T>)) &&
-                     aligned_to(a.gate, sizeof(Four<T>)) && aligned_to(a.ggate, sizeof(Four<T>)) &&
-                     aligned_to(a.gy, sizeof(Four<T>)) && aligned_to(a.gx, sizeof(Four<T>)) &&
-                     aligned_to(a.residual, sizeof(Four<R>)) &&
-                     aligned_to(a.grout, sizeof(Four<R>)) &&
-                     aligned_to(a.gresidual, sizeof(Four<R>)) && aligned_to_16(a.stats);
+    const bool vec = s.L % kV == 0 && aligned_to_16(a.x) &&
+                     aligned_to_16(a.gate) && aligned_to_16(a.ggate) &&
+                     aligned_to_16(a.gy) && aligned_to_16(a.gx) &&
+                     aligned_to_16(a.residual) &&
+                     aligned_to_16(a.grout) &&
+                     aligned_to_16(a.gresidual) && aligned_to_16(a.stats);
     const unsigned grid = (unsigned)part_count(s.B, s.D, s.L);
     const int64_t tiles = tile_count(s.B, s.D, s.L);
-    return by_tile(s.D, [&](auto tx, auto rows) {
+    return by_tile<kBwdThreads>(s.D, [&](auto tx, auto rows) {
       constexpr int ROWS = decltype(rows)::value;
       using Tile = BwdTile<T, R, ROWS>;
       const int smem = Tile::kStages * (int)sizeof(Tile);
       auto kern = block_norm_bwd_tile_kernel<T, R, decltype(tx)::value, ROWS, LAYER>;
       if (set_smem_once((const void *)kern, smem) != cudaSuccess)
         return check_launch("block_norm_bwd_tile_kernel shared memory");
-      kern<<<grid, kTileThreads, smem, st>>>(a, s, (unsigned)tiles, vec);
+      kern<<<grid, kBwdThreads, smem, st>>>(a, s, (unsigned)tiles, vec);
       return check_launch("block_norm_bwd_tile_kernel");
     });
   }

@@ -26,6 +26,37 @@ __device__ __forceinline__ uint32_t word_of(float2 v, __nv_bfloat16) {
 }
 
 // ---- eight positions of a row ------------------------------------------------------------
+// 2 N 16-bit elements from an address that need not be that of a word (rows of odd length): words
+// where it is, else the words between and an element at each end.
+template <int N>
+__device__ __forceinline__ void load_halves(uint32_t *w, const uint16_t *h) {
+  if ((reinterpret_cast<uintptr_t>(h) & 2u) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t *>(h)[i];
+  } else {
+    uint32_t m[N + 1];
+    m[0] = (uint32_t)h[0] << 16;
+#pragma unroll
+    for (int i = 1; i < N; ++i) m[i] = reinterpret_cast<const uint32_t *>(h - 1)[i];
+    m[N] = h[2 * N - 1];
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = __funnelshift_r(m[i], m[i + 1], 16);
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_halves(uint16_t *h, const uint32_t *w) {
+  if ((reinterpret_cast<uintptr_t>(h) & 2u) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) reinterpret_cast<uint32_t *>(h)[i] = w[i];
+  } else {
+    h[0] = (uint16_t)w[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i)
+      reinterpret_cast<uint32_t *>(h - 1)[i] = __funnelshift_r(w[i - 1], w[i], 16);
+    h[2 * N - 1] = (uint16_t)(w[N - 1] >> 16);
+  }
+}
+
 // Kept in whole 32-bit words from the load on, also where the elements are loaded one by one: the
 // conversion waits until it is asked for, so loads that come early stay in flight.
 template <typename T>
@@ -44,6 +75,8 @@ struct RowEight {
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = t + i < end ? reinterpret_cast<const uint32_t *>(row)[t + i] : 0u;
+    } else if (t + 8 <= end) {
+      load_halves<4>(w, reinterpret_cast<const uint16_t *>(row + t));
     } else {
       const uint16_t *h = reinterpret_cast<const uint16_t *>(row);
 #pragma unroll
@@ -52,12 +85,16 @@ struct RowEight {
                (t + 2 * i + 1 < end ? (uint32_t)h[t + 2 * i + 1] << 16 : 0u);
     }
   }
+  __device__ __forceinline__ float2 pair(int i) const {
+    if constexpr (sizeof(T) == 4)
+      return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else
+      return pair_of(w[i], T());
+  }
   __device__ __forceinline__ void get(float (&v)[8]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float2 p;
-      if constexpr (sizeof(T) == 4) p = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
-      else p = pair_of(w[i], T());
+      const float2 p = pair(i);
       v[2 * i] = p.x;
       v[2 * i + 1] = p.y;
     }
@@ -75,6 +112,13 @@ __device__ __forceinline__ void row_store8(T *row, int t, int end, const float (
       *reinterpret_cast<uint4 *>(row + t) =
           make_uint4(word_of(make_float2(v[0], v[1]), T()), word_of(make_float2(v[2], v[3]), T()),
                      word_of(make_float2(v[4], v[5]), T()), word_of(make_float2(v[6], v[7]), T()));
+    }
+  } else if (sizeof(T) == 2 && t + 8 <= end) {
+    if constexpr (sizeof(T) == 2) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = word_of(make_float2(v[2 * i], v[2 * i + 1]), T());
+      store_halves<4>(reinterpret_cast<uint16_t *>(row + t), w);
     }
   } else {
 #pragma unroll
@@ -196,6 +240,41 @@ template <>
 __device__ __forceinline__ float sigmoid_for<float>(float v) {
   return 1.f / (1.f + expf(-v));
 }
+
+// ---- sums across lanes ------------------------------------------------------------------------
+// Sums of n values each over the lanes that differ in the bits [STRIDE, STRIDE * LANES) of the
+// lane number. While there are several values, half of them go to the partner lane and half
+// come from it, so a stage costs n / 2 shuffles; afterwards lane l of the group (its number in
+// those bits) holds the sums of values l * n / LANES .. , or, with more lanes than n / KEEP
+// values, all lanes that agree in the upper bits hold the same KEEP values.
+template <int STRIDE, int LANES, int N, int KEEP = 1>
+struct Scatter {
+  static constexpr int kLeft = LANES == 1 || N == KEEP ? N : Scatter<STRIDE, LANES / 2, N / 2, KEEP>::kLeft;
+  static __device__ __forceinline__ void sum(float *v, int lane) {
+    if constexpr (LANES > 1) {
+      constexpr int o = STRIDE * LANES / 2;
+      if constexpr (N > KEEP) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          const float send = up ? v[i] : v[i + N / 2];
+          const float keep = up ? v[i + N / 2] : v[i];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+        Scatter<STRIDE, LANES / 2, N / 2, KEEP>::sum(v, lane);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+        Scatter<STRIDE, LANES / 2, N, KEEP>::sum(v, lane);
+      }
+    }
+  }
+};
+template <int STRIDE, int N, int KEEP>
+struct Scatter<STRIDE, 1, N, KEEP> {
+  static constexpr int kLeft = N;
+  static __device__ __forceinline__ void sum(float *, int) {}
+};
 
 // ---- asynchronous 16-byte copies into shared memory ------------------------------------------
 __device__ __forceinline__ void cp_async16(void *smem, const void *gmem) {

@@ -109,40 +109,6 @@ __device__ __forceinline__ float4 quad(const float2 &a, const float2 &b) {
   return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// Sums of n values each over the lanes that differ in the bits [STRIDE, STRIDE * LANES) of the
-// lane number. While there are several values, half of them go to the partner lane and half
-// come from it, so a stage costs n / 2 shuffles; afterwards lane l of the group (its number in
-// those bits) holds the sums of values l * n / LANES .. , or, with more lanes than n / KEEP
-// values, all lanes that agree in the upper bits hold the same KEEP values.
-template <int STRIDE, int LANES, int N, int KEEP = 1>
-struct Scatter {
-  static constexpr int kLeft = LANES == 1 || N == KEEP ? N : Scatter<STRIDE, LANES / 2, N / 2, KEEP>::kLeft;
-  static __device__ __forceinline__ void sum(float *v, int lane) {
-    if constexpr (LANES > 1) {
-      constexpr int o = STRIDE * LANES / 2;
-      if constexpr (N > KEEP) {
-        const bool up = lane & o;
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-          const float send = up ? v[i] : v[i + N / 2];
-          const float keep = up ? v[i + N / 2] : v[i];
-          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-        }
-        Scatter<STRIDE, LANES / 2, N / 2, KEEP>::sum(v, lane);
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-        Scatter<STRIDE, LANES / 2, N, KEEP>::sum(v, lane);
-      }
-    }
-  }
-};
-template <int STRIDE, int N, int KEEP>
-struct Scatter<STRIDE, 1, N, KEEP> {
-  static constexpr int kLeft = N;
-  static __device__ __forceinline__ void sum(float *, int) {}
-};
-
 // Input rows come in by stretches of one piece for each warp, copied by all the block's threads
 // into one of three buffers (rows of whole 16-byte pieces: a warp's own piece of a row is 8 to
 // 16 bytes, and copying it alone cost the load pipe eight times as many accesses). A warp that
