@@ -20,10 +20,8 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import load_extension
-from .state_space import _contig, _wants_grad
 
 _EXT = load_extension()
 
@@ -34,29 +32,6 @@ def _layer(norm: str) -> bool:
     if norm not in _NORMS:
         raise RuntimeError(f"norm must be 'rms' or 'layer', got {norm!r}.")
     return _NORMS[norm]
-
-
-class FusedGatedResidualNormFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias,
-                layer: bool, eps: float):
-        args = tuple(_contig(t) for t in (x, residual, gate, post_weight, post_bias, scale,
-                                          pre_weight, pre_bias))
-        y, rout, stats = _EXT.block_norm_forward(*args, layer, eps, True)
-        ctx.save_for_backward(*args, stats)
-        ctx.layer = layer
-        ctx.set_materialize_grads(False)
-        return y, rout
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_y, grad_residual):
-        *args, stats = ctx.saved_tensors
-        if grad_y is None and grad_residual is None:
-            return (None,) * 10
-        grad_y = torch.zeros_like(args[0]) if grad_y is None else grad_y.contiguous()
-        grads = _EXT.block_norm_backward(grad_y, _contig(grad_residual), *args, stats, ctx.layer)
-        return (*grads, None, None)
 
 
 def fused_gated_residual_norm(x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor,
@@ -73,10 +48,8 @@ def fused_gated_residual_norm(x: torch.Tensor, residual: torch.Tensor, post_weig
         raise RuntimeError("an rms norm has no bias.")
     if not eps > 0:
         raise RuntimeError(f"eps must be positive, got {eps}.")
-    args = (x, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias)
-    if _wants_grad(*args):
-        return FusedGatedResidualNormFunction.apply(*args, layer, float(eps))
-    y, rout, _ = _EXT.block_norm_forward(*(_contig(t) for t in args), layer, float(eps), False)
+    y, rout = _EXT.block_norm(x, residual, gate, post_weight, post_bias, scale, pre_weight,
+                              pre_bias, layer, float(eps))
     return y, rout
 
 

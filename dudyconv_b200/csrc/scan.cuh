@@ -85,7 +85,11 @@ __device__ __forceinline__ float decay<float>(float x) {
 // 1 + e would not). fp32 tensors: the accurate functions.
 template <typename T>
 __device__ __forceinline__ float softplus(float x, float &slope) {
-  const float e = ex2(-1.4426950408889634f * fabsf(x));
+  // exp(-|x|) with the exponent's rounding put back (at |x| = 5 it is 3e-7); beyond 100 it is
+  // zero, also for infinities and the types' lowest values, and NaN stays NaN
+  const float ax = fabsf(x) > 100.f ? 100.f : fabsf(x), t = -1.4426950408889634f * ax;
+  float e = ex2(t);
+  e = fmaf(e, 0.6931471805599453f * fmaf(-1.4426950408889634f, ax, -t), e);
   const float s = e * rcp(2.f + e), q = s * s;
   float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
   p = fmaf(p, q, 1.f / 9.f);

@@ -12,12 +12,11 @@
 // Both directions are bound by HBM: the forward reads and writes each row once, the backward
 // reads two rows and writes one. A warp takes up to 1024 positions of a row, 256 at a time, eight
 // to a lane (16-byte accesses); the S-1 <= 7 inputs before a lane's own come from the lane before
-// it by shuffles, so no row is read twice. The forward has all of a segment's loads in flight at
-// once; the backward loads the next block before it works on one. It walks its positions from the
-// right, because dx needs the S-1 values of dv behind it: those come from the next lane, and at
-// the right end of a block from the block done just before. Parameter gradients are summed in
-// registers over the segment, once across the warp, and by a second kernel over batch and
-// segments in a fixed order.
+// it by shuffles, so no row is read twice, and all of a segment's loads are in flight at once.
+// The backward walks its positions from the right, because dx needs the S-1 values of dv behind
+// it: those come from the next lane, and at the right end of a block from the block done just
+// before. Parameter gradients are summed in registers over the segment, once across the warp, and
+// by a second kernel over batch and segments in a fixed order.
 #include "rowvec.cuh"
 
 namespace dudy {
@@ -46,25 +45,28 @@ __device__ __forceinline__ float before(const T *state_row, int t) {
   return state_row && t >= -(S - 1) ? ldf(state_row + (S - 1) + t) : 0.f;
 }
 
-// The lane's window xw[0 .. S-2] = xe[t-(S-1) .. t-1], xw[S-1 ..] = xe[t .. t+7] from its own
-// eight, zero at and after `len`. `t0` is the warp's first position.
+// The S-1 inputs before position `t0`, in lane 31 (where the lane before lane 0 would be)
 template <typename T, int S>
-__device__ __forceinline__ void window(const RowEight<T> &x, const T *row, const T *state_row,
-                                       int t0, int len, int lane, float (&xw)[8 + S - 1]) {
-  float v[8];
-  x.get(v);
+__device__ __forceinline__ void inputs_before(const T *row, const T *state_row, int t0, int len,
+                                              int lane, float (&v)[S - 1]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) xw[S - 1 + i] = v[i];
+  for (int i = 0; i < S - 1; ++i) {
+    const int p = t0 - (S - 1) + i;
+    v[i] = 0.f;
+    if (lane == 31) v[i] = p < 0 ? before<T, S>(state_row, p) : (p < len ? ldf(row + p) : 0.f);
+  }
+}
+
+// The lane's window xw[0 .. S-2] = xe[t-(S-1) .. t-1], xw[S-1 ..] = xe[t .. t+7] from its own eight
+// and, by a shuffle, the lane before; lane 0's come from lane 31's `left`.
+template <int S>
+__device__ __forceinline__ void window(const float (&x)[8], const float (&left)[S - 1], int lane,
+                                       float (&xw)[8 + S - 1]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) xw[S - 1 + i] = x[i];
 #pragma unroll
   for (int i = 0; i < S - 1; ++i)
-    xw[i] = __shfl_up_sync(0xffffffffu, v[8 - (S - 1) + i], 1);
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < S - 1; ++i) {
-      const int p = t0 - (S - 1) + i;
-      xw[i] = p < 0 ? before<T, S>(state_row, p) : (p < len ? ldf(row + p) : 0.f);
-    }
-  }
+    xw[i] = __shfl_sync(0xffffffffu, lane == 31 ? left[i] : x[8 - (S - 1) + i], lane + 31);
 }
 
 // the row and segment of a warp; false: none
@@ -98,18 +100,26 @@ short_conv_fwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const T 
 #pragma unroll
   for (int j = 0; j < S; ++j) wt[j] = ldf(w + d * S + j);
   const float bv = bias ? ldf(bias + d) : 0.f;
+  float left[S - 1];
+  inputs_before<T, S>(xr, sr, lo, len, lane, left);
 #pragma unroll
   for (int k = 0; k < kSegBlocks; ++k) {
     const int t0 = lo + k * kBlockT, t = t0 + lane * 8;
     if (t0 >= hi) break;
-    float xw[8 + S - 1], o[8];
-    window<T, S>(xs[k], xr, sr, t0, len, lane, xw);
+    float xv[8], xw[8 + S - 1], o[8];
+    xs[k].get(xv);
+    window<S>(xv, left, lane, xw);
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) left[i] = xv[8 - (S - 1) + i];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float v = bv;
+      o[i] = bv;
 #pragma unroll
-      for (int j = 0; j < S; ++j) v = fmaf(wt[j], xw[i + j], v);
-      o[i] = s.silu ? v * sigmoid_for<T>(v) : v;
+      for (int j = 0; j < S; ++j) o[i] = fmaf(wt[j], xw[i + j], o[i]);
+    }
+    if (s.silu) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] *= sigmoid_for<T>(o[i]);
     }
     if (t + 8 > len) {
 #pragma unroll
@@ -149,10 +159,13 @@ short_conv_bwd_kernel(const T *__restrict__ go, const T *__restrict__ gfinal,
   T *gxr = gx + row * s.L;
   const T *sr = state ? state + row * (S - 1) : nullptr;
   const T *fr = gfinal ? gfinal + row * (S - 1) : nullptr;
-  const int last = lo + (hi - lo - 1) / kBlockT * kBlockT;
-  RowEight<T> xn, gn;  // the next block
-  xn.load(xr, last + lane * 8, len, s.vec);
-  gn.load(gr, last + lane * 8, len, s.vec);
+  RowEight<T> xs[kSegBlocks], gs[kSegBlocks];
+#pragma unroll
+  for (int k = kSegBlocks - 1; k >= 0; --k)
+    if (lo + k * kBlockT < hi) {
+      xs[k].load(xr, lo + k * kBlockT + lane * 8, len, s.vec);
+      gs[k].load(gr, lo + k * kBlockT + lane * 8, len, s.vec);
+    }
   float wt[S];
 #pragma unroll
   for (int j = 0; j < S; ++j) wt[j] = ldf(w + d * S + j);
@@ -161,6 +174,8 @@ short_conv_bwd_kernel(const T *__restrict__ go, const T *__restrict__ gfinal,
 #pragma unroll
   for (int j = 0; j < S; ++j) dw[j] = 0.f;
 
+  float first[S - 1];
+  inputs_before<T, S>(xr, sr, lo, len, lane, first);
   // dv at the S-1 positions behind the segment: lane i takes position hi + i
   float behind[S];
   {
@@ -178,22 +193,37 @@ short_conv_bwd_kernel(const T *__restrict__ go, const T *__restrict__ gfinal,
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) behind[i] = __shfl_sync(0xffffffffu, mine, i);
   }
-  for (int t0 = last; t0 >= lo; t0 -= kBlockT) {
-    const int t = t0 + lane * 8;
-    const RowEight<T> xc = xn, gc = gn;
-    if (t0 > lo) {
-      xn.load(xr, t - kBlockT, len, s.vec);
-      gn.load(gr, t - kBlockT, len, s.vec);
+#pragma unroll
+  for (int b4 = kSegBlocks - 1; b4 >= 0; --b4) {
+    const int t0 = lo + b4 * kBlockT, t = t0 + lane * 8;
+    if (t0 >= hi) continue;
+    float xv[8], xw[8 + S - 1], left[S - 1], dv[8 + S - 1];
+    xs[b4].get(xv);
+    if (b4 > 0) {
+      float next[8];
+      xs[b4 > 0 ? b4 - 1 : 0].get(next);
+#pragma unroll
+      for (int i = 0; i < S - 1; ++i) left[i] = next[8 - (S - 1) + i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < S - 1; ++i) left[i] = first[i];
     }
-    float xw[8 + S - 1], g[8], dv[8 + S - 1];
-    window<T, S>(xc, xr, sr, t0, len, lane, xw);
-    gc.get(g);
+    window<S>(xv, left, lane, xw);
+    {
+      float g[8];
+      gs[b4].get(g);
+      if (s.silu) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float v = bv;
+        for (int i = 0; i < 8; ++i) {
+          float v = bv;
 #pragma unroll
-      for (int j = 0; j < S; ++j) v = fmaf(wt[j], xw[i + j], v);
-      dv[i] = dv_of<T>(v, g[i], s.silu);
+          for (int j = 0; j < S; ++j) v = fmaf(wt[j], xw[i + j], v);
+          dv[i] = dv_of<T>(v, g[i], 1);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dv[i] = g[i];
+      }
     }
     if (t + 8 > len) {
 #pragma unroll

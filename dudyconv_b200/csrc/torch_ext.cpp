@@ -548,6 +548,26 @@ using OptTensor = c10::optional<torch::Tensor>;
 
 const void *opt_ptr(const OptTensor &t) { return t.has_value() ? t->data_ptr() : nullptr; }
 
+OptTensor contig(const OptTensor &t) {
+  return t.has_value() ? OptTensor(t->contiguous()) : t;
+}
+
+template <typename... Ts>
+bool wants_grad(const Ts &...ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  auto one = [](const OptTensor &t) { return t.has_value() && t->requires_grad(); };
+  return (one(ts) || ...);
+}
+
+// autograd's saved tensors: what was None comes back undefined
+torch::Tensor or_undefined(const OptTensor &t) { return t.has_value() ? *t : torch::Tensor(); }
+OptTensor or_none(const torch::Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+// in a backward that is itself being recorded
+void refuse_twice(const char *what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, " cannot be differentiated twice.");
+}
+
 // A [..] tensor of `like`'s device and of type `dt`, with the given sizes
 void check_like(const torch::Tensor &t, const char *name, at::IntArrayRef sizes,
                 at::ScalarType dt, const torch::Tensor &like) {
@@ -634,8 +654,60 @@ std::vector<torch::Tensor> short_conv_backward(torch::Tensor go, OptTensor gfina
   return {gx, gw, gb, gs};
 }
 
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct ShortConvFn : public torch::autograd::Function<ShortConvFn> {
+  static variable_list forward(AutogradContext *ctx, torch::Tensor x, torch::Tensor w,
+                               OptTensor bias, OptTensor state, OptTensor lengths, bool silu,
+                               bool want_final) {
+    x = x.contiguous();
+    w = w.contiguous();
+    bias = contig(bias);
+    state = contig(state);
+    lengths = contig(lengths);
+    auto out = short_conv_forward(x, w, bias, state, lengths, silu, want_final);
+    ctx->save_for_backward(
+        {x, w, or_undefined(bias), or_undefined(state), or_undefined(lengths)});
+    ctx->saved_data["silu"] = silu;
+    ctx->saved_data["want_state"] = state.has_value() && state->requires_grad();
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list g) {
+    refuse_twice("fused_short_conv");
+    const auto v = ctx->get_saved_variables();
+    variable_list none(7);
+    const bool final_grad = g.size() > 1 && g[1].defined();
+    if (!g[0].defined() && !final_grad) return none;
+    auto go = g[0].defined() ? g[0].contiguous() : torch::zeros_like(v[0]);
+    auto r = short_conv_backward(go, final_grad ? OptTensor(g[1].contiguous()) : OptTensor(), v[0],
+                                 v[1], or_none(v[2]), or_none(v[3]), or_none(v[4]),
+                                 ctx->saved_data["silu"].toBool(),
+                                 ctx->saved_data["want_state"].toBool());
+    for (int i = 0; i < 4; ++i)
+      if (i < 2 || r[i].numel() > 0) none[i] = r[i];
+    return none;
+  }
+};
+
+// out and, where wanted, the final state; recorded for the backward where an input asks for it
+std::vector<torch::Tensor> short_conv(torch::Tensor x, torch::Tensor w, OptTensor bias,
+                                      OptTensor state, OptTensor lengths, bool silu,
+                                      bool want_final) {
+  if (wants_grad(x, w, bias, state))
+    return ShortConvFn::apply(x, w, bias, state, lengths, silu, want_final);
+  return short_conv_forward(x.contiguous(), w.contiguous(), contig(bias), contig(state),
+                            contig(lengths), silu, want_final);
+}
+
 torch::Tensor short_conv_step(torch::Tensor x, torch::Tensor state, torch::Tensor w,
                               OptTensor bias, bool silu) {
+  TORCH_CHECK(!wants_grad(x, state, w, bias),
+              "fused_short_conv_step has no backward: call it under torch.no_grad().");
+  x = x.contiguous();
+  w = w.contiguous();
+  bias = contig(bias);
   TORCH_CHECK(x.is_cuda(), "x must be CUDA tensor.");
   TORCH_CHECK(x.dim() == 2 && x.numel() > 0, "x must be [B,D], got ", x.sizes(), ".");
   TORCH_CHECK(x.is_contiguous(), "x must be contiguous.");
@@ -758,9 +830,82 @@ std::vector<torch::Tensor> selective_scan_backward(torch::Tensor go, OptTensor g
   return {gu, gd, gA, gB, gC, gs, gb, gst};
 }
 
+// [B,N,L] (or [B,N] of one token) is one group
+torch::Tensor grouped(const torch::Tensor &t, int64_t dims) {
+  return (t.dim() == dims - 1 ? t.unsqueeze(1) : t).contiguous();
+}
+
+struct SelectiveScanFn : public torch::autograd::Function<SelectiveScanFn> {
+  static variable_list forward(AutogradContext *ctx, torch::Tensor u, torch::Tensor delta,
+                               torch::Tensor A, torch::Tensor Bm, torch::Tensor Cm,
+                               OptTensor skip, OptTensor bias, OptTensor state,
+                               OptTensor lengths, bool softplus, bool want_final) {
+    const auto bshape = Bm.sizes().vec(), cshape = Cm.sizes().vec();
+    u = u.contiguous();
+    delta = delta.contiguous();
+    A = A.contiguous();
+    Bm = grouped(Bm, 4);
+    Cm = grouped(Cm, 4);
+    skip = contig(skip);
+    bias = contig(bias);
+    state = contig(state);
+    lengths = contig(lengths);
+    auto r = selective_scan_forward(u, delta, A, Bm, Cm, skip, bias, state, lengths, softplus,
+                                    want_final, true);
+    ctx->save_for_backward({u, delta, A, Bm, Cm, or_undefined(skip), or_undefined(bias), r[2],
+                            or_undefined(lengths)});
+    ctx->saved_data["softplus"] = softplus;
+    ctx->saved_data["want_state"] = state.has_value() && state->requires_grad();
+    ctx->saved_data["bshape"] = bshape;
+    ctx->saved_data["cshape"] = cshape;
+    ctx->set_materialize_grads(false);
+    return want_final ? variable_list{r[0], r[1]} : variable_list{r[0]};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list g) {
+    refuse_twice("fused_selective_scan");
+    const auto v = ctx->get_saved_variables();
+    variable_list out(11);
+    const bool final_grad = g.size() > 1 && g[1].defined();
+    if (!g[0].defined() && !final_grad) return out;
+    auto go = g[0].defined() ? g[0].contiguous() : torch::zeros_like(v[0]);
+    auto r = selective_scan_backward(
+        go, final_grad ? OptTensor(g[1].contiguous()) : OptTensor(), v[0], v[1], v[2], v[3], v[4],
+        or_none(v[5]), or_none(v[6]), v[7], or_none(v[8]), ctx->saved_data["softplus"].toBool(),
+        ctx->saved_data["want_state"].toBool());
+    for (size_t i = 0; i < r.size(); ++i) out[i] = r[i];
+    out[3] = out[3].view(ctx->saved_data["bshape"].toIntVector());
+    out[4] = out[4].view(ctx->saved_data["cshape"].toIntVector());
+    return out;
+  }
+};
+
+// y and, where wanted, the final state
+std::vector<torch::Tensor> selective_scan(torch::Tensor u, torch::Tensor delta, torch::Tensor A,
+                                          torch::Tensor Bm, torch::Tensor Cm, OptTensor skip,
+                                          OptTensor bias, OptTensor state, OptTensor lengths,
+                                          bool softplus, bool want_final) {
+  if (wants_grad(u, delta, A, Bm, Cm, skip, bias, state))
+    return SelectiveScanFn::apply(u, delta, A, Bm, Cm, skip, bias, state, lengths, softplus,
+                                  want_final);
+  auto r = selective_scan_forward(u.contiguous(), delta.contiguous(), A.contiguous(),
+                                  grouped(Bm, 4), grouped(Cm, 4), contig(skip), contig(bias),
+                                  contig(state), contig(lengths), softplus, want_final, false);
+  r.resize(want_final ? 2 : 1);
+  return r;
+}
+
 torch::Tensor selective_scan_step(torch::Tensor u, torch::Tensor delta, torch::Tensor A,
                                   torch::Tensor Bm, torch::Tensor Cm, torch::Tensor state,
                                   OptTensor skip, OptTensor bias, bool softplus) {
+  TORCH_CHECK(!wants_grad(u, delta, A, Bm, Cm, state, skip, bias),
+              "fused_selective_scan_step has no backward: call it under torch.no_grad().");
+  u = u.contiguous();
+  delta = delta.contiguous();
+  A = A.contiguous();
+  Bm = grouped(Bm, 3);
+  Cm = grouped(Cm, 3);
+  skip = contig(skip);
+  bias = contig(bias);
   const ScanDims d = check_scan(u, delta, A, Bm, Cm, skip, bias, true);
   check_like(state, "state", {d.B, d.D, d.N}, at::kFloat, u);
   const c10::cuda::CUDAGuard guard(u.device());
@@ -842,6 +987,52 @@ std::vector<torch::Tensor> block_norm_backward(torch::Tensor gy, OptTensor grout
   return {gx, gr, gg, gw1, gb1, gsc, gw2, gb2};
 }
 
+struct BlockNormFn : public torch::autograd::Function<BlockNormFn> {
+  static variable_list forward(AutogradContext *ctx, torch::Tensor x, torch::Tensor residual,
+                               OptTensor gate, torch::Tensor w1, OptTensor b1, OptTensor scale,
+                               torch::Tensor w2, OptTensor b2, bool layer, double eps) {
+    x = x.contiguous();
+    residual = residual.contiguous();
+    gate = contig(gate);
+    w1 = w1.contiguous();
+    b1 = contig(b1);
+    scale = contig(scale);
+    w2 = w2.contiguous();
+    b2 = contig(b2);
+    auto r = block_norm_forward(x, residual, gate, w1, b1, scale, w2, b2, layer, eps, true);
+    ctx->save_for_backward({x, residual, or_undefined(gate), w1, or_undefined(b1),
+                            or_undefined(scale), w2, or_undefined(b2), r[2]});
+    ctx->saved_data["layer"] = layer;
+    ctx->set_materialize_grads(false);
+    return {r[0], r[1]};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list g) {
+    refuse_twice("fused_gated_residual_norm");
+    const auto v = ctx->get_saved_variables();
+    variable_list out(10);
+    if (!g[0].defined() && !g[1].defined()) return out;
+    auto gy = g[0].defined() ? g[0].contiguous() : torch::zeros_like(v[0]);
+    auto r = block_norm_backward(gy, g[1].defined() ? OptTensor(g[1].contiguous()) : OptTensor(),
+                                 v[0], v[1], or_none(v[2]), v[3], or_none(v[4]), or_none(v[5]),
+                                 v[6], or_none(v[7]), v[8], ctx->saved_data["layer"].toBool());
+    for (size_t i = 0; i < r.size(); ++i) out[i] = r[i];
+    return out;
+  }
+};
+
+// y, residual_out
+std::vector<torch::Tensor> block_norm(torch::Tensor x, torch::Tensor residual, OptTensor gate,
+                                      torch::Tensor w1, OptTensor b1, OptTensor scale,
+                                      torch::Tensor w2, OptTensor b2, bool layer, double eps) {
+  if (wants_grad(x, residual, gate, w1, b1, scale, w2, b2))
+    return BlockNormFn::apply(x, residual, gate, w1, b1, scale, w2, b2, layer, eps);
+  auto r = block_norm_forward(x.contiguous(), residual.contiguous(), contig(gate),
+                              w1.contiguous(), contig(b1), contig(scale), w2.contiguous(),
+                              contig(b2), layer, eps, false);
+  r.resize(2);
+  return r;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -877,33 +1068,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("logits_to_kernel_backward", &logits_to_kernel_backward,
         "Backward of logits_to_kernel from its output kc and grad_kc", py::arg("kc"),
         py::arg("grad_kc"));
-  m.def("short_conv_forward", &short_conv_forward, "Short causal depthwise conv forward",
-        py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("state"), py::arg("lengths"),
-        py::arg("silu"), py::arg("want_final"));
-  m.def("short_conv_backward", &short_conv_backward, "Short causal depthwise conv backward",
-        py::arg("go"), py::arg("grad_final"), py::arg("x"), py::arg("weight"), py::arg("bias"),
-        py::arg("state"), py::arg("lengths"), py::arg("silu"), py::arg("want_state"));
+  m.def("short_conv", &short_conv, "Short causal depthwise conv", py::arg("x"),
+        py::arg("weight"), py::arg("bias"), py::arg("state"), py::arg("lengths"), py::arg("silu"),
+        py::arg("want_final"));
   m.def("short_conv_step", &short_conv_step, "Short causal depthwise conv, one token",
         py::arg("x"), py::arg("state"), py::arg("weight"), py::arg("bias"), py::arg("silu"));
-  m.def("selective_scan_forward", &selective_scan_forward, "Selective scan forward",
-        py::arg("u"), py::arg("delta"), py::arg("A"), py::arg("B"), py::arg("C"),
-        py::arg("skip"), py::arg("delta_bias"), py::arg("state"), py::arg("lengths"),
-        py::arg("softplus"), py::arg("want_final"), py::arg("want_checkpoints"));
-  m.def("selective_scan_backward", &selective_scan_backward, "Selective scan backward",
-        py::arg("go"), py::arg("grad_final"), py::arg("u"), py::arg("delta"), py::arg("A"),
-        py::arg("B"), py::arg("C"), py::arg("skip"), py::arg("delta_bias"),
-        py::arg("checkpoints"), py::arg("lengths"), py::arg("softplus"), py::arg("want_state"));
+  m.def("selective_scan", &selective_scan, "Selective scan", py::arg("u"), py::arg("delta"),
+        py::arg("A"), py::arg("B"), py::arg("C"), py::arg("skip"), py::arg("delta_bias"),
+        py::arg("state"), py::arg("lengths"), py::arg("softplus"), py::arg("want_final"));
   m.def("selective_scan_step", &selective_scan_step, "Selective scan, one token", py::arg("u"),
         py::arg("delta"), py::arg("A"), py::arg("B"), py::arg("C"), py::arg("state"),
         py::arg("skip"), py::arg("delta_bias"), py::arg("softplus"));
-  m.def("block_norm_forward", &block_norm_forward, "Gate, norms and residual between blocks",
-        py::arg("x"), py::arg("residual"), py::arg("gate"), py::arg("post_weight"),
-        py::arg("post_bias"), py::arg("scale"), py::arg("pre_weight"), py::arg("pre_bias"),
-        py::arg("layer"), py::arg("eps"), py::arg("want_stats"));
-  m.def("block_norm_backward", &block_norm_backward, "Backward of block_norm_forward",
-        py::arg("grad_y"), py::arg("grad_residual_out"), py::arg("x"), py::arg("residual"),
-        py::arg("gate"), py::arg("post_weight"), py::arg("post_bias"), py::arg("scale"),
-        py::arg("pre_weight"), py::arg("pre_bias"), py::arg("stats"), py::arg("layer"));
+  m.def("block_norm", &block_norm, "Gate, norms and residual between blocks", py::arg("x"),
+        py::arg("residual"), py::arg("gate"), py::arg("post_weight"), py::arg("post_bias"),
+        py::arg("scale"), py::arg("pre_weight"), py::arg("pre_bias"), py::arg("layer"),
+        py::arg("eps"));
 }
 
 TORCH_LIBRARY(fused_source_conv_mixed, m) {

@@ -20,7 +20,9 @@ order: the same call gives the same bits.
 
 Inputs that are not contiguous are copied first; a state that a ``_step`` call updates must be
 contiguous. All work goes to the current stream of the inputs' device. The ``_step`` functions
-have no backward. Differentiating twice is refused.
+have no backward. A backward with ``create_graph`` is refused. A call can be captured into a CUDA graph,
+its backward too; as for any backward, no eager graph of the same leaves may be alive then (torch
+ends the capture otherwise), so drop earlier outputs first.
 
 The reference has no counterpart; these stand beside its operators and change none of them.
 """
@@ -29,7 +31,6 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import load_extension
 
@@ -38,53 +39,15 @@ _EXT = load_extension()
 _ACTIVATIONS = {"silu": True, None: False}
 
 
-def _contig(t):
-    return None if t is None else t.contiguous()
-
-
 def _silu(activation) -> bool:
     if activation not in _ACTIVATIONS:
         raise RuntimeError(f"activation must be 'silu' or None, got {activation!r}.")
     return _ACTIVATIONS[activation]
 
 
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _refuse_grad(name: str, *tensors) -> None:
-    if _wants_grad(*tensors):
-        raise RuntimeError(f"{name} has no backward: call it under torch.no_grad().")
-
-
 # ---------------------------------------------------------------------------------------
 # short causal conv
 # ---------------------------------------------------------------------------------------
-class FusedShortConvFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, initial_state, lengths, silu: bool, want_final: bool):
-        args = (x.contiguous(), weight.contiguous(), _contig(bias), _contig(initial_state),
-                _contig(lengths))
-        out = _EXT.short_conv_forward(*args, silu, want_final)
-        ctx.save_for_backward(*args)
-        ctx.silu = silu
-        ctx.set_materialize_grads(False)
-        return tuple(out) if want_final else out[0]
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out, grad_final=None):
-        x, weight, bias, state, lengths = ctx.saved_tensors
-        if grad_out is None and grad_final is None:
-            return (None,) * 7
-        grad_out = torch.zeros_like(x) if grad_out is None else grad_out.contiguous()
-        want_state = state is not None and ctx.needs_input_grad[3]
-        gx, gw, gb, gs = _EXT.short_conv_backward(grad_out, _contig(grad_final), x, weight, bias,
-                                                  state, lengths, ctx.silu, want_state)
-        return (gx, gw, gb if bias is not None else None, gs if want_state else None, None, None,
-                None)
-
-
 def fused_short_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
                      initial_state: torch.Tensor | None = None,
                      lengths: torch.Tensor | None = None, activation: str | None = "silu",
@@ -95,13 +58,8 @@ def fused_short_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor |
     ``initial_state [B,D,S-1]`` holds the inputs before position 0 (zeros without it). With
     ``return_final_state`` the result is ``(out, final_state)``, the state for the next chunk or
     for :func:`fused_short_conv_step`. Differentiable in all tensors but ``lengths``."""
-    silu = _silu(activation)
-    if _wants_grad(x, weight, bias, initial_state):
-        return FusedShortConvFunction.apply(x, weight, bias, initial_state, lengths, silu,
-                                            bool(return_final_state))
-    out = _EXT.short_conv_forward(x.contiguous(), weight.contiguous(), _contig(bias),
-                                  _contig(initial_state), _contig(lengths), silu,
-                                  bool(return_final_state))
+    out = _EXT.short_conv(x, weight, bias, initial_state, lengths, _silu(activation),
+                          bool(return_final_state))
     return tuple(out) if return_final_state else out[0]
 
 
@@ -110,9 +68,7 @@ def fused_short_conv_step(x: torch.Tensor, conv_state: torch.Tensor, weight: tor
                           activation: str | None = "silu") -> torch.Tensor:
     """One token of each sequence: ``x [B,D]`` -> ``[B,D]``; ``conv_state [B,D,S-1]`` takes the
     token in, in place."""
-    _refuse_grad("fused_short_conv_step", x, conv_state, weight, bias)
-    return _EXT.short_conv_step(x.contiguous(), conv_state, weight.contiguous(), _contig(bias),
-                                _silu(activation))
+    return _EXT.short_conv_step(x, conv_state, weight, bias, _silu(activation))
 
 
 class FusedShortConv1d(nn.Module):
@@ -154,38 +110,6 @@ class FusedShortConv1d(nn.Module):
 # ---------------------------------------------------------------------------------------
 # selective scan
 # ---------------------------------------------------------------------------------------
-class FusedSelectiveScanFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, u, delta, A, B, C, skip, delta_bias, initial_state, lengths,
-                delta_softplus: bool, want_final: bool):
-        u, delta, A, B, C = (t.contiguous() for t in (u, delta, A, B, C))
-        skip, delta_bias, lengths = _contig(skip), _contig(delta_bias), _contig(lengths)
-        y, final, ckpt = _EXT.selective_scan_forward(u, delta, A, B, C, skip, delta_bias,
-                                                     _contig(initial_state), lengths,
-                                                     delta_softplus, want_final, True)
-        ctx.save_for_backward(u, delta, A, B, C, skip, delta_bias, lengths, ckpt)
-        ctx.softplus = delta_softplus
-        ctx.set_materialize_grads(False)
-        return (y, final) if want_final else y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_y, grad_final=None):
-        u, delta, A, B, C, skip, delta_bias, lengths, ckpt = ctx.saved_tensors
-        if grad_y is None and grad_final is None:
-            return (None,) * 11
-        grad_y = torch.zeros_like(u) if grad_y is None else grad_y.contiguous()
-        grads = _EXT.selective_scan_backward(grad_y, _contig(grad_final), u, delta, A, B, C, skip,
-                                             delta_bias, ckpt, lengths, ctx.softplus,
-                                             ctx.needs_input_grad[7])
-        return (*grads, None, None, None)
-
-
-def _grouped(t: torch.Tensor, dims: int) -> torch.Tensor:
-    """``[B,N,L]`` (or ``[B,N]`` of one token) is one group."""
-    return t.unsqueeze(1) if t.dim() == dims - 1 else t
-
-
 def fused_selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
                          C: torch.Tensor, skip: torch.Tensor | None = None,
                          delta_bias: torch.Tensor | None = None, delta_softplus: bool = True,
@@ -199,16 +123,9 @@ def fused_selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, 
     for the next chunk or for :func:`fused_selective_scan_step`. Differentiable in all tensors
     but ``lengths``; a forward that will be differentiated keeps the states at every fourth
     position (``B D N L`` bytes)."""
-    B, C = _grouped(B, 4), _grouped(C, 4)
-    if _wants_grad(u, delta, A, B, C, skip, delta_bias, initial_state):
-        return FusedSelectiveScanFunction.apply(u, delta, A, B, C, skip, delta_bias,
-                                                initial_state, lengths, bool(delta_softplus),
-                                                bool(return_final_state))
-    y, final, _ = _EXT.selective_scan_forward(
-        u.contiguous(), delta.contiguous(), A.contiguous(), B.contiguous(), C.contiguous(),
-        _contig(skip), _contig(delta_bias), _contig(initial_state), _contig(lengths),
-        bool(delta_softplus), bool(return_final_state), False)
-    return (y, final) if return_final_state else y
+    out = _EXT.selective_scan(u, delta, A, B, C, skip, delta_bias, initial_state, lengths,
+                              bool(delta_softplus), bool(return_final_state))
+    return tuple(out) if return_final_state else out[0]
 
 
 def fused_selective_scan_step(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor,
@@ -218,11 +135,8 @@ def fused_selective_scan_step(u: torch.Tensor, delta: torch.Tensor, A: torch.Ten
                               delta_softplus: bool = True) -> torch.Tensor:
     """One token of each sequence: ``u``, ``delta`` ``[B,D]``, ``B``, ``C`` ``[B,G,N]`` (or
     ``[B,N]``) -> ``y [B,D]``; ``state [B,D,N]`` (fp32) is updated in place."""
-    B, C = _grouped(B, 3), _grouped(C, 3)
-    _refuse_grad("fused_selective_scan_step", u, delta, A, B, C, state, skip, delta_bias)
-    return _EXT.selective_scan_step(u.contiguous(), delta.contiguous(), A.contiguous(),
-                                    B.contiguous(), C.contiguous(), state, _contig(skip),
-                                    _contig(delta_bias), bool(delta_softplus))
+    return _EXT.selective_scan_step(u, delta, A, B, C, state, skip, delta_bias,
+                                    bool(delta_softplus))
 
 
 class FusedSelectiveScan1d(nn.Module):

@@ -263,6 +263,39 @@ def test_padding_holds_anything():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dt", ["fp32", "fp16", "bf16"])
+def test_steps_of_minus_infinity_pass_the_state(dt):
+    """delta at -infinity or at the type's lowest value is a step of zero: the state passes, the
+    gradients there are zero, and NaN is not made; a NaN in delta stays in its row."""
+    from dudyconv_b200.state_space import fused_selective_scan, fused_selective_scan_step
+
+    rng = _rng("low", dt)
+    B, D, L, N = 1, 8, 40, 16
+    t, r = _scan_inputs(B, D, L, N, 1, dt, rng)
+    go, gr = dev(rng.standard_normal((B, D, L)), dt)
+    de = t["delta"]
+    de[..., 10:14] = float("-inf")
+    de[..., 20:22] = torch.finfo(de.dtype).min
+    r["delta"] = de.double().cpu().numpy().clip(-1e4)  # exp(-1e4) is zero in float64 too
+    leaves = [t[k].requires_grad_(True) for k in t]
+    y = fused_selective_scan(t["u"], t["delta"], t["A"], t["B"], t["C"], t["skip"], t["delta_bias"], initial_state=t["state"])
+    grads = torch.autograd.grad(y, leaves, go)
+    ref, mag = (ss.selective_scan(r["u"], r["delta"], r["A"], r["B"], r["C"], r["skip"], r["delta_bias"], True, r["state"],
+                                  None, gr, None, mag=m) for m in (False, True))
+    check(y, ref[0], mag[0], L + 64, "y")
+    for k, g in zip(t, grads):
+        i = 2 + list(t).index(k)
+        check(g, ref[i], mag[i], L + 65, f"grad_{k}", dt)
+    with torch.no_grad():
+        h = t["state"].clone()
+        fused_selective_scan_step(t["u"][..., 0], de[..., 10], t["A"], t["B"][..., 0], t["C"][..., 0], h, t["skip"], t["delta_bias"])
+        assert torch.equal(h, t["state"])
+        de[0, 3, 5] = float("nan")
+        y = fused_selective_scan(t["u"], de, t["A"], t["B"], t["C"])
+        bad = y.isnan()[0]
+        assert bad[3, 5:].all() and not bad[3, :5].any() and not bad[:3].any() and not bad[4:].any()
+
+
 def test_strides_and_orders():
     """Slices of a projection, a transposed tensor and an expanded gradient are taken as they are."""
     from dudyconv_b200.state_space import fused_selective_scan, fused_short_conv
@@ -394,9 +427,8 @@ def test_refusals():
         with pytest.raises(RuntimeError, match=msg):
             call()
     u = x.clone().requires_grad_(True)
-    g = torch.autograd.grad(sp.fused_short_conv(u, w).sum(), u, create_graph=True)[0]
-    with pytest.raises(RuntimeError):
-        g.sum().backward()
+    with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
+        torch.autograd.grad(sp.fused_short_conv(u, w).sum(), u, create_graph=True)
 
 
 def test_modules():
