@@ -268,7 +268,7 @@ scan_bwd_kernel(Bwd a, Shape s) {
       for (int j = 0; j < ND; ++j)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float2 x = __fmul2_rn(dt[j], A[j][i]);
+          const float2 x = exponents<T>(dt[j], A[j][i]);
           const float2 e = make_float2(decay<T>(x.x), decay<T>(x.y));
           const float2 ci = i ? hi(cv) : lo(cv);
           dec[q][j][i] = e;

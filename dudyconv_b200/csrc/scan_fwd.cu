@@ -196,7 +196,7 @@ scan_fwd_kernel(Fwd a, Shape s) {
       for (int j = 0; j < kND; ++j)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float2 x = __fmul2_rn(both(j ? dt.y : dt.x), A[j][i]);
+          const float2 x = exponents<T>(both(j ? dt.y : dt.x), A[j][i]);
           const float2 e = make_float2(decay<T>(x.x), decay<T>(x.y));
           const float2 in = __fmul2_rn(both(j ? dt.w : dt.z), i ? hi(bv) : lo(bv));
           dec[q][j][i] = e;
@@ -402,7 +402,7 @@ scan_step_kernel(const T *__restrict__ u, const T *__restrict__ delta, const flo
       const int n = n0 + k;
       if (n >= s.N) break;
       float *h = state + row * s.N + n;
-      const float v = fmaf(decay<T>(dt * scaled<T>(A[d * s.N + n])), *h, du * ldf(Bm + bc + n));
+      const float v = fmaf(decay<T>(exponents<T>(both(dt), both(scaled<T>(A[d * s.N + n]))).x), *h, du * ldf(Bm + bc + n));
       *h = v;
       acc = fmaf(ldf(Cm + bc + n), v, acc);
     }
