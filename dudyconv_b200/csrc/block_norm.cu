@@ -671,29 +671,18 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, unsigned ntiles, bool vec) {
   }
 }
 
-// One column of threads per 32 channels: eight rows of threads take every eighth tile, then
-// the rows' sums are added in order.
+// The parameter gradients: the sum of the tiles' (or blocks') parts, 32 channels a block.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 block_norm_param_kernel(const float *__restrict__ part, T *g0, T *g1, T *g2, T *g3, T *g4,
                         int64_t tiles, int64_t D) {
-  __shared__ float red[8][32];
+  __shared__ float red[32][32];
   T *const outs[5] = {g0, g1, g2, g3, g4};
   T *out = outs[blockIdx.y];
   if (!out) return;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int64_t d = blockIdx.x * 32ll + tx;
-  const float *p = part + blockIdx.y * tiles * D;
-  float v = 0.f;
-  if (d < D)
-    for (int64_t i = ty; i < tiles; i += 8) v += p[i * D + d];
-  red[ty][tx] = v;
-  __syncthreads();
-  if (ty || d >= D) return;
-  v = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v += red[i][tx];
-  stf(out + d, v);
+  const int64_t d = blockIdx.x * 32ll + (threadIdx.x & 31);
+  const float v = column_sum<32>(part + blockIdx.y * tiles * D + d, tiles, D, d < D, red);
+  if (threadIdx.x < 32 && d < D) stf(out + d, v);
 }
 
 int validate(int64_t B, int64_t D, int64_t L, int dtype, int rdtype) {
@@ -803,7 +792,7 @@ template <typename T, typename R, bool LAYER>
 int bwd_launch(const NormBwd &a, const ParamGrads &g, const NormShape &s, cudaStream_t st) {
   if (int rc = bwd_main<T, R, LAYER>(a, s, st)) return rc;
   const dim3 pg((unsigned)cdiv(s.D, 32), 5);
-  block_norm_param_kernel<T><<<pg, 256, 0, st>>>(a.part, (T *)g.w1, (T *)g.w2, (T *)g.scale,
+  block_norm_param_kernel<T><<<pg, 1024, 0, st>>>(a.part, (T *)g.w1, (T *)g.w2, (T *)g.scale,
                                                   (T *)g.b1, (T *)g.b2,
                                                   part_count(s.B, s.D, s.L), s.D);
   return check_launch("block_norm_param_kernel");

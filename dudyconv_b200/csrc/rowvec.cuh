@@ -276,6 +276,29 @@ struct Scatter<STRIDE, 1, N, KEEP> {
   static __device__ __forceinline__ void sum(float *, int) {}
 };
 
+// The sum of p[i * stride], i < parts, of one of 32 columns a block of ROWS x 32 threads works on:
+// each row of threads takes every ROWS-th part, and the rows' sums are added in order. Returned to
+// row 0 (threadIdx.x < 32).
+template <int ROWS>
+__device__ __forceinline__ float column_sum(const float *p, int64_t parts, int64_t stride, bool in,
+                                            float (*red)[32]) {
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  float v = 0.f;
+  if (in) {
+#pragma unroll 4
+    for (int64_t i = ty; i < parts; i += ROWS) v += p[i * stride];
+  }
+  __syncthreads();
+  red[ty][tx] = v;
+  __syncthreads();
+  v = 0.f;
+  if (ty == 0) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) v += red[i][tx];
+  }
+  return v;
+}
+
 // ---- asynchronous 16-byte copies into shared memory ------------------------------------------
 __device__ __forceinline__ void cp_async16(void *smem, const void *gmem) {
   const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(smem));

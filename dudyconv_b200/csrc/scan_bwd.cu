@@ -1,43 +1,55 @@
 // scan_bwd.cu -- the selective scan's gradients: the sums over blocks, the choice of the kernel
 // and the C entry (the kernel is in scan_bwd.cuh).
+#include <algorithm>
+
 #include "scan_bwd.cuh"
 
 namespace dudy {
 namespace scan {
 namespace {
 
-// dB and dC: the sum of the channel blocks' parts, in order
+// What the blocks left in parts, added in order: dB and dC over the channel blocks (blockIdx.y 0
+// and 1), and dA, dskip and ddelta_bias over batch and chunks (blockIdx.y 2, 32 columns a block).
 template <typename T>
 __global__ void __launch_bounds__(256)
-scan_sum_parts_kernel(const float *__restrict__ pb, const float *__restrict__ pc,
-                      T *__restrict__ gb, T *__restrict__ gc, int64_t n, int64_t tiles) {
-  const float *p = blockIdx.y ? pc : pb;
-  T *out = blockIdx.y ? gc : gb;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    float v = 0.f;
-    for (int64_t k = 0; k < tiles; ++k) v += p[k * n + i];
-    stf(out + i, v);
-  }
-}
-
-// dA, dskip, ddelta_bias: the sum over batch and chunks, in order
-__global__ void __launch_bounds__(256)
-scan_param_kernel(const float *__restrict__ pa, const float *__restrict__ pd, float *ga,
-                  float *gskip, float *gbias, int64_t parts, int64_t D, int64_t N) {
-  const int64_t i = blockIdx.x * 256ll + threadIdx.x;
-  if (i < D * N) {
-    float v = 0.f;
-    for (int64_t b = 0; b < parts; ++b) v += pa[b * D * N + i];
-    ga[i] = v;
-  }
-  if (i < D) {
-    float v = 0.f, w = 0.f;
-    for (int64_t b = 0; b < parts; ++b) {
-      v += pd[b * D + i];
-      w += pd[(parts + b) * D + i];
+scan_sums_kernel(Bwd a, T *__restrict__ gB, T *__restrict__ gC, float *gA, float *gskip,
+                 float *gbias, int64_t n, int64_t tiles, int64_t parts, int64_t D, int64_t N) {
+  if (blockIdx.y < 2) {
+    const float *p = blockIdx.y ? a.part_c : a.part_b;
+    T *out = blockIdx.y ? gC : gB;
+    const bool four = n % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+    const int64_t step = gridDim.x * 256ll;
+    if (four) {
+      for (int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 4; i < n; i += step * 4) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int64_t k = 0; k < tiles; ++k) {
+          const float4 x = *reinterpret_cast<const float4 *>(p + k * n + i);
+          v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+        }
+        const float o[4] = {v.x, v.y, v.z, v.w};
+        row_store4(out, i, n, o, true);
+      }
+    } else {
+      for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += step) {
+        float v = 0.f;
+#pragma unroll 4
+        for (int64_t k = 0; k < tiles; ++k) v += p[k * n + i];
+        stf(out + i, v);
+      }
     }
-    if (gskip) gskip[i] = v;
-    if (gbias) gbias[i] = w;
+    return;
+  }
+  __shared__ float red[8][32];
+  const int64_t states = D * N, cols = states + 2 * D;
+  for (int64_t c0 = blockIdx.x * 32ll; c0 < cols; c0 += gridDim.x * 32ll) {
+    const int64_t c = c0 + (threadIdx.x & 31), d = c - states;
+    const float *p = c < states ? a.part_a + c : a.part_d + (d < D ? d : parts * D + d - D);
+    const float v = column_sum<8>(p, parts, c < states ? states : D, c < cols, red);
+    if (threadIdx.x >= 32 || c >= cols) continue;
+    if (c < states) gA[c] = v;
+    else if (d < D && gskip) gskip[d] = v;
+    else if (d >= D && gbias) gbias[d - D] = v;
   }
 }
 
@@ -54,9 +66,10 @@ int64_t channel_tiles(int64_t D, int64_t N, int64_t G, bool four) {
 }
 
 // as the forward's chunks, in whole stretches
+constexpr int kLeast = 4;
 int bwd_splits(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G, bool four, int64_t *chunk) {
   const int64_t blocks = B * G * channel_tiles(D, N, G, four);
-  const int64_t places = (four ? 1 : 2) * (int64_t)sm_count(), most = cdiv(L, kTS);
+  const int64_t places = (four ? 1 : 2) * (int64_t)sm_count(), most = cdiv(L, kLeast * kTS);
   int64_t n = blocks * 2 <= places ? places / blocks : 1;
   if (n > most) n = most;
   *chunk = cdiv(cdiv(L, n), kTS) * kTS;
@@ -89,13 +102,10 @@ struct Outs {
 template <typename T>
 int bwd_sums(const Bwd &a, const Outs &o, const Shape &s, int64_t tiles, cudaStream_t st) {
   const int64_t n = s.B * s.G * s.N * s.L, cap = 8 * (int64_t)sm_count();
-  const dim3 grid((unsigned)(cdiv(n, 256) < cap ? cdiv(n, 256) : cap), 2);
-  scan_sum_parts_kernel<T><<<grid, 256, 0, st>>>(a.part_b, a.part_c, (T *)o.gB, (T *)o.gC, n,
-                                                  tiles);
-  if (int rc = check_launch("scan_sum_parts_kernel")) return rc;
-  scan_param_kernel<<<(unsigned)cdiv(s.D * s.N, 256), 256, 0, st>>>(
-      a.part_a, a.part_d, o.gA, o.gskip, o.gbias, s.B * a.splits, s.D, s.N);
-  return check_launch("scan_param_kernel");
+  const int64_t want = std::max(cdiv(n, 1024), cdiv(s.D * s.N + 2 * s.D, 32));
+  scan_sums_kernel<T><<<dim3((unsigned)std::min(want, cap), 3), 256, 0, st>>>(
+      a, (T *)o.gB, (T *)o.gC, o.gA, o.gskip, o.gbias, n, tiles, s.B * a.splits, s.D, s.N);
+  return check_launch("scan_sums_kernel");
 }
 
 }  // namespace

@@ -345,7 +345,8 @@ int64_t fwd_blocks(const Shape &s) {
 }
 int fwd_splits(const Shape &s, int64_t *chunk) {
   const int64_t blocks = fwd_blocks(s), places = 2 * (int64_t)sm_count();
-  const int64_t most = cdiv(s.L, kWarps * kQ);  // a chunk has a piece for each of its warps
+  // two stretches a chunk at least, and four without a cut: the first kernel costs about two
+  const int64_t stretches = cdiv(s.L, kTS), most = stretches <= 4 ? 1 : cdiv(stretches, 2);
   int64_t n = blocks * 2 <= places ? places / blocks : 1;
   if (n > most) n = most;
   *chunk = cdiv(cdiv(s.L, n), kQ) * kQ;
