@@ -55,39 +55,21 @@ __device__ __forceinline__ int64_t clamp_len(const int32_t *lengths, int64_t b, 
   return n < 0 ? 0 : (n > L ? L : n);
 }
 
-// exp(dt A) as decay(dt * scaled(A)). 16-bit tensors: the base-2 exponential of the special
-// function unit on A log2(e) (relative error about 2^-22, against 2^-9 or 2^-12 of the result's
-// rounding); fp32 tensors: the accurate exponential.
-template <typename T>
-__device__ __forceinline__ float scaled(float a) {
-  return a * 1.4426950408889634f;
-}
-template <>
-__device__ __forceinline__ float scaled<float>(float a) {
-  return a;
-}
-template <typename T>
-__device__ __forceinline__ constexpr float unscaled() {
-  return sizeof(T) == 4 ? 1.f : 0.6931471805599453f;
-}
-template <typename T>
-__device__ __forceinline__ float decay(float x) {
-  return ex2(x);
-}
-template <>
-__device__ __forceinline__ float decay<float>(float x) {
-  return expf(x);
-}
-
-// The argument of decay() for a step dt. The 16-bit kernels' exponential is low by 0.6e-8 to 2e-8
-// of its value on average for exponents of -0.001 to -0.1 (measured against float64 on 2^20
-// arguments a range), and a bias, unlike the rounding around it, adds up over the hundreds of
-// positions that a slow state remembers: 2.4e-8 in the exponent centres it and divides the error
-// of dA (fp32) by three. At dt = 0 the result is still 1.
+// exp(dt A) as the base-2 exponential of the special function unit on dt A log2(e). Its rounding
+// error is 3e-8 to 6e-8 of the result (rms, that of an fp32 rounding), but it is low by 0.6e-8 to
+// 2e-8 on average for exponents of -0.001 to -0.1 (measured against float64 on 2^20 arguments a
+// range), and a bias, unlike the rounding around it, adds up over the hundreds of positions that a
+// slow state remembers. kCentre in the exponent takes it out; without it the error of dA was three
+// times as large. At dt = 0 the result is still 1. (The accurate expf cost the fp32 kernels five
+// more instructions a state and gave the same errors.)
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kCentre = 2.4e-8f;
-template <typename T>
-__device__ __forceinline__ float2 exponents(float2 dt, float2 a) {
-  return sizeof(T) == 4 ? __fmul2_rn(dt, a) : __ffma2_rn(dt, a, both(kCentre));
+__device__ __forceinline__ float decay(float dt, float a_log2e) {
+  return ex2(fmaf(dt, a_log2e, kCentre));
+}
+__device__ __forceinline__ float2 decays(float2 dt, float2 a_log2e) {
+  const float2 x = __ffma2_rn(dt, a_log2e, both(kCentre));
+  return make_float2(ex2(x.x), ex2(x.y));
 }
 
 // softplus(x) = max(x, 0) + log(1 + e), e = exp(-|x|), and its derivative. 16-bit tensors take
@@ -98,9 +80,9 @@ template <typename T>
 __device__ __forceinline__ float softplus(float x, float &slope) {
   // exp(-|x|) with the exponent's rounding put back (at |x| = 5 it is 3e-7); beyond 100 it is
   // zero, also for infinities and the types' lowest values, and NaN stays NaN
-  const float ax = fabsf(x) > 100.f ? 100.f : fabsf(x), t = -1.4426950408889634f * ax;
+  const float ax = fabsf(x) > 100.f ? 100.f : fabsf(x), t = -kLog2e * ax;
   float e = ex2(t);
-  e = fmaf(e, 0.6931471805599453f * fmaf(-1.4426950408889634f, ax, -t), e);
+  e = fmaf(e, kLn2 * fmaf(-kLog2e, ax, -t), e);
   const float s = e * rcp(2.f + e), q = s * s;
   float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
   p = fmaf(p, q, 1.f / 9.f);

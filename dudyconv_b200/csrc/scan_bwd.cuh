@@ -112,7 +112,7 @@ scan_bwd_kernel(Bwd a, Shape s) {
     for (int i = 0; i < kNS; ++i) {
       const bool ok = c0 + j < chans && n0 + i < s.N;
       const int64_t at = (row0 + c0 + j) * s.N + n0 + i;
-      av[i] = ok ? scaled<T>(a.A[(d0 + c0 + j) * s.N + n0 + i]) : 0.f;
+      av[i] = ok ? kLog2e * a.A[(d0 + c0 + j) * s.N + n0 + i] : 0.f;
       rv[i] = 0.f;
       if (!PRE && ok && warp == 0) {
         if (a.gfinal) rv[i] = a.gfinal[at];
@@ -268,8 +268,7 @@ scan_bwd_kernel(Bwd a, Shape s) {
       for (int j = 0; j < ND; ++j)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float2 x = exponents<T>(dt[j], A[j][i]);
-          const float2 e = make_float2(decay<T>(x.x), decay<T>(x.y));
+          const float2 e = decays(dt[j], A[j][i]);
           const float2 ci = i ? hi(cv) : lo(cv);
           dec[q][j][i] = e;
           own[j][i] = __fmul2_rn(
@@ -395,7 +394,7 @@ scan_bwd_kernel(Bwd a, Shape s) {
           const int at = q * CT + c0 + ln / kEach * kLeftN + i;
           const float gyj = m.go[at], uj = m.u[at];
           const float sbv = z[2 * i];
-          const float dd = fmaf(uj, sbv, z[2 * i + 1] * unscaled<T>()) * m.slope[at];
+          const float dd = fmaf(uj, sbv, z[2 * i + 1] * kLn2) * m.slope[at];
           m.u[at] = m.dt[at] * sbv;
           m.slope[at] = dd;
           dskip[i] = fmaf(gyj, uj, dskip[i]);

@@ -86,7 +86,7 @@ scan_fwd_kernel(Fwd a, Shape s) {
     for (int i = 0; i < kNS; ++i) {
       const bool ok = c0 + j < chans && n0 + i < s.N;
       const int64_t at = (row0 + c0 + j) * s.N + n0 + i, step = s.B * s.D * s.N;
-      av[i] = ok ? scaled<T>(a.A[(d0 + c0 + j) * s.N + n0 + i]) : 0.f;
+      av[i] = ok ? kLog2e * a.A[(d0 + c0 + j) * s.N + n0 + i] : 0.f;
       hv[i] = 0.f;
       if (!PRE && ok && warp == 0) {
         if (a.init) hv[i] = a.init[at];
@@ -196,8 +196,7 @@ scan_fwd_kernel(Fwd a, Shape s) {
       for (int j = 0; j < kND; ++j)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float2 x = exponents<T>(both(j ? dt.y : dt.x), A[j][i]);
-          const float2 e = make_float2(decay<T>(x.x), decay<T>(x.y));
+          const float2 e = decays(both(j ? dt.y : dt.x), A[j][i]);
           const float2 in = __fmul2_rn(both(j ? dt.w : dt.z), i ? hi(bv) : lo(bv));
           dec[q][j][i] = e;
           own[j][i] = q ? __ffma2_rn(e, own[j][i], in) : in;
@@ -403,7 +402,7 @@ scan_step_kernel(const T *__restrict__ u, const T *__restrict__ delta, const flo
       const int n = n0 + k;
       if (n >= s.N) break;
       float *h = state + row * s.N + n;
-      const float v = fmaf(decay<T>(exponents<T>(both(dt), both(scaled<T>(A[d * s.N + n]))).x), *h, du * ldf(Bm + bc + n));
+      const float v = fmaf(decay(dt, kLog2e * A[d * s.N + n]), *h, du * ldf(Bm + bc + n));
       *h = v;
       acc = fmaf(ldf(Cm + bc + n), v, acc);
     }
