@@ -555,6 +555,8 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, unsigned ntiles, bool vec) {
     }
     const Piece<float> &m1 = stat[buf][0][tid % TX], &inv1 = stat[buf][1][tid % TX];
     const Piece<float> &m2 = stat[buf][2][tid % TX], &inv2 = stat[buf][3][tid % TX];
+    const Two i1 = {inv1.pair(0), inv1.pair(1), inv1.pair(2), inv1.pair(3)};
+    const Two i2 = {inv2.pair(0), inv2.pair(1), inv2.pair(2), inv2.pair(3)};
     Two v, u;
 #pragma unroll
     for (int k = 0; k < kV / 2; ++k) v[k] = u[k] = both(0.f);
@@ -570,11 +572,11 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, unsigned ntiles, bool vec) {
           g = mul2(g, mul2(z, sigmoid2<T>(z)));
         }
         if (!ok) g = r = dy = both(0.f);
-        float2 h1 = mul2(LAYER ? add2(g, neg2(m1.pair(k))) : g, inv1.pair(k));
+        float2 h1 = mul2(LAYER ? add2(g, neg2(m1.pair(k))) : g, i1[k]);
         if (LAYER && !ok) h1 = both(0.f);
         float2 h2 = fma2(h1, both(sc[i] * w1[i]), r);
         if (LAYER) h2 = add2(h2, add2(both(sc[i] * b1[i]), neg2(m2.pair(k))));
-        h2 = mul2(h2, inv2.pair(k));
+        h2 = mul2(h2, i2[k]);
         if (LAYER && !ok) h2 = both(0.f);
         hat1[i][k] = h1;
         hat2[i][k] = h2;
@@ -606,7 +608,7 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, unsigned ntiles, bool vec) {
       for (int k = 0; k < kV / 2; ++k) {
         float2 o = fma2(hat2[i][k], c[k], mul2(m.gy[i][tid].pair(k), both(w2[i])));
         if (LAYER) o = add2(o, e[k]);
-        dr[k] = a.grout ? fma2(inv2.pair(k), o, m.gr[i][tid].pair(k)) : mul2(inv2.pair(k), o);
+        dr[k] = a.grout ? fma2(i2[k], o, m.gr[i][tid].pair(k)) : mul2(i2[k], o);
         if (!ok) dr[k] = both(0.f);
         const float2 d1 = mul2(dr[k], both(sc[i] * w1[i]));
         hat2[i][k] = d1;
@@ -635,7 +637,7 @@ block_norm_bwd_tile_kernel(NormBwd a, NormShape s, unsigned ntiles, bool vec) {
       for (int k = 0; k < kV / 2; ++k) {
         float2 o = fma2(hat1[i][k], c[k], hat2[i][k]);
         if (LAYER) o = add2(o, e[k]);
-        gx[k] = mul2(inv1.pair(k), o);
+        gx[k] = mul2(i1[k], o);
         if (a.gate) {
           const float2 z = m.z[i][tid].pair(k), sg = sigmoid2<T>(z), h = mul2(gx[k], sg);
           gx[k] = mul2(h, z);
@@ -824,6 +826,7 @@ int dudy_block_norm_forward(const void *x, const void *gate, const void *residua
   if (!x || !residual || !post_weight || !pre_weight || !y || !residual_out)
     return refuse("null tensor pointer");
   if (!layer && (post_bias || pre_bias)) return refuse("an rms norm has no bias.");
+  if (!(eps > 0.f)) return refuse("eps must be positive.");
   if (int rc = require_sm100()) return rc;
   const NormFwd a{x, gate, residual, post_weight, post_bias, scale, pre_weight, pre_bias, y,
                   residual_out, stats};

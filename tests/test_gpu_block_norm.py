@@ -161,6 +161,21 @@ def test_block_forward_and_backward():
         assert (a.double() - b).abs().max() <= 2 ** -11 * b.abs().max(), i
 
 
+def test_offsets_beyond_32_bits():
+    """Tokens behind the 2^31st element of the tensors, against the same tokens alone."""
+    from dudyconv_b200.block_norm import fused_gated_residual_norm as f
+
+    B, D, L = 3, 1024, (1 << 20) + 8
+    assert (B - 1) * D * L > 1 << 31
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(B, D, L, device="cuda", generator=g, dtype=torch.bfloat16)
+    w = torch.randn(D, device="cuda", generator=g, dtype=torch.bfloat16)
+    y, r = f(x, x, w, w)
+    tail = x[2:, :, -520:].contiguous()
+    y1, r1 = f(tail, tail, w, w)
+    assert torch.equal(y[2:, :, -520:], y1) and torch.equal(r[2:, :, -520:], r1)
+
+
 def test_module_and_capture():
     from dudyconv_b200.block_norm import FusedGatedResidualNorm1d
 

@@ -127,6 +127,10 @@ SCAN = [  # B, D, L, N, G, dtype, lengths, state, skip, delta_bias, softplus, of
     (2, 97, 75, 3, 1, "fp16", [75, 40], True, True, True, True, 0),
     (1, 24, 1000, 16, 1, "bf16", None, True, True, True, True, 0),
     (3, 24, 520, 24, 2, "fp32", [520, 33, 300], True, True, True, True, 0),
+    (2, 6, 70, 16, 6, "fp16", None, True, True, True, True, 0),  # a group for each channel
+    (16, 256, 40, 16, 1, "fp16", None, True, True, True, True, 0),  # channels enough for four to a thread
+    (7, 520, 33, 12, 1, "bf16", [33, 0, 1, 32, 31, 20, 7], True, True, True, True, 0),
+    (4, 1000, 37, 16, 1, "fp32", None, True, True, True, True, 1),
 ]
 
 
@@ -366,6 +370,102 @@ def test_other_stream_and_graph():
     cs.copy_(cs0), h.copy_(h0)
     for a, b in zip(got, step()):
         assert torch.equal(a, b)
+
+
+def test_lengths_beyond_the_batch_are_clamped():
+    from dudyconv_b200.state_space import fused_selective_scan, fused_short_conv
+
+    rng = _rng("clamp")
+    t, _ = _scan_inputs(3, 16, 50, 8, 1, "fp16", rng)
+    w, _ = dev(rng.standard_normal((16, 4)), "fp16")
+    res = []
+    for lengths in ([-5, 1 << 30, 20], [0, 50, 20]):
+        n = torch.tensor(lengths, device="cuda", dtype=torch.int32)
+        res.append([*fused_short_conv(t["u"], w, lengths=n, return_final_state=True),
+                    *fused_selective_scan(t["u"], t["delta"], t["A"], t["B"], t["C"], initial_state=t["state"], lengths=n,
+                                          return_final_state=True)])
+    for a, b in zip(*res):
+        assert torch.equal(a, b)
+
+
+def test_the_same_tensor_twice():
+    """u as delta and B as C: each gradient is the sum of its two."""
+    from dudyconv_b200.state_space import fused_selective_scan
+
+    rng = _rng("twice")
+    t, _ = _scan_inputs(2, 16, 33, 8, 1, "fp32", rng)
+    go, _ = dev(rng.standard_normal((2, 16, 33)), "fp32")
+    u, b = t["u"].requires_grad_(True), t["B"].requires_grad_(True)
+    gu, gb = torch.autograd.grad(fused_selective_scan(u, u, t["A"], b, b), [u, b], go)
+    four = [v.detach().clone().requires_grad_(True) for v in (u, u, b, b)]
+    g = torch.autograd.grad(fused_selective_scan(four[0], four[1], t["A"], four[2], four[3]), four, go)
+    assert torch.equal(gu, g[0] + g[1]) and torch.equal(gb, g[2] + g[3])
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on two streams give what they give alone."""
+    from dudyconv_b200.state_space import fused_selective_scan
+
+    rng = _rng("two")
+    sets = [_scan_inputs(2, 64, 700, 16, 1, "fp16", rng)[0] for _ in range(2)]
+
+    def run(t):
+        u = t["u"].detach().requires_grad_(True)
+        y = fused_selective_scan(u, t["delta"], t["A"], t["B"], t["C"], t["skip"], t["delta_bias"])
+        return y.detach(), *torch.autograd.grad(y, u, t["delta"])
+
+    want = [run(t) for t in sets]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] = run(sets[i])
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_c_abi():
+    """The C entries with a caller's buffers: results of the torch binding, nothing written beside
+    them, and the state of a step in place."""
+    from dudyconv_b200 import capi
+    from dudyconv_b200.state_space import fused_selective_scan, fused_short_conv, fused_short_conv_step
+
+    rng = _rng("capi")
+    B, D, L, N = 2, 40, 70, 16
+    t, _ = _scan_inputs(B, D, L, N, 1, "bf16", rng)
+    w, _ = dev(rng.standard_normal((D, 4)), "bf16")
+
+    def guarded(like, *shape):
+        buf = torch.full((like.numel() + 128,), 7.0, device="cuda", dtype=like.dtype)
+        return buf, buf[64:64 + like.numel()].view(shape or like.shape)
+
+    want, fin = fused_short_conv(t["u"], w, return_final_state=True)
+    buf, out = guarded(t["u"])
+    fbuf, f = guarded(fin)
+    capi.short_conv_forward(t["u"], w, None, None, None, out, f)
+    assert torch.equal(out, want) and torch.equal(f, fin)
+    assert (buf[:64] == 7).all() and (buf[-64:] == 7).all() and (fbuf[:64] == 7).all() and (fbuf[-64:] == 7).all()
+    st = fin.clone()
+    o = torch.empty(B, D, device="cuda", dtype=torch.bfloat16)
+    capi.short_conv_step(t["u"][..., 0].contiguous(), st, w, None, o)
+    st2 = fin.clone()
+    assert torch.equal(o, fused_short_conv_step(t["u"][..., 0], st2, w)) and torch.equal(st, st2)
+    y, h = fused_selective_scan(t["u"], t["delta"], t["A"], t["B"], t["C"], return_final_state=True)
+    need = capi.selective_scan_forward_workspace_size(t["u"], t["A"], t["B"])
+    ws = torch.full((need + 64,), 9, device="cuda", dtype=torch.uint8)
+    ybuf, yo = guarded(t["u"])
+    ck = torch.full((capi.selective_scan_checkpoint_bytes(t["u"], t["A"], t["B"]) + 64,), 9, device="cuda", dtype=torch.uint8)
+    capi.selective_scan_forward(t["u"], t["delta"], t["A"], t["B"], t["C"], None, None, None, None, yo, None, ck, ws)
+    assert torch.equal(yo, y) and (ybuf[:64] == 7).all() and (ybuf[-64:] == 7).all()
+    assert (ws[need:] == 9).all() and (ck[-64:] == 9).all()
+    if need:
+        with pytest.raises(capi.DudyError, match="workspace too small"):
+            capi.selective_scan_forward(t["u"], t["delta"], t["A"], t["B"], t["C"], None, None, None, None, yo, None, None,
+                                        ws[:need - 1])
+    assert capi.device_error() == 0
 
 
 def test_offsets_beyond_32_bits():
