@@ -241,6 +241,22 @@ __device__ __forceinline__ float sigmoid_for<float>(float v) {
   return 1.f / (1.f + expf(-v));
 }
 
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 neg2(float2 a) { return make_float2(-a.x, -a.y); }
+
+template <typename T>
+__device__ __forceinline__ float2 sigmoid2(float2 v) {
+  if constexpr (sizeof(T) == 4) {
+    return make_float2(sigmoid_for<T>(v.x), sigmoid_for<T>(v.y));
+  } else {
+    const float2 e = mul2(v, both(-1.4426950408889634f));
+    const float2 d = add2(make_float2(ex2(e.x), ex2(e.y)), both(1.f));
+    return make_float2(rcp(d.x), rcp(d.y));
+  }
+}
+
 // ---- sums across lanes ------------------------------------------------------------------------
 // Sums of n values each over the lanes that differ in the bits [STRIDE, STRIDE * LANES) of the
 // lane number. While there are several values, half of them go to the partner lane and half

@@ -71,9 +71,8 @@ __device__ __forceinline__ void window(const float (&x)[8], const float (&left)[
 
 // the row and segment of a warp; false: none
 __device__ __forceinline__ bool place(const ConvShape &s, int64_t &row, int &lo, int &hi) {
-  const unsigned seg = blockIdx.x % s.segs;
-  row = (int64_t)(blockIdx.x / s.segs) * kWarps + (threadIdx.x >> 5);
-  lo = (int)(seg * (unsigned)kSegT);
+  row = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  lo = (int)(blockIdx.y * (unsigned)kSegT);
   hi = lo + kSegT < s.L ? lo + (int)kSegT : (int)s.L;
   return row < s.rows;
 }
@@ -119,7 +118,11 @@ short_conv_fwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const T 
     }
     if (s.silu) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] *= sigmoid_for<T>(o[i]);
+      for (int i = 0; i < 8; i += 2) {
+        const float2 v = make_float2(o[i], o[i + 1]), p = mul2(v, sigmoid2<T>(v));
+        o[i] = p.x;
+        o[i + 1] = p.y;
+      }
     }
     if (t + 8 > len) {
 #pragma unroll
@@ -133,12 +136,11 @@ short_conv_fwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const T 
   }
 }
 
-// dv of one position from its pre-activation and the output's gradient
+// dv of two positions from their pre-activations and the output's gradients
 template <typename T>
-__device__ __forceinline__ float dv_of(float v, float go, int silu) {
-  if (!silu) return go;
-  const float sg = sigmoid_for<T>(v);
-  return go * (sg * fmaf(v, 1.f - sg, 1.f));
+__device__ __forceinline__ float2 dv_of(float2 v, float2 go) {
+  const float2 sg = sigmoid2<T>(v), rest = fma2(sg, both(-1.f), both(1.f));
+  return mul2(go, mul2(sg, fma2(v, rest, both(1.f))));
 }
 
 template <typename T, int S>
@@ -188,7 +190,7 @@ short_conv_bwd_kernel(const T *__restrict__ go, const T *__restrict__ gfinal,
         const int q = p - (S - 1) + j;
         v = fmaf(wt[j], q < 0 ? before<T, S>(sr, q) : ldf(xr + q), v);
       }
-      mine = dv_of<T>(v, ldf(gr + p), s.silu);
+      mine = s.silu ? dv_of<T>(both(v), both(ldf(gr + p))).x : ldf(gr + p);
     }
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) behind[i] = __shfl_sync(0xffffffffu, mine, i);
@@ -214,11 +216,16 @@ short_conv_bwd_kernel(const T *__restrict__ go, const T *__restrict__ gfinal,
       gs[b4].get(g);
       if (s.silu) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float v = bv;
+        for (int i = 0; i < 8; i += 2) {
+          float2 v = both(bv);
 #pragma unroll
-          for (int j = 0; j < S; ++j) v = fmaf(wt[j], xw[i + j], v);
-          dv[i] = dv_of<T>(v, g[i], 1);
+          for (int j = 0; j < S; ++j) {
+            v.x = fmaf(wt[j], xw[i + j], v.x);
+            v.y = fmaf(wt[j], xw[i + j + 1], v.y);
+          }
+          const float2 p = dv_of<T>(v, make_float2(g[i], g[i + 1]));
+          dv[i] = p.x;
+          dv[i + 1] = p.y;
         }
       } else {
 #pragma unroll
@@ -273,7 +280,7 @@ short_conv_bwd_kernel(const T *__restrict__ go, const T *__restrict__ gfinal,
     }
   }
   // part[(j * D + d) * per + b * segs + seg], j = S the bias
-  const int64_t per = s.rows / s.D * s.segs, at = (int64_t)b * s.segs + blockIdx.x % s.segs;
+  const int64_t per = s.rows / s.D * s.segs, at = (int64_t)b * s.segs + blockIdx.y;
 #pragma unroll
   for (int j = 0; j <= S; ++j) {
     float v = j < S ? dw[j] : db;
@@ -332,8 +339,8 @@ int validate(int64_t B, int64_t D, int64_t L, int64_t S, int dtype) {
     return refuse("S must be between 2 and " + std::to_string(DUDY_SHORT_CONV_MAX_TAPS) +
                   ", got " + std::to_string(S) + ".");
   if (!dtype_known(dtype)) return refuse("Unsupported dtype.");
-  if (L >= ((int64_t)1 << 30) || D >= ((int64_t)1 << 31) || B >= ((int64_t)1 << 31) ||
-      B * D >= ((int64_t)1 << 31) || cdiv(B * D, kWarps) * cdiv(L, kSegT) >= ((int64_t)1 << 31))
+  if (cdiv(L, kSegT) > 65535 || D >= ((int64_t)1 << 31) || B >= ((int64_t)1 << 31) ||
+      B * D >= ((int64_t)1 << 31))
     return refuse("tensor too large.");
   return DUDY_OK;
 }
@@ -357,7 +364,7 @@ struct BwdArgs {
 template <typename T, int S>
 int fwd_launch(const FwdArgs &a, ConvShape s, cudaStream_t st) {
   s.vec = s.L % 8 == 0 && aligned_to_16(a.x) && aligned_to_16(a.out);
-  short_conv_fwd_kernel<T, S><<<(unsigned)(cdiv(s.rows, kWarps) * s.segs), kWarps * 32, 0, st>>>(
+  short_conv_fwd_kernel<T, S><<<dim3((unsigned)cdiv(s.rows, kWarps), s.segs), kWarps * 32, 0, st>>>(
       (const T *)a.x, (const T *)a.w, (const T *)a.bias, (const T *)a.state, a.lengths,
       (T *)a.out, (T *)a.final_state, s);
   return check_launch("short_conv_fwd_kernel");
@@ -366,7 +373,7 @@ int fwd_launch(const FwdArgs &a, ConvShape s, cudaStream_t st) {
 template <typename T, int S>
 int bwd_launch(const BwdArgs &a, ConvShape s, cudaStream_t st) {
   s.vec = s.L % 8 == 0 && aligned_to_16(a.x) && aligned_to_16(a.go) && aligned_to_16(a.gx);
-  short_conv_bwd_kernel<T, S><<<(unsigned)(cdiv(s.rows, kWarps) * s.segs), kWarps * 32, 0, st>>>(
+  short_conv_bwd_kernel<T, S><<<dim3((unsigned)cdiv(s.rows, kWarps), s.segs), kWarps * 32, 0, st>>>(
       (const T *)a.go, (const T *)a.gfinal, (const T *)a.x, (const T *)a.w, (const T *)a.bias,
       (const T *)a.state, a.lengths, (T *)a.gx, (T *)a.gstate, a.part, s);
   if (int rc = check_launch("short_conv_bwd_kernel")) return rc;
