@@ -56,7 +56,7 @@ scan_sums_kernel(Bwd a, T *__restrict__ gB, T *__restrict__ gC, float *gA, float
 // ---- which kernel ----
 // Four channels to a thread where there are channels enough to give three quarters of the SMs a
 // block of them and N is 9 to 16: fewer shuffles and shared loads a state, but 255 registers and
-// one block an SM. B=16, D=256, L=4096, N=16, fp16: 435 us against 479; B=1: 70 against 66.
+// one block an SM. B=16, D=256, L=4096, N=16, fp16: 434 us against 479; B=1: 70 against 62.
 bool four_channels(int64_t B, int64_t D, int64_t N, int64_t G) {
   const int lpc = lanes_per_channel(N);
   return lpc == 4 && 4 * B * G * cdiv(D / G, 32 / lpc * 4) >= 3 * (int64_t)sm_count();
