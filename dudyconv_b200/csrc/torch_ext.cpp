@@ -13,6 +13,7 @@
 // allocated with the caching allocator, and all compute goes through the C ABI on the
 // current stream. A nonzero C-ABI status becomes a RuntimeError (TORCH_CHECK).
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 #include <torch/library.h>
@@ -583,12 +584,20 @@ void check_like(const OptTensor &t, const char *name, at::IntArrayRef sizes, at:
   if (t.has_value()) check_like(*t, name, sizes, dt, like);
 }
 
+// An output or scratch, straight from the caching allocator: through the dispatcher each cost
+// twice as much, and a backward makes up to ten.
+torch::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const torch::Tensor &like) {
+  return torch::Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+
+torch::Tensor fresh_like(const torch::Tensor &t) { return fresh(t.sizes(), t.scalar_type(), t); }
+
 torch::Tensor scratch(size_t bytes, const torch::Tensor &like) {
-  return torch::empty({(int64_t)std::max<size_t>(bytes, 16)}, like.options().dtype(torch::kUInt8));
+  return fresh({(int64_t)std::max<size_t>(bytes, 16)}, torch::kUInt8, like);
 }
 
 torch::Tensor floats(at::IntArrayRef sizes, const torch::Tensor &like) {
-  return torch::empty(sizes, like.options().dtype(torch::kFloat32));
+  return fresh(sizes, torch::kFloat32, like);
 }
 
 void check_seq(const torch::Tensor &x, const char *name) {
@@ -618,8 +627,8 @@ std::vector<torch::Tensor> short_conv_forward(torch::Tensor x, torch::Tensor w, 
   check_short_conv(x, w, bias, state, lengths);
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t B = x.size(0), D = x.size(1), L = x.size(2), S = w.size(1);
-  std::vector<torch::Tensor> out{torch::empty_like(x)};
-  if (want_final) out.push_back(torch::empty({B, D, S - 1}, x.options()));
+  std::vector<torch::Tensor> out{fresh_like(x)};
+  if (want_final) out.push_back(fresh({B, D, S - 1}, x.scalar_type(), x));
   check_status(dudy_short_conv_forward(
                    x.data_ptr(), w.data_ptr(), opt_ptr(bias), opt_ptr(state),
                    (const int32_t *)opt_ptr(lengths), out[0].data_ptr(),
@@ -639,9 +648,9 @@ std::vector<torch::Tensor> short_conv_backward(torch::Tensor go, OptTensor gfina
   check_like(go, "grad_out", x.sizes(), x.scalar_type(), x);
   check_like(gfinal, "grad_final_state", {B, D, S - 1}, x.scalar_type(), x);
   const c10::cuda::CUDAGuard guard(x.device());
-  auto gx = torch::empty_like(x), gw = torch::empty_like(w);
-  auto gb = torch::empty({bias.has_value() ? D : 0}, x.options());
-  auto gs = want_state ? torch::empty({B, D, S - 1}, x.options()) : torch::empty({0}, x.options());
+  auto gx = fresh_like(x), gw = fresh_like(w);
+  auto gb = fresh({bias.has_value() ? D : 0}, x.scalar_type(), x);
+  auto gs = want_state ? fresh({B, D, S - 1}, x.scalar_type(), x) : fresh({0}, x.scalar_type(), x);
   const int dt = dtype_code(x);
   auto ws = scratch(dudy_short_conv_backward_workspace_size(B, D, L, S, dt), x);
   check_status(dudy_short_conv_backward(
@@ -718,7 +727,7 @@ torch::Tensor short_conv_step(torch::Tensor x, torch::Tensor state, torch::Tenso
   check_like(bias, "bias", {D}, x.scalar_type(), x);
   check_like(state, "conv_state", {B, D, S - 1}, x.scalar_type(), x);
   const c10::cuda::CUDAGuard guard(x.device());
-  auto out = torch::empty_like(x);
+  auto out = fresh_like(x);
   check_status(dudy_short_conv_step(x.data_ptr(), state.data_ptr(), w.data_ptr(), opt_ptr(bias),
                                     out.data_ptr(), B, D, S, silu, dt, stream_ptr()),
                "fused_short_conv step");
@@ -773,7 +782,7 @@ std::vector<torch::Tensor> selective_scan_forward(torch::Tensor u, torch::Tensor
   check_like(lengths, "lengths", {d.B}, at::kInt, u);
   const c10::cuda::CUDAGuard guard(u.device());
   const int dt = dtype_code(u);
-  auto y = torch::empty_like(u);
+  auto y = fresh_like(u);
   auto fin = want_final ? floats({d.B, d.D, d.N}, u) : torch::Tensor();
   auto ck = want_ckpt
                 ? scratch(dudy_selective_scan_checkpoint_bytes(d.B, d.D, d.L, d.N, d.G, dt), u)
@@ -811,8 +820,8 @@ std::vector<torch::Tensor> selective_scan_backward(torch::Tensor go, OptTensor g
                       dudy_selective_scan_checkpoint_bytes(d.B, d.D, d.L, d.N, d.G, dt),
               "checkpoints do not belong to these inputs.");
   const c10::cuda::CUDAGuard guard(u.device());
-  auto gu = torch::empty_like(u), gd = torch::empty_like(u), gA = torch::empty_like(A);
-  auto gB = torch::empty_like(Bm), gC = torch::empty_like(Cm);
+  auto gu = fresh_like(u), gd = fresh_like(u), gA = fresh_like(A);
+  auto gB = fresh_like(Bm), gC = fresh_like(Cm);
   auto gs = skip.has_value() ? floats({d.D}, u) : torch::Tensor();
   auto gb = bias.has_value() ? floats({d.D}, u) : torch::Tensor();
   auto gst = want_state ? floats({d.B, d.D, d.N}, u) : torch::Tensor();
@@ -840,7 +849,7 @@ struct SelectiveScanFn : public torch::autograd::Function<SelectiveScanFn> {
                                torch::Tensor A, torch::Tensor Bm, torch::Tensor Cm,
                                OptTensor skip, OptTensor bias, OptTensor state,
                                OptTensor lengths, bool softplus, bool want_final) {
-    const auto bshape = Bm.sizes().vec(), cshape = Cm.sizes().vec();
+    const bool b3 = Bm.dim() == 3, c3 = Cm.dim() == 3;
     u = u.contiguous();
     delta = delta.contiguous();
     A = A.contiguous();
@@ -856,8 +865,8 @@ struct SelectiveScanFn : public torch::autograd::Function<SelectiveScanFn> {
                             or_undefined(lengths)});
     ctx->saved_data["softplus"] = softplus;
     ctx->saved_data["want_state"] = state.has_value() && state->requires_grad();
-    ctx->saved_data["bshape"] = bshape;
-    ctx->saved_data["cshape"] = cshape;
+    ctx->saved_data["b3"] = b3;
+    ctx->saved_data["c3"] = c3;
     ctx->set_materialize_grads(false);
     return want_final ? variable_list{r[0], r[1]} : variable_list{r[0]};
   }
@@ -873,8 +882,8 @@ struct SelectiveScanFn : public torch::autograd::Function<SelectiveScanFn> {
         or_none(v[5]), or_none(v[6]), v[7], or_none(v[8]), ctx->saved_data["softplus"].toBool(),
         ctx->saved_data["want_state"].toBool());
     for (size_t i = 0; i < r.size(); ++i) out[i] = r[i];
-    out[3] = out[3].view(ctx->saved_data["bshape"].toIntVector());
-    out[4] = out[4].view(ctx->saved_data["cshape"].toIntVector());
+    if (ctx->saved_data["b3"].toBool()) out[3] = out[3].squeeze(1);
+    if (ctx->saved_data["c3"].toBool()) out[4] = out[4].squeeze(1);
     return out;
   }
 };
@@ -909,7 +918,7 @@ torch::Tensor selective_scan_step(torch::Tensor u, torch::Tensor delta, torch::T
   const ScanDims d = check_scan(u, delta, A, Bm, Cm, skip, bias, true);
   check_like(state, "state", {d.B, d.D, d.N}, at::kFloat, u);
   const c10::cuda::CUDAGuard guard(u.device());
-  auto y = torch::empty_like(u);
+  auto y = fresh_like(u);
   check_status(dudy_selective_scan_step(
                    u.data_ptr(), delta.data_ptr(), (const float *)A.data_ptr(), Bm.data_ptr(),
                    Cm.data_ptr(), (const float *)opt_ptr(skip), (const float *)opt_ptr(bias),
@@ -944,7 +953,7 @@ std::vector<torch::Tensor> block_norm_forward(torch::Tensor x, torch::Tensor res
   check_block_norm(x, residual, gate, w1, b1, scale, w2, b2);
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t B = x.size(0), D = x.size(1), L = x.size(2);
-  auto y = torch::empty_like(x), rout = torch::empty_like(residual);
+  auto y = fresh_like(x), rout = fresh_like(residual);
   auto stats = want_stats ? floats({4, B, L}, x) : torch::Tensor();
   check_status(dudy_block_norm_forward(
                    x.data_ptr(), opt_ptr(gate), residual.data_ptr(), w1.data_ptr(), opt_ptr(b1),
@@ -969,12 +978,12 @@ std::vector<torch::Tensor> block_norm_backward(torch::Tensor gy, OptTensor grout
   check_like(stats, "stats", {4, B, L}, at::kFloat, x);
   const c10::cuda::CUDAGuard guard(x.device());
   auto like = [](const OptTensor &t) {
-    return t.has_value() ? torch::empty_like(*t) : torch::Tensor();
+    return t.has_value() ? fresh_like(*t) : torch::Tensor();
   };
   auto ptr = [](const torch::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
-  auto gx = torch::empty_like(x), gr = torch::empty_like(residual), gg = like(gate);
-  auto gw1 = torch::empty_like(w1), gb1 = like(b1), gsc = like(scale);
-  auto gw2 = torch::empty_like(w2), gb2 = like(b2);
+  auto gx = fresh_like(x), gr = fresh_like(residual), gg = like(gate);
+  auto gw1 = fresh_like(w1), gb1 = like(b1), gsc = like(scale);
+  auto gw2 = fresh_like(w2), gb2 = like(b2);
   const int dt = dtype_code(x), rdt = dtype_code(residual);
   auto ws = scratch(dudy_block_norm_backward_workspace_size(B, D, L, dt, rdt), x);
   check_status(dudy_block_norm_backward(
