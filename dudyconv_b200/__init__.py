@@ -8,7 +8,12 @@ Drop-in for the ``cuda_ops`` package of adjfangjiawei/DUDyConv:
 * ``cuda_ops_ext``            -- the compiled torch binding (built in-tree by
   ``dudyconv_b200.build``) over the C ABI of ``libdudyconv_b200.so``.
 
-``install_as_cuda_ops()`` registers both under the reference's import names
+* ``dudyconv_b200.state_space`` -- the selective state space scan and its short causal conv in
+  the same ``[B, D, L]`` layout, for training, prompts and single tokens (no counterpart there).
+* ``dudyconv_b200.block_norm``  -- the norms after and before a block with its gate, residual and
+  residual scale, one pass each way (no counterpart there).
+
+``install_as_cuda_ops()`` registers the first two under the reference's import names
 (``cuda_ops``, ``cuda_ops.fused_dynamic_conv``, ``cuda_ops.fused_source_conv_mixed``,
 ``cuda_ops_ext``) so unmodified callers such as ``backbone_dil_unshared.py`` use this
 implementation.
