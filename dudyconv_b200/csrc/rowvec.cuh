@@ -139,6 +139,7 @@ struct RowFour<float> {
     const uint4 q = *reinterpret_cast<const uint4 *>(p);
     w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
   }
+  __device__ __forceinline__ void load_shifted(const float *p, int) { load_all(p); }
   __device__ __forceinline__ void load_some(const float *p, int n) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = i < n ? reinterpret_cast<const uint32_t *>(p)[i] : 0u;
@@ -155,6 +156,13 @@ struct RowFour {
   __device__ __forceinline__ void load_all(const T *p) {
     const uint2 q = *reinterpret_cast<const uint2 *>(p);
     w[0] = q.x; w[1] = q.y;
+  }
+  // p[sh .. sh + 4), sh 0 or 1, from six elements
+  __device__ __forceinline__ void load_shifted(const T *p, int sh) {
+    const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
+    const uint32_t a = q[0], b = q[1], c = q[2];
+    w[0] = __funnelshift_r(a, b, 16 * sh);
+    w[1] = __funnelshift_r(b, c, 16 * sh);
   }
   __device__ __forceinline__ void load_some(const T *p, int n) {
     const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
@@ -194,6 +202,12 @@ __device__ __forceinline__ void row_store4(T *row, int64_t t, int64_t end, const
       RowFour<T> f;
       f.set(v);
       f.store_all(row + t);
+    }
+  } else if (sizeof(T) == 2 && t + 4 <= end) {
+    if constexpr (sizeof(T) == 2) {
+      RowFour<T> f;
+      f.set(v);
+      store_halves<2>(reinterpret_cast<uint16_t *>(row + t), f.w);
     }
   } else {
 #pragma unroll
@@ -319,6 +333,12 @@ __device__ __forceinline__ float column_sum(const float *p, int64_t parts, int64
 __device__ __forceinline__ void cp_async16(void *smem, const void *gmem) {
   const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(gmem) : "memory");
+}
+// `bytes` of four, the rest zero
+__device__ __forceinline__ void cp_async4(void *smem, const void *gmem, int bytes) {
+  const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(s), "l"(gmem), "r"(bytes)
+               : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>

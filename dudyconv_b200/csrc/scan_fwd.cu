@@ -56,8 +56,40 @@ struct FwdSmem {
   Ready ready;
 };
 
-// PRE: a chunk's end state from zero and its decay product only.
-template <typename T, int LPC, bool PRE>
+// Where rows do not all start on 16 bytes (odd lengths), a stretch comes in by words, as it lies in
+// memory: a 16-bit row that starts inside a word lies one element further on in its buffer
+// (row_shift), where the 16 bytes between rows have room for it. The threads of a row take
+// neighbouring words in turn. (fp32, B=5, D=256, L=1001: 47 us, 51 by elements, 43 at L=1000.)
+template <typename T>
+__device__ __forceinline__ int row_shift(const T *row) {
+  return sizeof(T) == 2 ? (int)(reinterpret_cast<uintptr_t>(row) >> 1) & 1 : 0;
+}
+template <int TS, typename T>  // TS: positions of a stretch
+__device__ __forceinline__ void row_words(T *raw, const RowCopy<T> &x, int64_t t0, int64_t end) {
+  constexpr int V = 16 / sizeof(T), E = 4 / sizeof(T), kRow = TS / V;
+  if (!x.src) return;
+  const T *row = x.src - x.c + t0;
+  T *to = raw + x.dst - x.c;
+  const int64_t rest = end - t0;
+  const int left = rest <= TS ? (int)rest : TS + 1;  // elements of the row that may be read
+  const int sh = row_shift(row), own = x.c / V;
+#pragma unroll
+  for (int k = 0; k < (E > 1 ? 5 : 4); ++k) {
+    if (k == 4 && (own || !sh)) break;
+    const int word = k < 4 ? k * kRow + own : TS / E, e = word * E - sh;
+    uint32_t *w = reinterpret_cast<uint32_t *>(to) + word;
+    if (left <= e) {
+      *w = 0u;
+    } else if (e < 0 && t0 == 0) {  // nothing of this row lies before it
+      *w = (uint32_t)*reinterpret_cast<const uint16_t *>(row) << 16;
+    } else {
+      cp_async4(w, row + e, left - e < E ? (left - e) * (int)sizeof(T) : 4);
+    }
+  }
+}
+
+// PRE: a chunk's end state from zero and its decay product only. VEC: all rows start on 16 bytes.
+template <typename T, int LPC, bool PRE, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2)
 scan_fwd_kernel(Fwd a, Shape s) {
   using Mine = FwdPiece<LPC>;
@@ -125,6 +157,10 @@ scan_fwd_kernel(Fwd a, Shape s) {
     const bool ok = i < Smem::ITEMS && r < (chan ? chans : s.N);
     return RowCopy<T>{ok ? base + r * s.L + c : nullptr, row * Smem::PITCH + c, c};
   };
+  // where row r of `rows` rows lies in its buffer
+  auto shift = [&](const T *base, int r, int rows) {
+    return r < rows ? row_shift(base) ^ (sizeof(T) == 2 ? r & (int)s.L & 1 : 0) : 0;
+  };
   constexpr int kKeep = Smem::EACH < kHeld ? Smem::EACH : kHeld;
   RowCopy<T> held[kKeep];
 #pragma unroll
@@ -134,9 +170,11 @@ scan_fwd_kernel(Fwd a, Shape s) {
       const int64_t t0 = from + (int64_t)st * kTS;
       T *raw = all.raw[st % kStages];
 #pragma unroll
-      for (int k = 0; k < Smem::EACH; ++k)
-        row_copy(raw, k < kKeep ? held[k < kKeep ? k : 0] : item(threadIdx.x + k * kThreads), t0,
-                 end, a.vec);
+      for (int k = 0; k < Smem::EACH; ++k) {
+        const RowCopy<T> x = k < kKeep ? held[k < kKeep ? k : 0] : item(threadIdx.x + k * kThreads);
+        if (VEC) row_copy(raw, x, t0, end, true);
+        else row_words<kTS>(raw, x, t0, end);
+      }
     }
     copies_commit();
   };
@@ -165,8 +203,14 @@ scan_fwd_kernel(Fwd a, Shape s) {
       const int i = lane + p * 32, d = i % CT, c = i / CT * 4;
       if (i >= CT * kQ / 4) break;
       RowFour<T> pu, pd;
-      pu.load_all(all.raw[buf] + d * Smem::PITCH + at + c);
-      pd.load_all(all.raw[buf] + (CT + d) * Smem::PITCH + at + c);
+      const T *src = all.raw[buf] + d * Smem::PITCH + at + c;
+      if (VEC) {
+        pu.load_all(src);
+        pd.load_all(src + CT * Smem::PITCH);
+      } else {
+        pu.load_shifted(src, shift(u, d, chans));
+        pd.load_shifted(src + CT * Smem::PITCH, shift(delta, d, chans));
+      }
       alignas(16) float yv[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -186,7 +230,9 @@ scan_fwd_kernel(Fwd a, Shape s) {
       const int i = lane + p * 32, r = i % (2 * NP), c = i / (2 * NP) * 4;
       if (i >= 2 * NP * kQ / 4) break;
       RowFour<T> pb;
-      pb.load_all(all.raw[buf] + (2 * CT + r) * Smem::PITCH + at + c);
+      const T *src = all.raw[buf] + (2 * CT + r) * Smem::PITCH + at + c;
+      if (VEC) pb.load_all(src);
+      else pb.load_shifted(src, r < NP ? shift(Bm, r, (int)s.N) : shift(Cm, r - NP, (int)s.N));
 #pragma unroll
       for (int j = 0; j < 4; ++j) m.bc[(c + j) * 2 * NP + r] = pb.get(j);
     }
@@ -307,6 +353,14 @@ scan_fwd_kernel(Fwd a, Shape s) {
       }
     }
     __syncwarp();
+    if (!VEC) {  // neighbouring lanes to neighbouring positions
+#pragma unroll 4
+      for (int i = lane; i < CT * kQ; i += 32) {
+        const int d = i / kQ, c = i % kQ;
+        if (d < chans && t0 + c < to) stf(y + d * s.L + t0 + c, t0 + c < end ? m.y[d * kYP + c] : 0.f);
+      }
+      continue;
+    }
 #pragma unroll
     for (int p = 0; p < Mine::UI; ++p) {
       const int i = lane + p * 32, d = i % CT, c = i / CT * 4;
@@ -315,7 +369,7 @@ scan_fwd_kernel(Fwd a, Shape s) {
       float o[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = t0 + c + j < end ? m.y[d * kYP + c + j] : 0.f;
-      row_store4(y + d * s.L, t0 + c, to, o, a.vec);
+      row_store4(y + d * s.L, t0 + c, to, o, true);
     }
   }
   if (!PRE) {  // padded positions behind the last piece
@@ -368,7 +422,8 @@ size_t fwd_workspace(const Shape &s) {
 template <typename T, int LPC>
 int fwd_launch(const Fwd &a, const Shape &s, cudaStream_t st) {
   const int smem = (int)sizeof(FwdSmem<T, LPC>);
-  auto main = scan_fwd_kernel<T, LPC, false>, pre = scan_fwd_kernel<T, LPC, true>;
+  auto main = a.vec ? scan_fwd_kernel<T, LPC, false, true> : scan_fwd_kernel<T, LPC, false, false>;
+  auto pre = a.vec ? scan_fwd_kernel<T, LPC, true, true> : scan_fwd_kernel<T, LPC, true, false>;
   const unsigned grid = (unsigned)(fwd_blocks(s) * a.splits);
   if (a.splits > 1) {
     if (set_smem_once((const void *)pre, smem) != cudaSuccess)

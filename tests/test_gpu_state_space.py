@@ -243,6 +243,45 @@ def test_prompt_then_tokens_is_the_whole_sequence(dt):
         assert (h[b] - hw[0]).abs().max() <= 4 * eps * hw.abs().max()
 
 
+@pytest.mark.parametrize("L", [63, 64, 65, 129, 191, 777])
+@pytest.mark.parametrize("dt", ["fp16", "bf16", "fp32"])
+def test_rows_that_start_inside_a_word(L, dt):
+    """Odd lengths and tensors that start on any element: the elements around a tensor and behind a
+    sequence's length (NaN here) are not used, and the bits are those of the same rows in a tensor
+    that starts on 16 bytes and has a length of whole words."""
+    from dudyconv_b200.state_space import fused_selective_scan
+
+    B, D, N, G = 2, 20, 6, 2
+    t, _ = _scan_inputs(B, D, L, N, G, dt, _rng("inside", L, dt))
+    lengths = torch.tensor([L, L // 2], device="cuda", dtype=torch.int32)
+    wide = (L + 7) // 8 * 8
+
+    def placed(v, off):
+        box = torch.full((v.numel() + off + 9,), float("nan"), device="cuda", dtype=v.dtype)
+        w = box[off:off + v.numel()].view(v.shape)
+        w.copy_(v)
+        for b, n in enumerate(lengths.tolist()):
+            w[b, ..., n:] = float("nan")
+        return w
+
+    def padded(v):
+        w = torch.zeros((*v.shape[:-1], wide), device="cuda", dtype=v.dtype)
+        w[..., :L] = v
+        return w
+
+    rows = ("u", "delta", "B", "C")
+    with torch.no_grad():
+        def call(u, delta, Bm, Cm):
+            return fused_selective_scan(u, delta, t["A"], Bm, Cm, t["skip"], t["delta_bias"], True, t["state"],
+                                        lengths, True)
+
+        y, h = call(*(padded(t[k]) for k in rows))
+        for offs in ((0, 0, 0, 0), (1, 0, 1, 0), (0, 1, 0, 1), (3, 2, 1, 5)):
+            y2, h2 = call(*(placed(t[k], o) for k, o in zip(rows, offs)))
+            assert torch.equal(y2, y[..., :L]), offs
+            assert torch.equal(h2, h), offs
+
+
 def test_padding_holds_anything():
     """Infinities and NaN at padded positions change nothing, forwards or backwards."""
     from dudyconv_b200.state_space import fused_selective_scan, fused_short_conv
