@@ -17,7 +17,7 @@
 // Waiting before the recurrence instead, and running it once, made the chain the bound: 222
 // and 861 us at the sizes below.
 // The special function unit (16 a clock and SM, 59 us for the 268 M exponentials of B=16,
-// D=256, L=4096, N=16) bounds the forward, not HBM (17 us).
+// D=256, L=4096, N=16) is the forward's floor, not HBM (17 us).
 //
 // Where there are too few rows of channels to fill the GPU, the sequence is cut into `splits`
 // chunks, a block to each: a first kernel finds each chunk's end state from zero and its decay

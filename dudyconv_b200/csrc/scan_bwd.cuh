@@ -22,8 +22,8 @@
 // 32 channels, one an SM), 62 us at B=1 in bf16 (818 with one block for the sequence). The floors
 // are 59 us of exponentials, 89 us of fp32 arithmetic (12 operations a state and position) and 60
 // us of HBM with the saved states. What it issues is 23 instructions a lane's state and position,
-// and eight warps an SM (255 registers a thread) fill 47% of the issue slots; the shared memory
-// pipe is at 54%. With the whole block on
+// and eight warps an SM (255 registers a thread) fill 45% of the issue slots; the shared memory
+// pipe is at 60%. With the whole block on
 // one piece, joined by barriers, it took 722 us.
 #pragma once
 

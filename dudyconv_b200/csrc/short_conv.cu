@@ -11,8 +11,8 @@
 //
 // The forward reads and writes each row once, the backward reads two rows and writes one: 67 and
 // 101 MB at B=16, D=256, L=4096 in fp16, 10.3 and 15.4 us of HBM at 6540 GB/s. They take 15.2 us
-// (4.4 TB/s, 68%) and 44 us with the parameter sums; the backward is bound by its instructions (45
-// an element with S = 4: 13 multiply-adds, the sigmoid, shuffles and conversions; 60% of the issue
+// (4.4 TB/s, 68%) and 44 us with the parameter sums; the backward is bound by its instructions (40
+// an element with S = 4: 13 multiply-adds, the sigmoid, shuffles and conversions; 54% of the issue
 // slots). Its multiply-adds two positions at a time (__ffma2_rn) took 91 registers for 80, and 50
 // us, or spilled, and 44; segments of 512 positions took 48. A warp takes up to 1024 positions of a row, 256 at a time, eight
 // to a lane (16-byte accesses); the S-1 <= 7 inputs before a lane's own come from the lane before
