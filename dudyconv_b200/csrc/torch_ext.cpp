@@ -553,11 +553,11 @@ OptTensor contig(const OptTensor &t) {
   return t.has_value() ? OptTensor(t->contiguous()) : t;
 }
 
+bool differentiated(const OptTensor &t) { return t.has_value() && t->requires_grad(); }
+
 template <typename... Ts>
 bool wants_grad(const Ts &...ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  auto one = [](const OptTensor &t) { return t.has_value() && t->requires_grad(); };
-  return (one(ts) || ...);
+  return at::GradMode::is_enabled() && (differentiated(ts) || ...);
 }
 
 // autograd's saved tensors: what was None comes back undefined
@@ -670,6 +670,8 @@ struct ShortConvFn : public torch::autograd::Function<ShortConvFn> {
   static variable_list forward(AutogradContext *ctx, torch::Tensor x, torch::Tensor w,
                                OptTensor bias, OptTensor state, OptTensor lengths, bool silu,
                                bool want_final) {
+    // asked before the copies: made without gradients, they no longer say what was given
+    const bool want_state = differentiated(state);
     x = x.contiguous();
     w = w.contiguous();
     bias = contig(bias);
@@ -679,7 +681,7 @@ struct ShortConvFn : public torch::autograd::Function<ShortConvFn> {
     ctx->save_for_backward(
         {x, w, or_undefined(bias), or_undefined(state), or_undefined(lengths)});
     ctx->saved_data["silu"] = silu;
-    ctx->saved_data["want_state"] = state.has_value() && state->requires_grad();
+    ctx->saved_data["want_state"] = want_state;
     ctx->set_materialize_grads(false);
     return out;
   }
@@ -850,6 +852,7 @@ struct SelectiveScanFn : public torch::autograd::Function<SelectiveScanFn> {
                                OptTensor skip, OptTensor bias, OptTensor state,
                                OptTensor lengths, bool softplus, bool want_final) {
     const bool b3 = Bm.dim() == 3, c3 = Cm.dim() == 3;
+    const bool want_state = differentiated(state);  // before the copies, as in the conv
     u = u.contiguous();
     delta = delta.contiguous();
     A = A.contiguous();
@@ -864,7 +867,7 @@ struct SelectiveScanFn : public torch::autograd::Function<SelectiveScanFn> {
     ctx->save_for_backward({u, delta, A, Bm, Cm, or_undefined(skip), or_undefined(bias), r[2],
                             or_undefined(lengths)});
     ctx->saved_data["softplus"] = softplus;
-    ctx->saved_data["want_state"] = state.has_value() && state->requires_grad();
+    ctx->saved_data["want_state"] = want_state;
     ctx->saved_data["b3"] = b3;
     ctx->saved_data["c3"] = c3;
     ctx->set_materialize_grads(false);
