@@ -13,7 +13,8 @@ PyTorch runs this as about ten passes over the tensors; here each direction read
 writes its outputs once. Statistics and sums are fp32; ``y`` is formed from ``residual_out``
 before its rounding. Gradients are sums in a fixed order: the same call gives the same bits.
 
-Inputs that are not contiguous are copied first. The reference has no counterpart.
+Inputs that are not contiguous are copied first. A backward with ``create_graph`` and an input that
+carries a forward-mode tangent are refused. The reference has no counterpart.
 """
 
 from __future__ import annotations

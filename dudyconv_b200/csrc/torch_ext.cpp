@@ -560,6 +560,14 @@ bool wants_grad(const Ts &...ts) {
   return at::GradMode::is_enabled() && (differentiated(ts) || ...);
 }
 
+// An output without a tangent would count inputs that carry one as constants.
+template <typename... Ts>
+void refuse_tangents(const char *what, const Ts &...ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  auto dual = [](const OptTensor &t) { return t.has_value() && t->_fw_grad(0).defined(); };
+  TORCH_CHECK(!(dual(ts) || ...), what, " has no forward-mode derivative.");
+}
+
 // autograd's saved tensors: what was None comes back undefined
 torch::Tensor or_undefined(const OptTensor &t) { return t.has_value() ? *t : torch::Tensor(); }
 OptTensor or_none(const torch::Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
@@ -706,6 +714,7 @@ struct ShortConvFn : public torch::autograd::Function<ShortConvFn> {
 std::vector<torch::Tensor> short_conv(torch::Tensor x, torch::Tensor w, OptTensor bias,
                                       OptTensor state, OptTensor lengths, bool silu,
                                       bool want_final) {
+  refuse_tangents("fused_short_conv", x, w, bias, state);
   if (wants_grad(x, w, bias, state))
     return ShortConvFn::apply(x, w, bias, state, lengths, silu, want_final);
   return short_conv_forward(x.contiguous(), w.contiguous(), contig(bias), contig(state),
@@ -714,6 +723,7 @@ std::vector<torch::Tensor> short_conv(torch::Tensor x, torch::Tensor w, OptTenso
 
 torch::Tensor short_conv_step(torch::Tensor x, torch::Tensor state, torch::Tensor w,
                               OptTensor bias, bool silu) {
+  refuse_tangents("fused_short_conv_step", x, state, w, bias);
   TORCH_CHECK(!wants_grad(x, state, w, bias),
               "fused_short_conv_step has no backward: call it under torch.no_grad().");
   x = x.contiguous();
@@ -896,6 +906,7 @@ std::vector<torch::Tensor> selective_scan(torch::Tensor u, torch::Tensor delta, 
                                           torch::Tensor Bm, torch::Tensor Cm, OptTensor skip,
                                           OptTensor bias, OptTensor state, OptTensor lengths,
                                           bool softplus, bool want_final) {
+  refuse_tangents("fused_selective_scan", u, delta, A, Bm, Cm, skip, bias, state);
   if (wants_grad(u, delta, A, Bm, Cm, skip, bias, state))
     return SelectiveScanFn::apply(u, delta, A, Bm, Cm, skip, bias, state, lengths, softplus,
                                   want_final);
@@ -909,6 +920,7 @@ std::vector<torch::Tensor> selective_scan(torch::Tensor u, torch::Tensor delta, 
 torch::Tensor selective_scan_step(torch::Tensor u, torch::Tensor delta, torch::Tensor A,
                                   torch::Tensor Bm, torch::Tensor Cm, torch::Tensor state,
                                   OptTensor skip, OptTensor bias, bool softplus) {
+  refuse_tangents("fused_selective_scan_step", u, delta, A, Bm, Cm, state, skip, bias);
   TORCH_CHECK(!wants_grad(u, delta, A, Bm, Cm, state, skip, bias),
               "fused_selective_scan_step has no backward: call it under torch.no_grad().");
   u = u.contiguous();
@@ -1036,6 +1048,7 @@ struct BlockNormFn : public torch::autograd::Function<BlockNormFn> {
 std::vector<torch::Tensor> block_norm(torch::Tensor x, torch::Tensor residual, OptTensor gate,
                                       torch::Tensor w1, OptTensor b1, OptTensor scale,
                                       torch::Tensor w2, OptTensor b2, bool layer, double eps) {
+  refuse_tangents("fused_gated_residual_norm", x, residual, gate, w1, b1, scale, w2, b2);
   if (wants_grad(x, residual, gate, w1, b1, scale, w2, b2))
     return BlockNormFn::apply(x, residual, gate, w1, b1, scale, w2, b2, layer, eps);
   auto r = block_norm_forward(x.contiguous(), residual.contiguous(), contig(gate),

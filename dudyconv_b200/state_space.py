@@ -20,7 +20,8 @@ order: the same call gives the same bits.
 
 Inputs that are not contiguous are copied first; a state that a ``_step`` call updates must be
 contiguous. All work goes to the current stream of the inputs' device. The ``_step`` functions
-have no backward. A backward with ``create_graph`` is refused. A call can be captured into a CUDA graph,
+have no backward. A backward with ``create_graph`` is refused, and so is an input that carries a
+forward-mode tangent. A call can be captured into a CUDA graph,
 its backward too; as for any backward, no eager graph of the same leaves may be alive then (torch
 ends the capture otherwise), so drop earlier outputs first.
 
