@@ -572,6 +572,12 @@ void refuse_tangents(const char *what, const Ts &...ts) {
 torch::Tensor or_undefined(const OptTensor &t) { return t.has_value() ? *t : torch::Tensor(); }
 OptTensor or_none(const torch::Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
+// A kernel wrote t through its pointer: a graph that kept t for its backward must not use it now.
+// (Tensors made in inference mode have no version and are kept by none.)
+void written(const torch::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // in a backward that is itself being recorded
 void refuse_twice(const char *what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " cannot be differentiated twice.");
@@ -743,6 +749,7 @@ torch::Tensor short_conv_step(torch::Tensor x, torch::Tensor state, torch::Tenso
   check_status(dudy_short_conv_step(x.data_ptr(), state.data_ptr(), w.data_ptr(), opt_ptr(bias),
                                     out.data_ptr(), B, D, S, silu, dt, stream_ptr()),
                "fused_short_conv step");
+  written(state);
   return out;
 }
 
@@ -940,6 +947,7 @@ torch::Tensor selective_scan_step(torch::Tensor u, torch::Tensor delta, torch::T
                    (float *)state.data_ptr(), y.data_ptr(), d.B, d.D, d.N, d.G, softplus,
                    dtype_code(u), stream_ptr()),
                "fused_selective_scan step");
+  written(state);
   return y;
 }
 
