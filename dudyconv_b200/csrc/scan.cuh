@@ -187,6 +187,12 @@ inline int validate(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G, int d
   return DUDY_OK;
 }
 
+// saved states go out and come back by 16 bytes where a channel's number of them allows it
+inline int require_checkpoints(const void *p, int64_t N) {
+  if (N % 4 != 0 || aligned_to_16(p)) return DUDY_OK;
+  return refuse("checkpoints must be 16-byte aligned.");
+}
+
 template <typename F>
 int by_type_and_lanes(int dtype, int64_t N, F &&f) {
   auto lanes = [&](auto t) {

@@ -136,6 +136,10 @@ int dudy_selective_scan_backward(const void *go, const float *grad_final, const 
   if (!go || !u || !delta || !A || !Bm || !Cm || !checkpoints || !grad_u || !grad_delta ||
       !grad_A || !grad_B || !grad_C)
     return refuse("null tensor pointer");
+  if (int rc = scan::require_checkpoints(checkpoints, N)) return rc;
+  // dB's and dC's parts go out and come back by 16 bytes where their number allows it
+  if (B * G * N * L % 4 == 0 && !aligned_to_16(workspace))
+    return refuse("workspace must be 16-byte aligned.");
   if (int rc = require_workspace(workspace, workspace_bytes,
                                  dudy_selective_scan_backward_workspace_size(B, D, L, N, G, dtype)))
     return rc;

@@ -329,7 +329,8 @@ DUDY_API int dudy_short_conv_step(const void *x, void *state, const void *weight
  *   dt = softplus(delta + delta_bias) (softplus != 0) or delta + delta_bias
  *   h[n] = exp(dt A[d,n]) h[n] + dt u Bm[n];   y = sum_n Cm[n] h[n] + skip u
  * 1 <= N <= DUDY_SCAN_MAX_STATE, D a multiple of G. `checkpoints` (or NULL) receives the states
- * that the backward starts from, dudy_selective_scan_checkpoint_bytes bytes. */
+ * that the backward starts from, dudy_selective_scan_checkpoint_bytes bytes. `checkpoints` and
+ * the backward's `workspace` must be 16-byte aligned. */
 #define DUDY_SCAN_MAX_STATE 64
 DUDY_API size_t dudy_selective_scan_checkpoint_bytes(int64_t B, int64_t D, int64_t L, int64_t N,
                                                      int64_t G, int dtype);
