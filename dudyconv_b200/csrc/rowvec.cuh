@@ -364,6 +364,11 @@ inline int require_sm100() {
                 "for sm_100a only", DUDY_ERR_DEVICE);
 }
 
+inline int require_apart(const void *state, const void *final_state) {
+  if (!state || state != final_state) return DUDY_OK;
+  return refuse("final_state must not be the initial state's memory.");
+}
+
 inline int require_workspace(const void *ws, size_t got, size_t need) {
   if (need == 0 || (ws && got >= need)) return DUDY_OK;
   return refuse("workspace too small: need " + std::to_string(need) + " bytes, got " +

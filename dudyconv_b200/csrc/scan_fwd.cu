@@ -506,6 +506,7 @@ int dudy_selective_scan_forward(const void *u, const void *delta, const float *A
   if (int rc = scan::validate(B, D, L, N, G, dtype)) return rc;
   if (!u || !delta || !A || !Bm || !Cm || !y) return refuse("null tensor pointer");
   if (int rc = scan::require_checkpoints(checkpoints, N)) return rc;
+  if (int rc = require_apart(state, final_state)) return rc;  // chunks' blocks read state when they start
   if (int rc = require_workspace(workspace, workspace_bytes,
                                  dudy_selective_scan_forward_workspace_size(B, D, L, N, G, dtype)))
     return rc;

@@ -433,6 +433,7 @@ int dudy_short_conv_forward(const void *x, const void *weight, const void *bias,
   clear_error();
   if (int rc = validate(B, D, L, S, dtype)) return rc;
   if (!x || !weight || !out) return refuse("null tensor pointer");
+  if (int rc = require_apart(state, final_state)) return rc;  // its lanes read entries that others write
   if (int rc = require_sm100()) return rc;
   const FwdArgs a{x, weight, bias, state, lengths, out, final_state};
   const ConvShape s{B * D, D, L, (unsigned)cdiv(L, kSegT), silu, 0};

@@ -297,6 +297,7 @@ DUDY_API int dudy_fscm_backward(const void *go, const void *x, const void *weigh
  * NULL) gives each sequence's length in a batch padded on the right, clamped to [0, L]:
  * positions at and behind it are not read, come out as zeros and carry no gradient, and the
  * final state is the one at the length. Each gradient is a sum in a fixed order (no atomics).
+ * No output may overlap an input or another output, except a step's state.
  * ======================================================================================== */
 
 /* ---- short causal depthwise conv ----

@@ -31,3 +31,14 @@ def test_buffers_start_on_16_bytes(call, name, offset):
     """The scan writes and reads saved states and partial sums 16 bytes at a time."""
     assert call(**{name: _at(offset)}) == capi.ERR_INVALID
     assert capi.last_error() == f"{name} must be 16-byte aligned."
+
+
+def test_a_final_state_is_not_the_initial_one():
+    """Blocks of a sequence's chunks read the initial state at times of their own, so the final state
+    cannot take its place."""
+    lib = capi.lib()
+    rc = lib.dudy_selective_scan_forward(F, F, F, F, F, None, None, _at(64), None, F, _at(64), None, F, 1 << 30, 1, 8, 4096, 16,
+                                         1, 1, 1, None)
+    assert rc == capi.ERR_INVALID and capi.last_error() == "final_state must not be the initial state's memory."
+    rc = lib.dudy_short_conv_forward(F, F, None, _at(64), None, F, _at(64), 1, 8, 4096, 4, 1, 1, None)
+    assert rc == capi.ERR_INVALID and capi.last_error() == "final_state must not be the initial state's memory."
