@@ -72,6 +72,12 @@ __device__ __forceinline__ float2 decays(float2 dt, float2 a_log2e) {
   return make_float2(ex2(x.x), ex2(x.y));
 }
 
+// What leaves a chunk: its decays' product times what enters, and its end from zero. A chunk of decays
+// above 1 may have a product beyond fp32; where nothing enters, nothing of it is passed on.
+__device__ __forceinline__ float pass_chunk(float prod, float in, float end) {
+  return in == 0.f ? end : fmaf(prod, in, end);
+}
+
 // softplus(x) = max(x, 0) + log(1 + e), e = exp(-|x|), and its derivative. 16-bit tensors take
 // log(1 + e) = 2 artanh(e / (2 + e)) by its power series: the argument is at most 1/3, so seven
 // terms leave 2^-26, and small steps keep their relative precision (the logarithm of a rounded

@@ -126,7 +126,7 @@ scan_bwd_kernel(Bwd a, Shape s) {
       if (!PRE && ok && warp == 0) {
         if (a.gfinal) rv[i] = a.gfinal[at];
         for (int k = a.splits - 1; k > split; --k)
-          rv[i] = fmaf(a.prod[k * nst + at], rv[i], a.rend[k * nst + at]);
+          rv[i] = pass_chunk(a.prod[k * nst + at], rv[i], a.rend[k * nst + at]);
       }
     }
     A[j][0] = make_float2(av[0], av[1]);

@@ -130,7 +130,8 @@ scan_fwd_kernel(Fwd a, Shape s) {
       hv[i] = 0.f;
       if (!PRE && ok && warp == 0) {
         if (a.init) hv[i] = a.init[at];
-        for (int k = 0; k < split; ++k) hv[i] = fmaf(a.prod[k * step + at], hv[i], a.end[k * step + at]);
+        for (int k = 0; k < split; ++k)
+          hv[i] = pass_chunk(a.prod[k * step + at], hv[i], a.end[k * step + at]);
       }
     }
     A[j][0] = make_float2(av[0], av[1]);

@@ -18,6 +18,9 @@ behind a sequence's length are not read, come out as zeros and carry no gradient
 state is the one at the length (0 gives the initial state back). Gradients are sums in a fixed
 order: the same call gives the same bits.
 
+States may grow (``dt A`` above zero): the decays' product over any eight positions, and over any
+stretch that a state or its gradient other than zero crosses, has to stay in fp32's range.
+
 Inputs that are not contiguous are copied first; a state that a ``_step`` call updates must be
 contiguous. All work goes to the current stream of the inputs' device. The ``_step`` functions
 have no backward. A backward with ``create_graph`` is refused, and so is an input that carries a
