@@ -134,16 +134,11 @@ template <>
 struct RowFour<float> {
   uint32_t w[4];
   __device__ __forceinline__ float get(int i) const { return __uint_as_float(w[i]); }
-  __device__ __forceinline__ float2 pair(int i) const { return make_float2(get(2 * i), get(2 * i + 1)); }
   __device__ __forceinline__ void load_all(const float *p) {
     const uint4 q = *reinterpret_cast<const uint4 *>(p);
     w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
   }
   __device__ __forceinline__ void load_shifted(const float *p, int) { load_all(p); }
-  __device__ __forceinline__ void load_some(const float *p, int n) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = i < n ? reinterpret_cast<const uint32_t *>(p)[i] : 0u;
-  }
 };
 template <typename T>
 struct RowFour {
@@ -152,7 +147,6 @@ struct RowFour {
     const uint16_t h = (uint16_t)(w[i >> 1] >> (i & 1 ? 16 : 0));
     return Elem<T>::to_f(*reinterpret_cast<const T *>(&h));
   }
-  __device__ __forceinline__ float2 pair(int i) const { return pair_of(w[i], T()); }
   __device__ __forceinline__ void load_all(const T *p) {
     const uint2 q = *reinterpret_cast<const uint2 *>(p);
     w[0] = q.x; w[1] = q.y;
@@ -164,11 +158,6 @@ struct RowFour {
     w[0] = __funnelshift_r(a, b, 16 * sh);
     w[1] = __funnelshift_r(b, c, 16 * sh);
   }
-  __device__ __forceinline__ void load_some(const T *p, int n) {
-    const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
-    w[0] = (n > 0 ? (uint32_t)h[0] : 0u) | (n > 1 ? (uint32_t)h[1] << 16 : 0u);
-    w[1] = (n > 2 ? (uint32_t)h[2] : 0u) | (n > 3 ? (uint32_t)h[3] << 16 : 0u);
-  }
   __device__ __forceinline__ void set(const float (&v)[4]) {
     w[0] = word_of(make_float2(v[0], v[1]), T());
     w[1] = word_of(make_float2(v[2], v[3]), T());
@@ -177,19 +166,6 @@ struct RowFour {
     *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
   }
 };
-
-// row[t .. t+4), zero at and behind `end`, which is not read. `vec`: rows and t start on four
-// elements.
-template <typename T>
-__device__ __forceinline__ void row_load4(RowFour<T> &f, const T *row, int64_t t, int64_t end,
-                                          bool vec) {
-  if (vec && t + 4 <= end) {
-    f.load_all(row + t);
-  } else {
-    const int64_t n = end - t;
-    f.load_some(row + t, n < 0 ? 0 : (n > 4 ? 4 : (int)n));
-  }
-}
 
 // row[t .. t+4) = v, before `end`
 template <typename T>
