@@ -97,7 +97,10 @@ def fscm_main(a):
 
 def state_space_main(a):
     """Forward and backward of one operator of the state-space block (short_conv,
-    selective_scan, block_norm) through the C ABI. Algorithmic bytes: each row tensor once."""
+    selective_scan, block_norm) through the C ABI. Algorithmic bytes: each row tensor once. Launches
+    rotate through sets of rows (and of B and C), so many that even a launch of two row tensors comes
+    back to its own after twice the L2's bytes: rows come from HBM. Saved states, statistics and partial
+    sums are one set, left where the launch before put them."""
     dev = torch.device("cuda")
     dt = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}[a.dtype]
     B, L, D, N, G, S = a.batch, a.seq, a.dim, a.state, a.groups, a.taps
@@ -109,8 +112,10 @@ def state_space_main(a):
     def scratch(nbytes):
         return torch.empty(max(256, nbytes), dtype=torch.uint8, device=dev)
 
-    rows = [[randn(B, D, L) for _ in range(5)] for _ in range(2)]
-    outs = [torch.empty(B, D, L, device=dev, dtype=dt) for _ in range(3)]
+    l2 = torch.cuda.get_device_properties(dev).L2_cache_size
+    sets = min(512, max(2, -(-l2 // (B * D * L * dt.itemsize))))
+    rows = [[randn(B, D, L) for _ in range(5)] for _ in range(sets)]
+    outs = [[torch.empty(B, D, L, device=dev, dtype=dt) for _ in range(3)] for _ in range(sets)]
     x0 = rows[0][0]
     if a.op == "short_conv":
         w, bias = randn(D, S, scale=S ** -0.5), randn(D)
@@ -119,15 +124,15 @@ def state_space_main(a):
         moved = {"forward": 2, "backward": 3}
 
         def launch(stage, i):
-            x, go = rows[i % 2][:2]
+            (x, go), o = rows[i % sets][:2], outs[i % sets]
             if stage == "forward":
-                capi.short_conv_forward(x, w, bias, None, None, outs[0])
+                capi.short_conv_forward(x, w, bias, None, None, o[0])
             else:
-                capi.short_conv_backward(go, None, x, w, bias, None, None, outs[1], gw, gb, None, ws)
+                capi.short_conv_backward(go, None, x, w, bias, None, None, o[1], gw, gb, None, ws)
     elif a.op == "selective_scan":
         A = -torch.arange(1, N + 1, device=dev, dtype=torch.float32).repeat(D, 1)
         skip, dbias = torch.ones(D, device=dev), torch.full((D,), -4.0, device=dev)
-        bc = [[randn(B, G, N, L) for _ in range(2)] for _ in range(2)]
+        bc = [[randn(B, G, N, L) for _ in range(2)] for _ in range(sets)]
         gA, gskip, gbias = torch.empty_like(A), torch.empty_like(skip), torch.empty_like(skip)
         gB, gC = torch.empty_like(bc[0][0]), torch.empty_like(bc[0][0])
         ck = scratch(capi.selective_scan_checkpoint_bytes(x0, A, bc[0][0]))
@@ -136,14 +141,14 @@ def state_space_main(a):
         moved = {"forward": 3, "forward_saving": 3, "backward": 5}
 
         def launch(stage, i):
-            u, de, go = rows[i % 2][:3]
-            Bm, Cm = bc[i % 2]
+            (u, de, go), o = rows[i % sets][:3], outs[i % sets]
+            Bm, Cm = bc[i % sets]
             if stage != "backward":
-                capi.selective_scan_forward(u, de, A, Bm, Cm, skip, dbias, None, None, outs[0], None,
+                capi.selective_scan_forward(u, de, A, Bm, Cm, skip, dbias, None, None, o[0], None,
                                             ck if stage == "forward_saving" else None, wf)
             else:
                 capi.selective_scan_backward(go, None, u, de, A, Bm, Cm, skip, dbias, ck, None,
-                                             outs[1], outs[2], gA, gB, gC, gskip, gbias, None, ws)
+                                             o[1], o[2], gA, gB, gC, gskip, gbias, None, ws)
     else:
         par = [randn(D) for _ in range(3)]
         gp = [torch.empty_like(p) for p in par]
@@ -152,23 +157,21 @@ def state_space_main(a):
         moved = {"forward": 5, "backward": 8}
 
         def launch(stage, i):
-            x, z, r, gy, gr = rows[i % 2]
+            (x, z, r, gy, gr), o = rows[i % sets], outs[i % sets]
             if stage == "forward":
-                capi.block_norm_forward(x, z, r, par[0], None, par[1], par[2], None, outs[0],
-                                        outs[1], stats)
+                capi.block_norm_forward(x, z, r, par[0], None, par[1], par[2], None, o[0], o[1], stats)
             else:
                 capi.block_norm_backward(gy, gr, x, z, r, par[0], None, par[1], par[2], stats,
-                                         outs[0], outs[1], outs[2], gp[0], None, gp[1], gp[2],
-                                         None, ws)
+                                         o[0], o[1], o[2], gp[0], None, gp[1], gp[2], None, ws)
 
     if a.profile:  # 4 launches of each pass, nothing timed
         for st in moved:
             for i in range(4):
                 launch(st, i)
         torch.cuda.synchronize()
-        print(json.dumps({"profile_launches": 4}))
+        print(json.dumps({"profile_launches": 4, "device_error": capi.device_error_info()}))
         return
-    res = {"op": a.op, "batch": B, "seq": L, "D": D, "N": N, "G": G, "S": S, "dtype": a.dtype}
+    res = {"op": a.op, "batch": B, "seq": L, "D": D, "N": N, "G": G, "S": S, "dtype": a.dtype, "sets": sets}
     for st, n in moved.items():
         for i in range(3):
             launch(st, i)
@@ -181,6 +184,7 @@ def state_space_main(a):
         torch.cuda.synchronize()
         us = e0.elapsed_time(e1) / a.iters * 1e3
         res[st] = {"us": round(us, 2), "GB/s": round(n * x0.numel() * x0.element_size() / us / 1e3, 1)}
+    res["device_error"] = capi.device_error_info()
     print(json.dumps(res))
 
 

@@ -28,6 +28,10 @@ forward-mode tangent. A call can be captured into a CUDA graph,
 its backward too; as for any backward, no eager graph of the same leaves may be alive then (torch
 ends the capture otherwise), so drop earlier outputs first.
 
+The scan's blocks wait for their own copies, for 2 s at most. A wait that ran out would leave wrong
+results and no exception: ``capi.device_error()`` tells of it, as for the framework's other operators,
+and ``capi.device_error_info()`` where it was.
+
 The reference has no counterpart; these stand beside its operators and change none of them.
 """
 
