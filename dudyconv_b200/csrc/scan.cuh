@@ -73,9 +73,13 @@ __device__ __forceinline__ float2 decays(float2 dt, float2 a_log2e) {
 }
 
 // What leaves a chunk: its decays' product times what enters, and its end from zero. A chunk of decays
-// above 1 may have a product beyond fp32; where nothing enters, nothing of it is passed on.
+// above 1 may have a product beyond fp32; where nothing enters, nothing of it is passed on. (Written
+// out as a selection: as a branch, each chunk's loads waited for the chunk before; 40 us instead of
+// 36 at B=1, D=256, L=4096, N=16.)
 __device__ __forceinline__ float pass_chunk(float prod, float in, float end) {
-  return in == 0.f ? end : fmaf(prod, in, end);
+  float v = fmaf(prod, in, end);
+  asm("{.reg .pred p; setp.eq.f32 p, %1, 0f00000000; selp.f32 %0, %2, %0, p;}" : "+f"(v) : "f"(in), "f"(end));
+  return v;
 }
 
 // softplus(x) = max(x, 0) + log(1 + e), e = exp(-|x|), and its derivative. 16-bit tensors take
