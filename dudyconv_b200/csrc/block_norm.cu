@@ -240,10 +240,11 @@ block_norm_bwd_any_kernel(NormBwd a, NormShape s) {
 // while they work on one, each thread's own pieces side by side (no thread reads another's, so its
 // own copies' completion is all it waits for). Arithmetic goes two tokens at a time (__ffma2_rn).
 // At B=16, D=256, L=4096 in fp16 with a gate, rms: 35 us forward (168 MB, 4.8 TB/s, 73% of a copy's
-// 6540 GB/s) and 78 us backward with the parameter sums (268 MB, 3.4 TB/s), bound by instructions:
-// two norms' sums, the gate's sigmoid twice and three parameter sums an element. Four tokens to a
-// thread, with twice the addresses and sums a token, took 62 and 107 us; re-reading the tile for
-// each sum, 462 in all.
+// 6540 GB/s) and 78 us backward with the parameter sums (268 MB, 3.4 TB/s). The backward's one block of
+// 512 threads an SM waits as a whole at each of a tile's barriers: the issue slots are 45% busy (two
+// norms' sums, the gate's sigmoid twice and three parameter sums an element), shared memory 54%, HBM
+// 52%. Four tokens to a thread, with twice the addresses and sums a token, took 62 and 107 us;
+// re-reading the tile for each sum, 462 in all.
 constexpr int kFwdThreads = 256, kBwdThreads = 512;
 constexpr int kV = 8;  // tokens of a thread
 

@@ -59,9 +59,12 @@ __device__ __forceinline__ int64_t clamp_len(const int32_t *lengths, int64_t b, 
 // error is 3e-8 to 6e-8 of the result (rms, that of an fp32 rounding), but it is low by 0.6e-8 to
 // 2e-8 on average for exponents of -0.001 to -0.1 (measured against float64 on 2^20 arguments a
 // range), and a bias, unlike the rounding around it, adds up over the hundreds of positions that a
-// slow state remembers. kCentre in the exponent takes it out; without it the error of dA was three
-// times as large. At dt = 0 the result is still 1. (The accurate expf cost the fp32 kernels five
-// more instructions a state and gave the same errors.)
+// slow state remembers. kCentre in the exponent, a relative 1.7e-8 (a fourth of a half rounding), takes
+// it out; without it the error of dA was three times as large. Outside that range: with the constant the
+// mean is 1.1e-8 too high for exponents above -0.001; below -0.5 the instruction is low by 5e-8 to
+// 7e-8, of which the constant takes 1.7e-8 back, but there a state halves every second position and
+// little adds up. At dt = 0 the result is still 1. (The accurate expf cost the fp32 kernels five more
+// instructions a state and gave the same errors.)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kCentre = 2.4e-8f;
 __device__ __forceinline__ float decay(float dt, float a_log2e) {
@@ -75,7 +78,8 @@ __device__ __forceinline__ float2 decays(float2 dt, float2 a_log2e) {
 // What leaves a chunk: its decays' product times what enters, and its end from zero. A chunk of decays
 // above 1 may have a product beyond fp32; where nothing enters, nothing of it is passed on. (Written
 // out as a selection: as a branch, each chunk's loads waited for the chunk before; 40 us instead of
-// 36 at B=1, D=256, L=4096, N=16.)
+// 36 at B=1, D=256, L=4096, N=16. A second, guarded pass where the first ends in NaN cost every
+// kernel registers: 1 to 7%.)
 __device__ __forceinline__ float pass_chunk(float prod, float in, float end) {
   float v = fmaf(prod, in, end);
   asm("{.reg .pred p; setp.eq.f32 p, %1, 0f00000000; selp.f32 %0, %2, %0, p;}" : "+f"(v) : "f"(in), "f"(end));

@@ -1,10 +1,11 @@
 // scan_fwd.cu -- the selective scan forward over whole sequences, and over one token.
 //
 // Measured with N = 16, D = 256, L = 4096: 179 us at B=16 in fp16 (197 when it saves the states
-// for the backward, 268 MB more to write), against 59 us of exponentials and 17 us of HBM; 35 us
+// for the backward, 268 MB more to write), against 59 us of exponentials and 17 us of HBM; 36 us
 // at B=1 in bf16 (111 with one block for the sequence). Its 256 blocks of 16 channels at B=16 leave
-// 40 SMs with one block where the others have two; issue slots and shared memory's return
-// bandwidth (every lane reads its positions' dt, dt u, B and C) bound those. A
+// 40 SMs with one block where the others have two; there the pipe of shared memory and L1 (every lane
+// reads its positions' dt, dt u, B and C; y goes out eight bytes a lane, along channels) is busiest,
+// at 67%, before the issue slots' 56% and the special function unit's 39%. A
 // recurrence costs two packed instructions a pair of states, so running it twice is cheap next to
 // the exponentials. With the whole block on one piece, joined by barriers, it took 280 us.
 #include "scan.cuh"

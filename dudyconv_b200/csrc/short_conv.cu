@@ -10,12 +10,14 @@
 // Positions at and behind a sequence's length are not read, give zeros and carry no gradient.
 //
 // The forward reads and writes each row once, the backward reads two rows and writes one: 67 and
-// 101 MB at B=16, D=256, L=4096 in fp16, 10.3 and 15.4 us of HBM at 6540 GB/s. They take 15.2 us
-// (4.4 TB/s, 68%) and 44 us with the parameter sums; the backward is bound by its instructions (40
-// an element with S = 4: 13 multiply-adds, the sigmoid, shuffles and conversions; 54% of the issue
-// slots). Its multiply-adds two positions at a time (__ffma2_rn) took 91 registers for 80, and 50
-// us, or spilled, and 44; segments of 512 positions took 48. A warp takes up to 1024 positions of a row, 256 at a time, eight
-// to a lane (16-byte accesses); the S-1 <= 7 inputs before a lane's own come from the lane before
+// 101 MB at B=16, D=256, L=4096 in fp16, 10.3 and 15.4 us of HBM at 6540 GB/s. With rows from HBM they
+// take 16.8 us (4.0 TB/s, 61%; the special function unit is 59% busy, the issue slots 61%) and 45 us
+// with the parameter sums. The backward waits for latency: all of a segment's loads come first,
+// then all its arithmetic, and 80 registers leave three blocks an SM (33% of the warps), so the issue
+// slots are 55% busy (40 instructions an element with S = 4) and HBM 34% (2.2 TB/s). Multiply-adds two
+// positions at a time (__ffma2_rn) took 91 registers and 13% more time, or spilled and won nothing;
+// segments of 512 positions took 9% more. A warp takes up to 1024 positions of a row, 256 at a time,
+// eight to a lane (16-byte accesses); the S-1 <= 7 inputs before a lane's own come from the lane before
 // it by shuffles, so no row is read twice, and all of a segment's loads are in flight at once.
 // The backward walks its positions from the right, because dx needs the S-1 values of dv behind
 // it: those come from the next lane, and at the right end of a block from the block done just
